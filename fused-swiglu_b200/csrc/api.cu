@@ -21,6 +21,7 @@
 #include "gemm_quad_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "host_slabs.h"
+#include "host_state.h"
 
 namespace fsw {
 
@@ -856,6 +857,19 @@ int mlp_impl(DeviceState& st, const void* x, int64_t ldx, const void* w_gate, co
 }
 
 }  // namespace
+
+namespace fsw {
+
+int current_device_sms(int* num_sms) {
+  DeviceState* st = nullptr;
+  if (int rc = device_state(&st)) return rc;
+  *num_sms = st->num_sms;
+  return FSWIGLU_OK;
+}
+
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+}  // namespace fsw
 
 extern "C" {
 

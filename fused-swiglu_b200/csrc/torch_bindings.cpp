@@ -13,6 +13,8 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <tuple>
+#include <vector>
 
 #include "fswiglu.h"
 
@@ -190,6 +192,277 @@ at::Tensor fused_swiglu_mlp_bf16_meta(at::Tensor const& x, at::Tensor const&, at
   return at::empty({x.size(0), W_down.size(0)}, x.options().dtype(fp32_out ? at::kFloat : at::kBFloat16));
 }
 
+// ---- training operators: norms with gradients, AdamW over many tensors, clipped gradient norm (include/fswiglu.h) ----
+
+namespace {
+
+int element_type(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, " must be a bfloat16 or float32 tensor");
+  return t.scalar_type() == at::kFloat ? FSWIGLU_OUT_F32 : FSWIGLU_OUT_BF16;
+}
+
+// A [M, d] operand of a norm, of x's type and on its device; its row pitch.
+int64_t norm_rows(const at::Tensor& t, const char* name, const at::Tensor& x) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 2 && t.sizes() == x.sizes(), name, " must be 2-D, of the shape of x");
+  TORCH_CHECK(t.scalar_type() == x.scalar_type() && t.device() == x.device(), name, " must have the type and device of x");
+  return row_pitch(t, name);
+}
+
+const void* norm_vector(const std::optional<at::Tensor>& v, const char* name, const at::Tensor& x) {
+  if (!v.has_value() || !v->defined()) return nullptr;
+  TORCH_CHECK(v->dim() == 1 && v->size(0) == x.size(1) && v->is_contiguous() && v->device() == x.device(), name,
+              " must be a contiguous vector of x's row length on the device of x");
+  return v->data_ptr();
+}
+
+int norm_vector_type(const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias, const at::Tensor& x) {
+  const bool w = weight.has_value() && weight->defined(), b = bias.has_value() && bias->defined();
+  if (w && b) TORCH_CHECK(weight->scalar_type() == bias->scalar_type(), "weight and bias must have one type");
+  return w ? element_type(*weight, "weight") : b ? element_type(*bias, "bias") : element_type(x, "x");
+}
+
+const float* norm_statistic(const at::Tensor& t, const char* name, const at::Tensor& x) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 1 && t.size(0) == x.size(0) &&
+                  t.is_contiguous(),
+              name, " must be a contiguous float32 vector with one entry per row of x, on the device of x");
+  return t.data_ptr<float>();
+}
+
+at::Tensor like_rows(const at::Tensor& x) { return at::empty({x.size(0), x.size(1)}, x.options()); }
+
+struct NormGradients {
+  at::Tensor dx, dweight, dbias;
+};
+
+NormGradients norm_backward(bool layer, at::Tensor const& dout, at::Tensor const& x, const at::Tensor* mean,
+                            at::Tensor const& rstd, std::optional<at::Tensor> const& weight,
+                            std::optional<at::Tensor> const& residual, bool fp32_grads, bool weight_grad, bool bias_grad) {
+  const int64_t ldx = norm_rows(x, "x", x), ld_dout = norm_rows(dout, "dout", x);
+  const int xt = element_type(x, "x"), wt = norm_vector_type(weight, std::nullopt, x);
+  const void* w = norm_vector(weight, "weight", x);
+  const bool res = residual.has_value() && residual->defined();
+  const int64_t ld_res = res ? norm_rows(*residual, "residual", x) : 0;
+  const float* m = layer ? norm_statistic(*mean, "mean", x) : nullptr;
+  const float* r = norm_statistic(rstd, "rstd", x);
+  const int64_t M = x.size(0), d = x.size(1);
+  const c10::cuda::OptionalCUDAGuard guard(device_of(x));
+  const int gt = fp32_grads ? FSWIGLU_OUT_F32 : wt;
+  const auto grads = x.options().dtype(gt == FSWIGLU_OUT_F32 ? at::kFloat : at::kBFloat16);
+  NormGradients g;
+  g.dx = like_rows(x);
+  if (w != nullptr && weight_grad) g.dweight = at::empty({d}, grads);
+  if (bias_grad) g.dbias = at::empty({d}, grads);
+  at::Tensor ws;
+  size_t bytes = 0;
+  if ((g.dweight.defined() || g.dbias.defined()) && M > 0) {
+    bytes = fswiglu_norm_backward_workspace_bytes(M, d);
+    ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  }
+  void* dw = g.dweight.defined() ? g.dweight.data_ptr() : nullptr;
+  void* db = g.dbias.defined() ? g.dbias.data_ptr() : nullptr;
+  void* wsp = ws.defined() ? ws.data_ptr() : nullptr;
+  const void* resp = res ? residual->data_ptr() : nullptr;
+  if (layer) {
+    check_status(fswiglu_layer_norm_backward(dout.data_ptr(), ld_dout, x.data_ptr(), ldx, m, r, w, resp, ld_res,
+                                             g.dx.data_ptr(), d, dw, db, M, d, xt, wt, gt, wsp, bytes, current_stream(x)),
+                 "layer_norm_backward");
+  } else {
+    check_status(fswiglu_rms_norm_backward(dout.data_ptr(), ld_dout, x.data_ptr(), ldx, r, w, resp, ld_res,
+                                           g.dx.data_ptr(), d, dw, M, d, xt, wt, gt, wsp, bytes, current_stream(x)),
+                 "rms_norm_backward");
+  }
+  return g;
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward(at::Tensor const& x, std::optional<at::Tensor> const& weight,
+                                                                  std::optional<at::Tensor> const& bias, double eps) {
+  const int64_t ldx = norm_rows(x, "x", x), M = x.size(0), d = x.size(1);
+  const int xt = element_type(x, "x"), wt = norm_vector_type(weight, bias, x);
+  const void* w = norm_vector(weight, "weight", x);
+  const void* b = norm_vector(bias, "bias", x);
+  const c10::cuda::OptionalCUDAGuard guard(device_of(x));
+  at::Tensor y = like_rows(x), mean = at::empty({M}, x.options().dtype(at::kFloat)),
+             rstd = at::empty({M}, x.options().dtype(at::kFloat));
+  check_status(fswiglu_layer_norm_forward(x.data_ptr(), ldx, w, b, y.data_ptr(), d, mean.data_ptr<float>(),
+                                          rstd.data_ptr<float>(), M, d, xt, wt, static_cast<float>(eps), current_stream(x)),
+               "layer_norm_forward");
+  return {y, mean, rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_forward(at::Tensor const& x, std::optional<at::Tensor> const& weight, double eps) {
+  const int64_t ldx = norm_rows(x, "x", x), M = x.size(0), d = x.size(1);
+  const int xt = element_type(x, "x"), wt = norm_vector_type(weight, std::nullopt, x);
+  const void* w = norm_vector(weight, "weight", x);
+  const c10::cuda::OptionalCUDAGuard guard(device_of(x));
+  at::Tensor y = like_rows(x), rstd = at::empty({M}, x.options().dtype(at::kFloat));
+  check_status(fswiglu_rms_norm_forward(x.data_ptr(), ldx, w, y.data_ptr(), d, rstd.data_ptr<float>(), M, d, xt, wt,
+                                        static_cast<float>(eps), current_stream(x)),
+               "rms_norm_forward");
+  return {y, rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(at::Tensor const& dout, at::Tensor const& x,
+                                                                   at::Tensor const& mean, at::Tensor const& rstd,
+                                                                   std::optional<at::Tensor> const& weight, bool bias_grad,
+                                                                   std::optional<at::Tensor> const& residual,
+                                                                   bool fp32_grads, bool weight_grad) {
+  NormGradients g = norm_backward(true, dout, x, &mean, rstd, weight, residual, fp32_grads, weight_grad, bias_grad);
+  return {g.dx, g.dweight, g.dbias};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_backward(at::Tensor const& dout, at::Tensor const& x, at::Tensor const& rstd,
+                                                     std::optional<at::Tensor> const& weight,
+                                                     std::optional<at::Tensor> const& residual, bool fp32_grads,
+                                                     bool weight_grad) {
+  NormGradients g = norm_backward(false, dout, x, nullptr, rstd, weight, residual, fp32_grads, weight_grad, false);
+  return {g.dx, g.dweight};
+}
+
+namespace {
+
+// One list of a step over many tensors: as many entries as parameters, each contiguous, of one type, on one device.
+void check_list(at::TensorList list, at::TensorList params, at::ScalarType type, const char* name) {
+  TORCH_CHECK(list.size() == params.size(), name, " must have one tensor for each parameter");
+  const auto device = params[0].device();
+  for (size_t i = 0; i < list.size(); ++i) {
+    TORCH_CHECK(list[i].scalar_type() == type, name, " must all be ", type, " tensors");
+    TORCH_CHECK(list[i].device() == device, name, " must all be on the device of the parameters");
+    TORCH_CHECK(list[i].is_contiguous(), name, " must all be contiguous");
+  }
+}
+
+const void* scalar_on_device(const std::optional<at::Tensor>& t, at::ScalarType type, const at::Tensor& p, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->scalar_type() == type && t->numel() == 1 && t->device() == p.device(), name, " must be one ", type,
+              " element on the device of the parameters");
+  return t->data_ptr();
+}
+
+}  // namespace
+
+void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs, int64_t step,
+                double lr, double beta1, double beta2, double eps, double weight_decay, at::TensorList masters,
+                at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, std::optional<at::Tensor> const& grad_scale,
+                int64_t seed, std::optional<at::Tensor> const& lr_tensor, std::optional<at::Tensor> const& step_tensor) {
+  if (params.empty()) {
+    TORCH_CHECK(grads.empty() && exp_avgs.empty() && exp_avg_sqs.empty(), "the lists must be of one length");
+    return;
+  }
+  const at::Tensor& p0 = params[0];
+  TORCH_CHECK(p0.is_cuda(), "params must be CUDA tensors");
+  TORCH_CHECK(grads.size() == params.size() && exp_avgs.size() == params.size(), "the lists must be of one length");
+  const int pt = element_type(p0, "params"), gt = element_type(grads[0], "grads");
+  const bool eight = exp_avgs[0].scalar_type() == at::kFloat8_e4m3fn;
+  check_list(params, params, p0.scalar_type(), "params");
+  check_list(grads, params, grads[0].scalar_type(), "grads");
+  check_list(exp_avgs, params, eight ? at::kFloat8_e4m3fn : at::kFloat, "exp_avgs");
+  check_list(exp_avg_sqs, params, eight ? at::kFloat8_e5m2 : at::kFloat, "exp_avg_sqs");
+  if (!masters.empty()) {
+    TORCH_CHECK(pt == FSWIGLU_OUT_BF16, "masters go with bfloat16 params");
+    check_list(masters, params, at::kFloat, "masters");
+  }
+  if (eight) {
+    check_list(exp_avg_scales, params, at::kFloat, "exp_avg_scales");
+    check_list(exp_avg_sq_scales, params, at::kFloat, "exp_avg_sq_scales");
+  } else {
+    TORCH_CHECK(exp_avg_scales.empty() && exp_avg_sq_scales.empty(), "scales go with 8-bit moments");
+  }
+  std::vector<fswiglu_adamw_tensor> table(params.size());
+  for (size_t i = 0; i < params.size(); ++i) {
+    const int64_t n = params[i].numel();
+    TORCH_CHECK(grads[i].numel() == n && exp_avgs[i].numel() == n && exp_avg_sqs[i].numel() == n &&
+                    (masters.empty() || masters[i].numel() == n),
+                "tensor ", i, ": parameter, gradient, moments and master must have as many elements");
+    if (eight) {
+      TORCH_CHECK(exp_avg_scales[i].numel() == (n + 255) / 256 && exp_avg_sq_scales[i].numel() == (n + 255) / 256, "tensor ",
+                  i, ": scales must have one element for each 256 of the parameter");
+    }
+    table[i] = {params[i].data_ptr(),
+                grads[i].data_ptr(),
+                exp_avgs[i].data_ptr(),
+                exp_avg_sqs[i].data_ptr(),
+                masters.empty() ? nullptr : masters[i].data_ptr<float>(),
+                eight ? exp_avg_scales[i].data_ptr<float>() : nullptr,
+                eight ? exp_avg_sq_scales[i].data_ptr<float>() : nullptr,
+                n};
+  }
+  fswiglu_adamw_options o = {};
+  o.lr = lr;
+  o.beta1 = beta1;
+  o.beta2 = beta2;
+  o.eps = eps;
+  o.weight_decay = weight_decay;
+  o.step = step;
+  o.seed = static_cast<uint64_t>(seed);
+  o.lr_device = static_cast<const float*>(scalar_on_device(lr_tensor, at::kFloat, p0, "lr_tensor"));
+  o.step_device = static_cast<const int64_t*>(scalar_on_device(step_tensor, at::kLong, p0, "step_tensor"));
+  o.grad_scale = static_cast<const float*>(scalar_on_device(grad_scale, at::kFloat, p0, "grad_scale"));
+  const c10::cuda::OptionalCUDAGuard guard(device_of(p0));
+  check_status(fswiglu_adamw_step(table.data(), static_cast<int64_t>(table.size()), pt, gt, eight ? 8 : 32, &o, current_stream(p0)),
+               "adamw_step");
+  // written through raw pointers: what a graph saved of a parameter is known to be stale
+  for (const at::Tensor& p : params) {
+    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+// [norm, factor]: the 2-norm over all gradients, and min(1, max_norm / (norm + 1e-6)) for adamw_step's grad_scale.
+at::Tensor grad_norm_clip(at::TensorList grads, double max_norm) {
+  TORCH_CHECK(!grads.empty(), "grads must not be empty");
+  const at::Tensor& g0 = grads[0];
+  std::vector<fswiglu_grad_tensor> table(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor& g = grads[i];
+    TORCH_CHECK(g.is_cuda() && g.device() == g0.device(), "grads must all be CUDA tensors of one device");
+    TORCH_CHECK(g.is_contiguous(), "grads must all be contiguous");
+    table[i] = {g.data_ptr(), g.numel(), element_type(g, "grads")};
+  }
+  const c10::cuda::OptionalCUDAGuard guard(device_of(g0));
+  at::Tensor out = at::empty({2}, g0.options().dtype(at::kFloat));
+  const size_t bytes = fswiglu_grad_norm_workspace_bytes();
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, g0.options().dtype(at::kByte));
+  check_status(fswiglu_grad_norm_clip(table.data(), static_cast<int64_t>(table.size()), static_cast<float>(max_norm),
+                                      out.data_ptr<float>(), ws.data_ptr(), bytes, current_stream(g0)),
+               "grad_norm_clip");
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward_meta(at::Tensor const& x, std::optional<at::Tensor> const&,
+                                                                       std::optional<at::Tensor> const&, double) {
+  const auto f32 = x.options().dtype(at::kFloat);
+  return {at::empty({x.size(0), x.size(1)}, x.options()), at::empty({x.size(0)}, f32), at::empty({x.size(0)}, f32)};
+}
+std::tuple<at::Tensor, at::Tensor> rms_norm_forward_meta(at::Tensor const& x, std::optional<at::Tensor> const&, double) {
+  return {at::empty({x.size(0), x.size(1)}, x.options()), at::empty({x.size(0)}, x.options().dtype(at::kFloat))};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_meta(at::Tensor const&, at::Tensor const& x, at::Tensor const&,
+                                                                        at::Tensor const&,
+                                                                        std::optional<at::Tensor> const& weight, bool bias_grad,
+                                                                        std::optional<at::Tensor> const&, bool fp32_grads,
+                                                                        bool weight_grad) {
+  const bool w = weight.has_value() && weight->defined();
+  const auto g = x.options().dtype(fp32_grads ? at::kFloat : w ? weight->scalar_type() : x.scalar_type());
+  return {at::empty({x.size(0), x.size(1)}, x.options()), w && weight_grad ? at::empty({x.size(1)}, g) : at::Tensor(),
+          bias_grad ? at::empty({x.size(1)}, g) : at::Tensor()};
+}
+std::tuple<at::Tensor, at::Tensor> rms_norm_backward_meta(at::Tensor const& dout, at::Tensor const& x, at::Tensor const& rstd,
+                                                          std::optional<at::Tensor> const& weight,
+                                                          std::optional<at::Tensor> const& residual, bool fp32_grads,
+                                                          bool weight_grad) {
+  auto g = layer_norm_backward_meta(dout, x, rstd, rstd, weight, false, residual, fp32_grads, weight_grad);
+  return {std::get<0>(g), std::get<1>(g)};
+}
+void adamw_step_meta(at::TensorList, at::TensorList, at::TensorList, at::TensorList, int64_t, double, double, double, double,
+                     double, at::TensorList, at::TensorList, at::TensorList, std::optional<at::Tensor> const&, int64_t,
+                     std::optional<at::Tensor> const&, std::optional<at::Tensor> const&) {}
+at::Tensor grad_norm_clip_meta(at::TensorList grads, double) {
+  TORCH_CHECK(!grads.empty(), "grads must not be empty");
+  return at::empty({2}, grads[0].options().dtype(at::kFloat));
+}
+
 namespace Fused_MLP {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -204,6 +477,32 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_swiglu_mlp_bf16", &fused_swiglu_mlp_bf16, "(residual +) (silu(s x Wg^T) * (s x Wu^T)) Wd^T",
         py::arg("x"), py::arg("W_gate"), py::arg("W_up"), py::arg("W_down"), py::arg("residual") = py::none(),
         py::arg("row_scale") = py::none(), py::arg("fp32_out") = false);
+  m.def("layer_norm_forward", &layer_norm_forward, "(y, mean, rstd) of layer norm over the rows of x", py::arg("x"),
+        py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
+  m.def("rms_norm_forward", &rms_norm_forward, "(y, rstd) of RMS norm over the rows of x", py::arg("x"),
+        py::arg("weight") = py::none(), py::arg("eps") = 1e-6);
+  m.def("layer_norm_backward", &layer_norm_backward, "(dx, dweight, dbias); residual is added to dx", py::arg("dout"),
+        py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("weight") = py::none(), py::arg("bias_grad") = false,
+        py::arg("residual") = py::none(), py::arg("fp32_grads") = false, py::arg("weight_grad") = true);
+  m.def("rms_norm_backward", &rms_norm_backward, "(dx, dweight); residual is added to dx", py::arg("dout"), py::arg("x"),
+        py::arg("rstd"), py::arg("weight") = py::none(), py::arg("residual") = py::none(), py::arg("fp32_grads") = false,
+        py::arg("weight_grad") = true);
+  using Tensors = std::vector<at::Tensor>;
+  m.def("adamw_step",
+        [](const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs, int64_t step,
+           double lr, double beta1, double beta2, double eps, double weight_decay, const Tensors& masters,
+           const Tensors& exp_avg_scales, const Tensors& exp_avg_sq_scales, const std::optional<at::Tensor>& grad_scale,
+           int64_t seed, const std::optional<at::Tensor>& lr_tensor, const std::optional<at::Tensor>& step_tensor) {
+          adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales,
+                     exp_avg_sq_scales, grad_scale, seed, lr_tensor, step_tensor);
+        },
+        "one AdamW step over many tensors, in place", py::arg("params"), py::arg("grads"), py::arg("exp_avgs"),
+        py::arg("exp_avg_sqs"), py::arg("step"), py::arg("lr"), py::arg("beta1") = 0.9, py::arg("beta2") = 0.999,
+        py::arg("eps") = 1e-8, py::arg("weight_decay") = 0.01, py::arg("masters") = Tensors(),
+        py::arg("exp_avg_scales") = Tensors(), py::arg("exp_avg_sq_scales") = Tensors(), py::arg("grad_scale") = py::none(),
+        py::arg("seed") = 0, py::arg("lr_tensor") = py::none(), py::arg("step_tensor") = py::none());
+  m.def("grad_norm_clip", [](const Tensors& grads, double max_norm) { return grad_norm_clip(grads, max_norm); },
+        "[2-norm over all gradients, min(1, max_norm / (norm + 1e-6))]", py::arg("grads"), py::arg("max_norm"));
 }
 
 TORCH_LIBRARY(ASMLLM, m) {
@@ -215,6 +514,17 @@ TORCH_LIBRARY(ASMLLM, m) {
   m.def("swiglu_down_bf16(Tensor h, Tensor W_down, bool fp32_out=False, Tensor? residual=None) -> Tensor");
   m.def("fused_swiglu_mlp_bf16(Tensor x, Tensor W_gate, Tensor W_up, Tensor W_down, Tensor? residual=None, "
         "Tensor? row_scale=None, bool fp32_out=False) -> Tensor");
+  m.def("layer_norm_forward(Tensor x, Tensor? weight=None, Tensor? bias=None, float eps=1e-05) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm_forward(Tensor x, Tensor? weight=None, float eps=1e-06) -> (Tensor, Tensor)");
+  m.def("layer_norm_backward(Tensor dout, Tensor x, Tensor mean, Tensor rstd, Tensor? weight=None, bool bias_grad=False, "
+        "Tensor? residual=None, bool fp32_grads=False, bool weight_grad=True) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm_backward(Tensor dout, Tensor x, Tensor rstd, Tensor? weight=None, Tensor? residual=None, "
+        "bool fp32_grads=False, bool weight_grad=True) -> (Tensor, Tensor)");
+  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, int step, float lr, "
+        "float beta1, float beta2, float eps, float weight_decay, Tensor(d!)[] masters, "
+        "Tensor(e!)[] exp_avg_scales, Tensor(f!)[] exp_avg_sq_scales, Tensor? grad_scale=None, int seed=0, "
+        "Tensor? lr_tensor=None, Tensor? step_tensor=None) -> ()");
+  m.def("grad_norm_clip(Tensor[] grads, float max_norm) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(ASMLLM, CUDA, m) {
@@ -225,6 +535,12 @@ TORCH_LIBRARY_IMPL(ASMLLM, CUDA, m) {
   m.impl("fused_swiglu_gateup_bf16", &fused_swiglu_gateup_bf16);
   m.impl("swiglu_down_bf16", &swiglu_down_bf16);
   m.impl("fused_swiglu_mlp_bf16", &fused_swiglu_mlp_bf16);
+  m.impl("layer_norm_forward", &layer_norm_forward);
+  m.impl("rms_norm_forward", &rms_norm_forward);
+  m.impl("layer_norm_backward", &layer_norm_backward);
+  m.impl("rms_norm_backward", &rms_norm_backward);
+  m.impl("adamw_step", &adamw_step);
+  m.impl("grad_norm_clip", &grad_norm_clip);
 }
 
 TORCH_LIBRARY_IMPL(ASMLLM, Meta, m) {
@@ -234,6 +550,12 @@ TORCH_LIBRARY_IMPL(ASMLLM, Meta, m) {
   m.impl("fused_swiglu_gateup_bf16", &fused_swiglu_gateup_bf16_meta);
   m.impl("swiglu_down_bf16", &swiglu_down_bf16_meta);
   m.impl("fused_swiglu_mlp_bf16", &fused_swiglu_mlp_bf16_meta);
+  m.impl("layer_norm_forward", &layer_norm_forward_meta);
+  m.impl("rms_norm_forward", &rms_norm_forward_meta);
+  m.impl("layer_norm_backward", &layer_norm_backward_meta);
+  m.impl("rms_norm_backward", &rms_norm_backward_meta);
+  m.impl("adamw_step", &adamw_step_meta);
+  m.impl("grad_norm_clip", &grad_norm_clip_meta);
 }
 
 }  // namespace Fused_MLP

@@ -1,0 +1,397 @@
+// C ABI of the training operators around the MLP (declared in include/fswiglu.h): norms with their gradients, AdamW over
+// many tensors, the clipped gradient norm.  Argument checks and launches; no allocation of device memory, no throw.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <memory>
+#include <new>
+
+#include "../../include/fswiglu.h"
+#include "host_state.h"
+#include "norm_sm100.cuh"
+#include "optim_sm100.cuh"
+
+namespace {
+
+using namespace fsw;
+
+bool known_type(int t) { return t == FSWIGLU_OUT_BF16 || t == FSWIGLU_OUT_F32; }
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+size_t type_bytes(int t) { return t == FSWIGLU_OUT_F32 ? 4u : 2u; }
+
+int launched() {
+  count_launch();
+  return cudaGetLastError() == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
+}
+
+// ---- norms ----
+
+constexpr int64_t kMaxNormWidth = 1 << 24;  // a row's length is exact in fp32
+constexpr int kMaxNormSplits = 296;         // two thread blocks for each of 148 SMs
+
+int check_rows(const void* p, int64_t M, int64_t d, int64_t ld, int type) {
+  if (p == nullptr) return FSWIGLU_ERR_BAD_ARG;
+  if (ld < d && M > 1) return FSWIGLU_ERR_SHAPE;
+  return aligned(p, type_bytes(type)) ? FSWIGLU_OK : FSWIGLU_ERR_ALIGNMENT;
+}
+
+int check_norm(int64_t M, int64_t d, int x_dtype, int w_dtype) {
+  if (M < 0 || d <= 0 || !known_type(x_dtype) || !known_type(w_dtype)) return FSWIGLU_ERR_BAD_ARG;
+  if (M > 0x7fffffffll || d > kMaxNormWidth) return FSWIGLU_ERR_SHAPE;
+  return FSWIGLU_OK;
+}
+
+int norm_splits(int64_t M) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(M, kMaxNormSplits))); }
+
+template <typename T, bool kLayer>
+int launch_norm_forward(const NormForwardParams& p, int sms, cudaStream_t s) {
+  const int grid = static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8));
+  norm_forward_any_kernel<T, kLayer><<<grid, kNormThreads, 0, s>>>(p);
+  return launched();
+}
+
+template <typename T, bool kLayer>
+int launch_norm_backward(const NormBackwardParams& p, bool columns, int sms, cudaStream_t s) {
+  const int grid = static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8));
+  norm_backward_any_kernel<T, kLayer><<<grid, kNormThreads, 0, s>>>(p);
+  if (int rc = launched()) return rc;
+  if (!columns) return FSWIGLU_OK;
+  const int64_t tiles = (p.d + kNormThreads - 1) / kNormThreads * static_cast<int64_t>(p.splits);
+  norm_backward_columns_any_kernel<T, kLayer>
+      <<<static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(sms) * 32)), kNormThreads, 0, s>>>(p);
+  return launched();
+}
+
+int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, const void* bias, void* y, int64_t ldy,
+                 float* mean, float* rstd, int64_t M, int64_t d, int x_dtype, int w_dtype, float eps, void* stream) {
+  if (int rc = check_norm(M, d, x_dtype, w_dtype)) return rc;
+  if (!(eps >= 0.0f)) return FSWIGLU_ERR_BAD_ARG;
+  if (M == 0) return FSWIGLU_OK;
+  if (int rc = check_rows(x, M, d, ldx, x_dtype)) return rc;
+  if (int rc = check_rows(y, M, d, ldy, x_dtype)) return rc;
+  if (rstd == nullptr || (layer && mean == nullptr)) return FSWIGLU_ERR_BAD_ARG;
+  if (!aligned(weight, type_bytes(w_dtype)) || !aligned(bias, type_bytes(w_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return FSWIGLU_ERR_ALIGNMENT;
+  int sms = 0;
+  if (int rc = current_device_sms(&sms)) return rc;
+  NormForwardParams p = {};
+  p.x = x;
+  p.weight = weight;
+  p.bias = bias;
+  p.y = y;
+  p.mean = mean;
+  p.rstd = rstd;
+  p.ldx = ldx;
+  p.ldy = ldy;
+  p.M = static_cast<int>(M);
+  p.d = static_cast<int>(d);
+  p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
+  p.eps = eps;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x_dtype == FSWIGLU_OUT_F32)
+    return layer ? launch_norm_forward<float, true>(p, sms, s) : launch_norm_forward<float, false>(p, sms, s);
+  return layer ? launch_norm_forward<__nv_bfloat16, true>(p, sms, s) : launch_norm_forward<__nv_bfloat16, false>(p, sms, s);
+}
+
+int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* mean,
+                  const float* rstd, const void* weight, const void* residual, int64_t ld_res, void* dx, int64_t ld_dx,
+                  void* dweight, void* dbias, int64_t M, int64_t d, int x_dtype, int w_dtype, int grad_dtype,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_norm(M, d, x_dtype, w_dtype)) return rc;
+  if (!known_type(grad_dtype)) return FSWIGLU_ERR_BAD_ARG;
+  if (!aligned(weight, type_bytes(w_dtype)) || !aligned(dweight, type_bytes(grad_dtype)) ||
+      !aligned(dbias, type_bytes(grad_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return FSWIGLU_ERR_ALIGNMENT;
+  const bool columns = dweight != nullptr || dbias != nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  NormBackwardParams p = {};
+  if (M > 0) {
+    if (int rc = check_rows(dout, M, d, ld_dout, x_dtype)) return rc;
+    if (int rc = check_rows(x, M, d, ldx, x_dtype)) return rc;
+    if (int rc = check_rows(dx, M, d, ld_dx, x_dtype)) return rc;
+    if (residual != nullptr) {
+      if (int rc = check_rows(residual, M, d, ld_res, x_dtype)) return rc;
+    }
+    if (rstd == nullptr || (layer && mean == nullptr)) return FSWIGLU_ERR_BAD_ARG;
+    if (columns && (workspace == nullptr || workspace_bytes < fswiglu_norm_backward_workspace_bytes(M, d) || !aligned(workspace, 256)))
+      return FSWIGLU_ERR_WORKSPACE;
+  }
+  int sms = 0;
+  if (int rc = current_device_sms(&sms)) return rc;
+  if (M > 0) {
+    p.dout = dout;
+    p.x = x;
+    p.weight = weight;
+    p.residual = residual;
+    p.mean = mean;
+    p.rstd = rstd;
+    p.dx = dx;
+    p.partial = static_cast<float*>(workspace);
+    p.ld_dout = ld_dout;
+    p.ldx = ldx;
+    p.ld_res = ld_res;
+    p.ld_dx = ld_dx;
+    p.M = static_cast<int>(M);
+    p.d = static_cast<int>(d);
+    p.splits = norm_splits(M);
+    p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
+    int rc;
+    if (x_dtype == FSWIGLU_OUT_F32)
+      rc = layer ? launch_norm_backward<float, true>(p, columns, sms, s) : launch_norm_backward<float, false>(p, columns, sms, s);
+    else
+      rc = layer ? launch_norm_backward<__nv_bfloat16, true>(p, columns, sms, s)
+                 : launch_norm_backward<__nv_bfloat16, false>(p, columns, sms, s);
+    if (rc) return rc;
+  }
+  if (!columns) return FSWIGLU_OK;
+  NormReduceParams q = {};  // no rows: no splits, the gradients are zero
+  q.partial = p.partial;
+  q.dweight = dweight;
+  q.dbias = dbias;
+  q.d = static_cast<int>(d);
+  q.splits = p.splits;
+  q.out_f32 = grad_dtype == FSWIGLU_OUT_F32;
+  norm_reduce_kernel<<<static_cast<int>((d + kNormThreads - 1) / kNormThreads), kNormThreads, 0, s>>>(q);
+  return launched();
+}
+
+// ---- many tensors ----
+
+constexpr int kSmallTable = 48;   // kernel parameters below 4 KB: what every launch copies
+constexpr int kLargeTable = 400;  // below the 32764 bytes that a launch takes
+
+struct Range {
+  uintptr_t begin, end;
+};
+
+// Whether no two of the call's written ranges of one kind overlap.  Ranges in ascending order, as an allocator hands
+// them out, need no copy; others are sorted.
+template <typename Get>
+int disjoint(int64_t count, Get get) {
+  bool ascending = true;
+  uintptr_t last = 0;
+  for (int64_t i = 0; i < count && ascending; ++i) {
+    const Range r = get(i);
+    if (r.begin == r.end) continue;
+    ascending = r.begin >= last;
+    last = r.end;
+  }
+  if (ascending) return FSWIGLU_OK;
+  std::unique_ptr<Range[]> all(new (std::nothrow) Range[count]);
+  if (all == nullptr) return FSWIGLU_ERR_BAD_ARG;
+  int64_t n = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const Range r = get(i);
+    if (r.begin != r.end) all[n++] = r;
+  }
+  std::sort(all.get(), all.get() + n, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (int64_t i = 1; i < n; ++i) {
+    if (all[i].begin < all[i - 1].end) return FSWIGLU_ERR_BAD_ARG;
+  }
+  return FSWIGLU_OK;
+}
+
+Range range_of(const void* p, int64_t bytes) {
+  const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+  return Range{b, b + static_cast<uintptr_t>(p == nullptr ? 0 : bytes)};
+}
+
+uint32_t chunks_of(int64_t numel) { return static_cast<uint32_t>((numel + kAdamChunk - 1) / kAdamChunk); }
+
+constexpr int64_t kMaxNumel = 1ll << 35;  // chunks of a full table are counted in 32 bits
+
+template <typename P, bool kEight, int kCapacity>
+int launch_adamw(const AdamTable<kCapacity>& t, int sms, cudaStream_t s) {
+  const uint32_t grid = std::min<uint32_t>(t.first_chunk[t.count], static_cast<uint32_t>(sms) * 8u);
+  adamw_kernel<P, kEight, kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
+  return launched();
+}
+
+template <int kCapacity>
+int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const AdamOptions& o, int param_dtype, int state_bits,
+                   int sms, cudaStream_t s) {
+  AdamTable<kCapacity> t;
+  t.opt = o;
+  t.count = 0;
+  t.first_chunk[0] = 0;
+  long long blocks = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const fswiglu_adamw_tensor& a = tensors[i];
+    if (a.numel > 0) {
+      t.tensors[t.count] = AdamTensor{a.param,  a.grad, a.exp_avg, a.exp_avg_sq, a.master, a.exp_avg_scale,
+                                      a.exp_avg_sq_scale, static_cast<long long>(a.numel)};
+      t.first_block[t.count] = blocks;
+      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(a.numel);
+      blocks += (a.numel + kAdamBlock - 1) / kAdamBlock;
+      ++t.count;
+    }
+    if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
+    int rc;
+    if (param_dtype == FSWIGLU_OUT_F32)
+      rc = state_bits == 8 ? launch_adamw<float, true>(t, sms, s) : launch_adamw<float, false>(t, sms, s);
+    else
+      rc = state_bits == 8 ? launch_adamw<__nv_bfloat16, true>(t, sms, s) : launch_adamw<__nv_bfloat16, false>(t, sms, s);
+    if (rc) return rc;
+    t.count = 0;
+  }
+  return FSWIGLU_OK;
+}
+
+template <int kCapacity>
+int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double* slots, int* used, int sms, cudaStream_t s) {
+  GradTable<kCapacity> t;
+  t.slots = slots;
+  t.count = 0;
+  t.first_chunk[0] = 0;
+  t.accumulate = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (tensors[i].numel > 0) {
+      t.tensors[t.count] = GradTensor{tensors[i].grad, static_cast<long long>(tensors[i].numel),
+                                      tensors[i].dtype == FSWIGLU_OUT_F32};
+      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(tensors[i].numel);
+      ++t.count;
+    }
+    if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
+    // every launch of a call has the same thread blocks: a later one adds to the slots of the first
+    const int grid = std::min(kGradNormSlots, sms * 8);
+    grad_norm_kernel<kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
+    if (int rc = launched()) return rc;
+    *used = grid;
+    t.accumulate = 1;
+    t.count = 0;
+  }
+  return FSWIGLU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fswiglu_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, void* y, int64_t ldy,
+                               float* mean, float* rstd, int64_t M, int64_t d, int x_dtype, int w_dtype, float eps,
+                               void* stream) {
+  return norm_forward(true, x, ldx, weight, bias, y, ldy, mean, rstd, M, d, x_dtype, w_dtype, eps, stream);
+}
+
+int fswiglu_rms_norm_forward(const void* x, int64_t ldx, const void* weight, void* y, int64_t ldy, float* rstd, int64_t M,
+                             int64_t d, int x_dtype, int w_dtype, float eps, void* stream) {
+  return norm_forward(false, x, ldx, weight, nullptr, y, ldy, nullptr, rstd, M, d, x_dtype, w_dtype, eps, stream);
+}
+
+size_t fswiglu_norm_backward_workspace_bytes(int64_t M, int64_t d) {
+  if (M <= 0 || d <= 0 || d > kMaxNormWidth) return 0;
+  return (static_cast<size_t>(norm_splits(M)) * 2u * static_cast<size_t>(d) * 4u + 255u) / 256u * 256u;
+}
+
+int fswiglu_layer_norm_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* mean,
+                                const float* rstd, const void* weight, const void* residual, int64_t ld_res, void* dx,
+                                int64_t ld_dx, void* dweight, void* dbias, int64_t M, int64_t d, int x_dtype, int w_dtype,
+                                int grad_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return norm_backward(true, dout, ld_dout, x, ldx, mean, rstd, weight, residual, ld_res, dx, ld_dx, dweight, dbias, M, d,
+                       x_dtype, w_dtype, grad_dtype, workspace, workspace_bytes, stream);
+}
+
+int fswiglu_rms_norm_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* rstd,
+                              const void* weight, const void* residual, int64_t ld_res, void* dx, int64_t ld_dx,
+                              void* dweight, int64_t M, int64_t d, int x_dtype, int w_dtype, int grad_dtype,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return norm_backward(false, dout, ld_dout, x, ldx, nullptr, rstd, weight, residual, ld_res, dx, ld_dx, dweight, nullptr,
+                       M, d, x_dtype, w_dtype, grad_dtype, workspace, workspace_bytes, stream);
+}
+
+int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int param_dtype, int grad_dtype, int state_bits,
+                       const fswiglu_adamw_options* options, void* stream) {
+  if (count < 0 || (count > 0 && tensors == nullptr) || options == nullptr) return FSWIGLU_ERR_BAD_ARG;
+  if (!known_type(param_dtype) || !known_type(grad_dtype) || (state_bits != 8 && state_bits != 32)) return FSWIGLU_ERR_BAD_ARG;
+  const fswiglu_adamw_options& in = *options;
+  if (!(in.beta1 >= 0.0 && in.beta1 < 1.0 && in.beta2 >= 0.0 && in.beta2 < 1.0 && in.eps >= 0.0 && in.weight_decay >= 0.0) ||
+      !std::isfinite(in.eps) || !std::isfinite(in.weight_decay))
+    return FSWIGLU_ERR_BAD_ARG;
+  if (in.lr_device == nullptr && !(in.lr >= 0.0 && std::isfinite(in.lr))) return FSWIGLU_ERR_BAD_ARG;
+  if (in.step_device == nullptr && in.step < 1) return FSWIGLU_ERR_BAD_ARG;
+  if (!aligned(in.lr_device, 4) || !aligned(in.step_device, 8) || !aligned(in.grad_scale, 4)) return FSWIGLU_ERR_ALIGNMENT;
+  const size_t pb = type_bytes(param_dtype), gb = type_bytes(grad_dtype), sb = state_bits == 8 ? 1u : 4u;
+  bool any = false;
+  for (int64_t i = 0; i < count; ++i) {
+    const fswiglu_adamw_tensor& a = tensors[i];
+    if (a.numel < 0) return FSWIGLU_ERR_BAD_ARG;
+    if (a.numel == 0) continue;
+    if (a.numel > kMaxNumel) return FSWIGLU_ERR_SHAPE;
+    any = true;
+    if (a.param == nullptr || a.grad == nullptr || a.exp_avg == nullptr || a.exp_avg_sq == nullptr) return FSWIGLU_ERR_BAD_ARG;
+    if (state_bits == 8 && (a.exp_avg_scale == nullptr || a.exp_avg_sq_scale == nullptr)) return FSWIGLU_ERR_BAD_ARG;
+    if (param_dtype == FSWIGLU_OUT_F32 && a.master != nullptr) return FSWIGLU_ERR_BAD_ARG;
+    if (!aligned(a.param, pb) || !aligned(a.grad, gb) || !aligned(a.exp_avg, sb) || !aligned(a.exp_avg_sq, sb) ||
+        !aligned(a.master, 4) || !aligned(a.exp_avg_scale, 4) || !aligned(a.exp_avg_sq_scale, 4))
+      return FSWIGLU_ERR_ALIGNMENT;
+  }
+  if (!any) return FSWIGLU_OK;
+  int rc;
+  if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].param, tensors[i].numel * static_cast<int64_t>(pb)); })))
+    return rc;
+  if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg, tensors[i].numel * static_cast<int64_t>(sb)); })))
+    return rc;
+  if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg_sq, tensors[i].numel * static_cast<int64_t>(sb)); })))
+    return rc;
+  if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].master, tensors[i].numel * 4); }))) return rc;
+  int sms = 0;
+  if ((rc = current_device_sms(&sms))) return rc;
+  AdamOptions o = {};
+  o.log_beta1 = std::log(in.beta1);
+  o.log_beta2 = std::log(in.beta2);
+  o.lr = static_cast<float>(in.lr);
+  o.beta1 = static_cast<float>(in.beta1);
+  o.one_minus_beta1 = static_cast<float>(1.0 - in.beta1);
+  o.beta2 = static_cast<float>(in.beta2);
+  o.one_minus_beta2 = static_cast<float>(1.0 - in.beta2);
+  o.eps = static_cast<float>(in.eps);
+  o.weight_decay = static_cast<float>(in.weight_decay);
+  if (in.step_device == nullptr) {
+    const double t = static_cast<double>(in.step);
+    const double lr = in.lr_device == nullptr ? in.lr : 1.0;
+    o.step_size = static_cast<float>(lr / (1.0 - std::pow(in.beta1, t)));
+    o.inv_sqrt_correction2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(in.beta2, t)));
+  }
+  o.lr_device = in.lr_device;
+  o.step_device = reinterpret_cast<const long long*>(in.step_device);
+  o.grad_scale = in.grad_scale;
+  o.seed_lo = static_cast<uint32_t>(in.seed);
+  o.seed_hi = static_cast<uint32_t>(in.seed >> 32);
+  o.step_lo = static_cast<uint32_t>(in.step);
+  o.grad_dtype_f32 = grad_dtype == FSWIGLU_OUT_F32;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, param_dtype, state_bits, sms, s)
+                              : adamw_launches<kLargeTable>(tensors, count, o, param_dtype, state_bits, sms, s);
+}
+
+size_t fswiglu_grad_norm_workspace_bytes(void) { return kGradNormSlots * sizeof(double); }
+
+int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, float max_norm, float* out, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  if (count < 0 || (count > 0 && tensors == nullptr) || out == nullptr || !(max_norm >= 0.0f)) return FSWIGLU_ERR_BAD_ARG;
+  if (workspace == nullptr || workspace_bytes < fswiglu_grad_norm_workspace_bytes() || !aligned(workspace, 256))
+    return FSWIGLU_ERR_WORKSPACE;
+  if (!aligned(out, 4)) return FSWIGLU_ERR_ALIGNMENT;
+  for (int64_t i = 0; i < count; ++i) {
+    const fswiglu_grad_tensor& a = tensors[i];
+    if (a.numel < 0 || !known_type(a.dtype)) return FSWIGLU_ERR_BAD_ARG;
+    if (a.numel == 0) continue;
+    if (a.numel > kMaxNumel) return FSWIGLU_ERR_SHAPE;
+    if (a.grad == nullptr) return FSWIGLU_ERR_BAD_ARG;
+    if (!aligned(a.grad, type_bytes(a.dtype))) return FSWIGLU_ERR_ALIGNMENT;
+  }
+  int sms = 0;
+  if (int rc = current_device_sms(&sms)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  double* slots = static_cast<double*>(workspace);
+  int used = 0;
+  const int rc = count <= kSmallTable ? grad_norm_launches<kSmallTable>(tensors, count, slots, &used, sms, s)
+                                      : grad_norm_launches<kLargeTable>(tensors, count, slots, &used, sms, s);
+  if (rc) return rc;
+  grad_norm_finish_kernel<<<1, kAdamThreads, 0, s>>>(slots, used, max_norm, out);
+  return launched();
+}
+
+}  // extern "C"

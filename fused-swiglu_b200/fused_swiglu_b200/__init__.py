@@ -7,10 +7,11 @@
     tp      Megatron-style tensor-parallel forward (one process per GPU, NCCL)
     inputs  seeded synthetic inputs of the benchmark configurations
     module  nn.Module wrapper (gate_proj / up_proj / down_proj) over the dispatcher op
+    train   norms with gradients, the pre-norm block with autograd, clipped gradient norm, AdamW
 
 Importing the package loads the CUDA library and raises if it has not been built.
 """
-from . import capi, inputs, ops, pack  # noqa: F401
+from . import capi, inputs, ops, pack, train  # noqa: F401
 from .ops import (  # noqa: F401
     fused_swiglu_bf16,
     fused_swiglu_gateup_bf16,

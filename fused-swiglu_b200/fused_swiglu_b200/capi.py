@@ -48,6 +48,16 @@ SIGNATURES = {
                                          _i64, _int, _i64, _i64, _i64, _vp, _sz, _vp]),
     "fswiglu_gemm_tn_bf16": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
     "fswiglu_transpose_bf16": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "fswiglu_layer_norm_forward": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _int, _int, _f32, _vp]),
+    "fswiglu_rms_norm_forward": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _int, _int, _f32, _vp]),
+    "fswiglu_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "fswiglu_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
+                                           _int, _int, _int, _vp, _sz, _vp]),
+    "fswiglu_rms_norm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _int, _int,
+                                         _int, _vp, _sz, _vp]),
+    "fswiglu_adamw_step": (_int, [_vp, _i64, _int, _int, _int, _vp, _vp]),
+    "fswiglu_grad_norm_workspace_bytes": (_sz, []),
+    "fswiglu_grad_norm_clip": (_int, [_vp, _i64, _f32, _vp, _vp, _sz, _vp]),
     "fswiglu_cast_f32_to_bf16": (_int, [_vp, _vp, _i64, _vp]),
     "fswiglu_down_scatter_bf16": (_int, [_vp, _i64, _vp, _i64, ctypes.POINTER(ctypes.c_void_p), _int, _int, _i64, _i64,
                                          _i64, _i64, _vp, _sz, _vp]),
@@ -62,6 +72,27 @@ SIGNATURES = {
     "fswiglu_version": (ctypes.c_char_p, []),
     "fswiglu_launch_count": (ctypes.c_uint64, []),
 }
+
+
+class AdamWTensor(ctypes.Structure):
+    """fswiglu_adamw_tensor"""
+
+    _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("master", _vp),
+                ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp), ("numel", _i64)]
+
+
+class AdamWOptions(ctypes.Structure):
+    """fswiglu_adamw_options"""
+
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("step", _i64), ("seed", ctypes.c_uint64), ("lr_device", _vp),
+                ("step_device", _vp), ("grad_scale", _vp)]
+
+
+class GradTensor(ctypes.Structure):
+    """fswiglu_grad_tensor"""
+
+    _fields_ = [("grad", _vp), ("numel", _i64), ("dtype", _int)]
 
 
 class FswigluError(RuntimeError):

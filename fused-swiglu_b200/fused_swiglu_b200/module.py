@@ -99,3 +99,31 @@ class FusedNormSwiGLUBlock(nn.Module):
         scale = ops.rms_scale(x2, self.eps)
         out = ops.fused_swiglu_mlp_bf16(x2, self._folded[0], self._folded[1], self.mlp.down_proj, x2, scale, False)
         return out.reshape(*lead, hidden)
+
+
+class NormSwiGLUBlock(nn.Module):
+    """out = x + down_proj(silu(gate_proj(n)) * up_proj(n)),  n = RMSNorm(x) or LayerNorm(x): the block to train.
+
+    Same parameters as `FusedNormSwiGLUBlock` (plus `norm_bias` for norm="layer"), all of them with gradients; forward and
+    backward run on the fused kernels (`train.norm_swiglu_block`).  The norm is not folded into the matrices here, whose
+    weights change with every step.
+    """
+
+    def __init__(self, hidden_size: int, intermediate_size: int, norm: str = "rms", eps: float = 1e-6, device=None):
+        super().__init__()
+        if norm not in ("rms", "layer"):
+            raise ValueError('norm must be "rms" or "layer"')
+        self.mlp = FusedSwiGLUMLP(hidden_size, intermediate_size, device=device)
+        self.mlp.requires_grad_(True)
+        kw = dict(dtype=torch.bfloat16, device=device)
+        self.norm_weight = nn.Parameter(torch.ones((hidden_size,), **kw))
+        self.norm_bias = nn.Parameter(torch.zeros((hidden_size,), **kw)) if norm == "layer" else None
+        self.norm, self.eps = norm, eps
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        from . import train
+
+        if x.size(-1) != self.mlp.hidden_size:
+            raise RuntimeError(f"expected last dimension {self.mlp.hidden_size}, got {x.size(-1)}")
+        return train.norm_swiglu_block(x, self.norm_weight, self.norm_bias, self.mlp.gate_proj, self.mlp.up_proj,
+                                       self.mlp.down_proj, self.eps, self.norm)

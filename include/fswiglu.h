@@ -223,6 +223,106 @@ int fswiglu_transpose_bf16(const void* src, int64_t ld_src, void* dst, int64_t l
                            void* stream);
 
 /*
+ * Training operators around the MLP: norms with their gradients, AdamW over many tensors, the clipped gradient
+ * norm.  No counterpart in the reference, which is forward only.  Element types are FSWIGLU_OUT_BF16 and
+ * FSWIGLU_OUT_F32.  All sums, statistics and moments' arithmetic are fp32 (the gradient norm's total fp64), every
+ * output is rounded once, and every result is the same from call to call: no atomics.
+ *
+ * Unlike the MLP's entry points these take any width, pitch (ld >= d) and element-aligned base; 16-byte aligned
+ * bases and pitches take wider loads.  Outputs must not overlap inputs or one another, except where a call says
+ * that it updates in place.
+ *
+ *     z = (x - mean) rstd      y = z w + b      rstd = 1 / sqrt(mean((x - mean)^2) + eps)      (RMS norm: mean = 0)
+ *
+ * x, y [M, d] of x_dtype, weight and bias [d] of w_dtype (NULL: ones and zeros), mean and rstd [M] fp32: what the
+ * backward pass needs.  1 <= d <= 2^24; M == 0 is a no-op.  rstd of the RMS form is fswiglu_rms_scale_f32's.
+ */
+int fswiglu_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, void* y,
+                               int64_t ldy, float* mean, float* rstd, int64_t M, int64_t d, int x_dtype,
+                               int w_dtype, float eps, void* stream);
+int fswiglu_rms_norm_forward(const void* x, int64_t ldx, const void* weight, void* y, int64_t ldy, float* rstd,
+                             int64_t M, int64_t d, int x_dtype, int w_dtype, float eps, void* stream);
+
+/*
+ * Given dout = dL/dy, with a = dout w:
+ *     dx = rstd (a - mean(a) - z mean(a z)) + residual      dweight = sum_rows dout z      dbias = sum_rows dout
+ * residual (NULL, or [M, d] of x_dtype) is the gradient that reaches x past the norm: in out = x + f(norm(x)) it is
+ * the gradient of out.  dweight and dbias [d] are written (not accumulated) as grad_dtype; either may be NULL, and
+ * with M == 0 they are zero.  The workspace (256-byte aligned, fswiglu_norm_backward_workspace_bytes) holds the row
+ * splits' partial sums; it is not needed where both are NULL.
+ */
+size_t fswiglu_norm_backward_workspace_bytes(int64_t M, int64_t d);
+int fswiglu_layer_norm_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* mean,
+                                const float* rstd, const void* weight, const void* residual, int64_t ld_res,
+                                void* dx, int64_t ld_dx, void* dweight, void* dbias, int64_t M, int64_t d,
+                                int x_dtype, int w_dtype, int grad_dtype, void* workspace, size_t workspace_bytes,
+                                void* stream);
+int fswiglu_rms_norm_backward(const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* rstd,
+                              const void* weight, const void* residual, int64_t ld_res, void* dx, int64_t ld_dx,
+                              void* dweight, int64_t M, int64_t d, int x_dtype, int w_dtype, int grad_dtype,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One AdamW step over `count` tensors, in place:
+ *     g = grad_scale grad      m = beta1 m + (1 - beta1) g      v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ *
+ * All tensors of a call share param_dtype, grad_dtype and state_bits; each is `numel` contiguous elements, and
+ * tensors without elements are skipped.  `master` is NULL, or (bf16 parameters only) the parameter's fp32 copy, from
+ * which the step computes and into which it writes, param being its rounding.  Without it a bf16 parameter loses
+ * what the rounding of each step drops.
+ *   state_bits == 32 : exp_avg and exp_avg_sq are fp32.
+ *   state_bits == 8  : in blocks of 256 elements (the last may be shorter), exp_avg is float8_e4m3fn and exp_avg_sq
+ *       float8_e5m2, each times the block's scale, a power of two in exp_avg_scale / exp_avg_sq_scale
+ *       [ceil(numel / 256)].  All zeros is the state to start from.  They are rounded stochastically, by 16 bits
+ *       for each value that depend on seed, step and the value's position in the call's list alone: the same call
+ *       gives the same bits.  A second moment above zero is kept above zero.  A block with a moment that is not
+ *       finite gets NaN for its scale.
+ * The tensors are described in host memory, which the call has read when it returns (it may be freed then); the
+ * launches carry the pointers, so that a captured graph needs nothing but the tensors themselves.  No two tensors
+ * may share parameters, masters or moments (checked: FSWIGLU_ERR_BAD_ARG).
+ * Options: lr_device (fp32) and step_device (int64, >= 1), where not NULL, are read on the device in the place of lr
+ * and step, so that a captured graph can be replayed with other values.  grad_scale (fp32, NULL: 1) is read on the
+ * device too; where it is not finite the step changes nothing.
+ */
+typedef struct fswiglu_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* master;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  int64_t numel;
+} fswiglu_adamw_tensor;
+typedef struct fswiglu_adamw_options {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  uint64_t seed;
+  const float* lr_device;
+  const int64_t* step_device;
+  const float* grad_scale;
+} fswiglu_adamw_options;
+int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int param_dtype, int grad_dtype,
+                       int state_bits, const fswiglu_adamw_options* options, void* stream);
+
+/*
+ * out[0] = the 2-norm over all elements of `count` gradients, out[1] = min(1, max_norm / (out[0] + 1e-6)): the
+ * grad_scale that clips them, without a copy to the host.  Where the norm is not finite out[1] is NaN, which makes
+ * fswiglu_adamw_step skip the step.  Squares are summed in fp32 over the elements that one thread reads of a chunk,
+ * in fp64 from there; an element above 1.8e19 makes the norm infinite.  Types may differ from gradient to gradient.
+ * The workspace is 256-byte aligned; calls that may overlap need one each.
+ */
+typedef struct fswiglu_grad_tensor {
+  const void* grad;
+  int64_t numel;
+  int dtype;
+} fswiglu_grad_tensor;
+size_t fswiglu_grad_norm_workspace_bytes(void);
+int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, float max_norm, float* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * dst[i] = bf16(src[i]) for n contiguous elements (round to nearest even): the single rounding after
  * tensor-parallel fp32 partial sums have been reduced.  No counterpart in the reference (single GPU).
  * src and dst must be 16-byte aligned.

@@ -1,0 +1,278 @@
+"""The training operators as a user runs them together: norms under autograd, the pre-norm block forward and backward, clipping
+and the optimiser, eagerly and from a captured graph.
+
+Tolerances: single norms as in test_train_gpu.py are held elementwise there; here gradients go through bf16 intermediates
+(norm output, gate, up, their gradients: one rounding of 2^-8 each, random in sign), so outputs are held to a relative 2-norm
+of 5e-3 and gradients to 1e-2, the bounds of the MLP's own tests.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def fsw(cuda_dev):
+    import fused_swiglu_b200 as pkg
+
+    yield pkg
+    torch.cuda.synchronize()
+    assert pkg.capi.device_status() == 0
+
+
+def rel(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert got.shape == want.shape and bool(torch.isfinite(got).all())
+    return float((got - want).norm() / want.norm())
+
+
+def norm64(x, w, b, eps, layer):
+    mean = x.mean(-1, keepdim=True) if layer else 0.0
+    z = (x - mean) / torch.sqrt((x - mean).square().mean(-1, keepdim=True) + eps)
+    z = z if w is None else z * w
+    return z if b is None else z + b
+
+
+def leaf64(t):
+    return None if t is None else t.detach().double().cpu().requires_grad_()
+
+
+@pytest.mark.parametrize("layer", [True, False], ids=["layer", "rms"])
+@pytest.mark.parametrize("shape,how", [((3, 5, 96), "plain"), ((1, 1001), "plain"), ((4, 6, 64), "transposed"),
+                                       ((4, 40, 2), "sliced"), ((5, 72), "broadcast"), ((0, 64), "plain"), ((64,), "plain")],
+                         ids=str)
+def test_norms_under_autograd(fsw, cuda_dev, shape, how, layer):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(shape, generator=g).to(cuda_dev)
+    if how == "transposed":
+        x = x.transpose(0, 1)
+    if how == "sliced":
+        x = x.transpose(1, 2)
+    x = x.detach().requires_grad_()
+    used = x[:1].expand(7, shape[-1]) if how == "broadcast" else x
+    d = used.size(-1)
+    w = torch.randn(d, generator=g).to(cuda_dev).requires_grad_()
+    b = torch.randn(d, generator=g).to(cuda_dev).requires_grad_() if layer else None
+    y = fsw.train.layer_norm(used, w, b, 1e-5) if layer else fsw.train.rms_norm(used, w, 1e-5)
+    dout = torch.randn(used.shape, generator=g).to(cuda_dev)
+    y.backward(dout)
+    x64, w64, b64 = leaf64(x), leaf64(w), leaf64(b)
+    y64 = norm64(x64[:1].expand(7, shape[-1]) if how == "broadcast" else x64, w64, b64, 1e-5, layer)
+    y64.backward(dout.double().cpu())
+    if x.numel() == 0:
+        assert y.shape == x.shape and not w.grad.any()
+        return
+    # sums of at most 1001 terms, off by 48 units of their magnitudes; two of them meet in dx
+    for got, want in ((y, y64), (x.grad, x64.grad), (w.grad, w64.grad)) + (((b.grad, b64.grad),) if layer else ()):
+        assert rel(got, want) <= 128 * U
+
+
+def test_norm_gradients_that_nobody_asked_for(fsw, cuda_dev):
+    x = torch.randn(6, 64, device=cuda_dev, dtype=BF, requires_grad=True)
+    w = torch.ones(64, device=cuda_dev, dtype=BF)
+    b = torch.zeros(64, device=cuda_dev, requires_grad=True)
+    fsw.train.layer_norm(x, w).sum().backward()
+    assert w.grad is None and x.grad is not None
+    y = fsw.train.layer_norm(x, None, b)  # an fp32 bias without a weight keeps its gradient in fp32
+    y.backward(torch.full_like(y, 1.0078125))
+    assert b.grad.dtype == torch.float32 and bool((b.grad == 6 * 1.0078125).all())
+    y = fsw.train.rms_norm(x)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(y.sum(), x, create_graph=True)[0].sum(), x)
+
+
+def block_inputs(M, d, F, dev, seed, norm):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((M, d), generator=g)
+    w, b = 1 + 0.1 * torch.randn(d, generator=g), 0.1 * torch.randn(d, generator=g)
+    mats = [torch.randn(s, generator=g) * 0.05 for s in ((F, d), (F, d), (d, F))]
+    ts = [x, w, b if norm == "layer" else None, *mats]
+    return [None if t is None else t.to(BF).to(dev) for t in ts]
+
+
+def block64(x, w, b, wg, wu, wd, eps, norm):
+    n = norm64(x, w, b, eps, norm == "layer")
+    g, u = n @ wg.T, n @ wu.T
+    return x + (g * torch.sigmoid(g) * u) @ wd.T
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("M,d,F", [(1, 64, 128), (33, 72, 136), (300, 520, 1096), (512, 256, 512)])
+def test_block_and_its_gradients(fsw, cuda_dev, M, d, F, norm):
+    ts = [None if t is None else t.requires_grad_() for t in block_inputs(M, d, F, cuda_dev, M, norm)]
+    out = fsw.train.norm_swiglu_block(*ts, eps=1e-6, norm=norm)
+    dout = torch.randn((M, d), generator=torch.Generator().manual_seed(3)).to(BF).to(cuda_dev)
+    out.backward(dout)
+    ts64 = [leaf64(t) for t in ts]
+    out64 = block64(*ts64, 1e-6, norm)
+    out64.backward(dout.double().cpu())
+    assert rel(out, out64) <= 5e-3
+    for t, t64 in zip(ts, ts64):
+        if t is not None:
+            assert t.grad.dtype == BF and rel(t.grad, t64.grad) <= 1e-2
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_block_module_agrees_with_the_inference_block(fsw, cuda_dev, norm):
+    from fused_swiglu_b200.module import FusedNormSwiGLUBlock, NormSwiGLUBlock
+
+    x, w, b, wg, wu, wd = block_inputs(70, 128, 256, cuda_dev, 5, norm)
+    train, serve = NormSwiGLUBlock(128, 256, norm=norm, device=cuda_dev), FusedNormSwiGLUBlock(128, 256, device=cuda_dev)
+    with torch.no_grad():
+        for block in (train, serve):
+            block.norm_weight.copy_(w)
+            for p, t in ((block.mlp.gate_proj, wg), (block.mlp.up_proj, wu), (block.mlp.down_proj, wd)):
+                p.copy_(t)
+        if norm == "layer":
+            train.norm_bias.copy_(b)
+    out = train(x.view(7, 10, 128))
+    assert out.shape == (7, 10, 128) and out.requires_grad
+    assert rel(out.view(70, 128), block64(*(None if t is None else t.double().cpu() for t in (x, w, b, wg, wu, wd)), 1e-6, norm)) <= 5e-3
+    if norm == "rms":
+        assert rel(out.view(70, 128), serve(x)) <= 5e-3
+    assert len(list(train.parameters())) == (5 if norm == "layer" else 4) and all(p.requires_grad for p in train.parameters())
+    with pytest.raises(RuntimeError, match="last dimension"):
+        train(x[:, :64])
+
+
+def values(opt, p):
+    s = opt.state.get(p, {})
+    return {k: v.clone() for k, v in s.items() if isinstance(v, torch.Tensor)} | {"p": p.detach().clone()}
+
+
+def moments(fsw, s, key):
+    return (fsw.train.moments_to_float(s[key], s[key + "_scale"]) if key + "_scale" in s else s[key]).double().cpu()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_training_steps_follow_the_formulas(fsw, cuda_dev, norm, bits):
+    """Forward, backward, clip, AdamW: each step's weights from the step's own gradients, in 64 bits."""
+    from fused_swiglu_b200.module import NormSwiGLUBlock
+
+    torch.manual_seed(0)
+    block = NormSwiGLUBlock(136, 264, norm=norm, device=cuda_dev)
+    with torch.no_grad():
+        for p in (block.mlp.gate_proj, block.mlp.up_proj, block.mlp.down_proj):
+            p.normal_(0, 0.1)
+    vectors = [p for p in block.parameters() if p.dim() == 1]
+    opt = fsw.train.FusedAdamW([{"params": [p for p in block.parameters() if p.dim() == 2], "weight_decay": 0.1},
+                                {"params": vectors, "weight_decay": 0.0, "lr": 3e-3}], lr=1e-2, state_bits=bits,
+                               max_grad_norm=0.7, seed=5)
+    x = torch.randn(50, 136, device=cuda_dev, dtype=BF)
+    for step in range(1, 4):
+        opt.zero_grad()
+        block(x).float().square().mean().mul(100.0).backward()
+        before = {p: values(opt, p) for p in block.parameters()}
+        opt.step()
+        norm64_ = sum(float(p.grad.double().square().sum()) for p in block.parameters()) ** 0.5
+        assert abs(float(opt.last_grad_norm[0]) - norm64_) <= 10 * U * norm64_
+        scale = min(1.0, 0.7 / (norm64_ + 1e-6))
+        for group in opt.param_groups:
+            for p in group["params"]:
+                old, new = before[p], values(opt, p)
+                zero = torch.zeros(p.shape, dtype=torch.float64)
+                m0 = moments(fsw, old, "exp_avg") if step > 1 else zero
+                v0 = moments(fsw, old, "exp_avg_sq") if step > 1 else zero
+                w0 = (old["master"] if step > 1 else old["p"]).double().cpu()
+                g = p.grad.double().cpu() * scale
+                m, v = 0.9 * m0 + 0.1 * g, 0.999 * v0 + 0.001 * g * g
+                update = group["lr"] / (1 - 0.9 ** step) * m / ((v / (1 - 0.999 ** step)).sqrt() + 1e-8)
+                w = w0 * (1 - group["lr"] * group["weight_decay"]) - update
+                # the norm's 10 units reach the moments, the rest as in test_train_gpu.py; m is a difference
+                rate = group["lr"] / (1 - 0.9 ** step) / ((v / (1 - 0.999 ** step)).sqrt() + 1e-8)
+                tol = 6 * U * w0.abs() + 48 * U * update.abs() + rate * 16 * U * (m0.abs() + g.abs())
+                assert bool(((new["master"].double().cpu() - w).abs() <= tol).all())
+                assert torch.equal(new["p"], new["master"].to(BF))
+                if bits == 32:
+                    assert rel(new["exp_avg"], m) <= 16 * U and rel(new["exp_avg_sq"], v) <= 32 * U
+                else:  # one unit at most: 1/8 and 1/4 of a value, or of the smallest normal one
+                    got_m, got_v = moments(fsw, new, "exp_avg"), moments(fsw, new, "exp_avg_sq")
+                    peak = lambda t: torch.nn.functional.pad(t.flatten().abs(), (0, -t.numel() % 256)).view(-1, 256).amax(1)  # noqa: E731
+                    per = lambda t: peak(t).repeat_interleave(256)[:t.numel()].view(t.shape)  # noqa: E731
+                    assert bool(((got_m - m).abs() <= m.abs() / 8 * 1.001 + per(m) * 2.0 ** -16).all())
+                    assert bool(((got_v - v).abs() <= v / 4 * 1.001 + per(v) * 2.0 ** -30).all())
+
+
+def test_optimizer_skips_a_step_with_a_bad_gradient(fsw, cuda_dev):
+    p = torch.nn.Parameter(torch.ones(300, device=cuda_dev, dtype=BF))
+    q = torch.nn.Parameter(torch.ones(30, device=cuda_dev))
+    opt = fsw.train.FusedAdamW([p, q], max_grad_norm=1.0)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt.step()
+    before = [values(opt, t) for t in (p, q)]
+    p.grad[7] = float("nan")
+    opt.step()
+    for t, old in zip((p, q), before):
+        assert all(torch.equal(old[k], v) for k, v in values(opt, t).items())
+    p.grad[7] = 1.0
+    opt.step()
+    assert not torch.equal(before[0]["master"], values(opt, p)["master"])
+
+
+def test_a_step_is_seen_by_autograd(fsw, cuda_dev):
+    """Weights that a step has changed are not those that an earlier forward pass kept."""
+    x = torch.randn(4, 64, device=cuda_dev, dtype=BF, requires_grad=True)
+    w = torch.nn.Parameter(torch.ones(64, device=cuda_dev, dtype=BF))
+    y = fsw.train.rms_norm(x, w)
+    w.grad = torch.ones_like(w)
+    fsw.train.FusedAdamW([w]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_whole_training_step_from_a_captured_graph(fsw, cuda_dev, bits):
+    """Two graphs of one step each, replayed in turn; both give what the eager step gives from the same state."""
+    from fused_swiglu_b200.module import NormSwiGLUBlock
+
+    torch.manual_seed(0)
+    block = NormSwiGLUBlock(128, 256, device=cuda_dev)
+    with torch.no_grad():
+        for p in (block.mlp.gate_proj, block.mlp.up_proj, block.mlp.down_proj):
+            p.normal_(0, 0.1)
+    opt = fsw.train.FusedAdamW(block.parameters(), lr=1e-2, state_bits=bits, max_grad_norm=1.0, capturable=True)
+    x = torch.randn(64, 128, device=cuda_dev, dtype=BF)
+
+    def train_step():
+        opt.zero_grad(set_to_none=False)
+        out = block(x)
+        out.backward(out.detach())
+        opt.step()
+
+    def state():
+        tensors = [p.data for p in block.parameters()]
+        for p in block.parameters():
+            tensors += [v for v in opt.state[p].values() if isinstance(v, torch.Tensor)]
+        return tensors + [opt.param_groups[0]["step_tensor"]]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            train_step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            train_step()
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for graph in (graphs[0], graphs[1], graphs[0]):
+        start = [t.clone() for t in state()]
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in state()]
+        for t, s in zip(state(), start):
+            t.copy_(s)
+        with torch.cuda.stream(side):
+            train_step()
+        torch.cuda.synchronize()
+        assert int(replayed[-1]) == int(start[-1]) + 1
+        for a, b in zip(state(), replayed):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

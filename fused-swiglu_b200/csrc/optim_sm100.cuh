@@ -17,9 +17,11 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cstdint>
 
 #include "ptx_sm100.cuh"
+#include "vector_io_sm100.cuh"
 
 namespace fsw {
 
@@ -36,7 +38,7 @@ struct AdamTensor {
   float* master;
   float* exp_avg_scale;
   float* exp_avg_sq_scale;
-  long long numel;
+  long long numel;  // negative (its complement) where some pointer is not aligned to eight of its elements
 };
 
 struct AdamOptions {
@@ -47,7 +49,6 @@ struct AdamOptions {
   const long long* step_device;
   const float* grad_scale;
   uint32_t seed_lo, seed_hi, step_lo;
-  int grad_dtype_f32;
 };
 
 template <int kCapacity>
@@ -102,25 +103,45 @@ __device__ __forceinline__ AdamRates adam_rates(const AdamOptions& o) {
   return r;
 }
 
-// m, v and p of one element.
-__device__ __forceinline__ void adam_element(const AdamOptions& o, const AdamRates& r, float g, float& m, float& v, float& p) {
+// m, v and p of one element from b1 m, b2 v and the gradient.  The root and the quotient are the fast ones, off by a few
+// units of fp32: p alone depends on them.
+__device__ __forceinline__ void adam_element(const AdamOptions& o, const AdamRates& r, float g, float old_m, float old_v,
+                                             float& m, float& v, float& p) {
   g = __fmul_rn(g, r.scale);
-  m = __fadd_rn(__fmul_rn(o.beta1, m), __fmul_rn(o.one_minus_beta1, g));
-  v = __fadd_rn(__fmul_rn(o.beta2, v), __fmul_rn(o.one_minus_beta2, __fmul_rn(g, g)));
-  const float root = sqrtf(v) * r.inv_sqrt_correction2 + o.eps;
-  p = p * r.decay - __fdividef(r.step_size * m, root);
+  m = __fadd_rn(old_m, __fmul_rn(o.one_minus_beta1, g));
+  v = __fadd_rn(old_v, __fmul_rn(o.one_minus_beta2, __fmul_rn(g, g)));
+  float root, quotient;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+  root = fmaf(root, r.inv_sqrt_correction2, o.eps);
+  asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(quotient) : "f"(r.step_size * m), "f"(root));
+  p = fmaf(p, r.decay, -quotient);
 }
 
 // ---- 8-bit floats with a block's scale ----
 
-__device__ __forceinline__ float decode_e4m3(uint32_t code, float scale) {
-  // the exponent of the 8-bit type moved to where fp32 has it, subnormal values too
-  const uint32_t bits = ((code & 0x7fu) << 20) | ((code & 0x80u) << 24);
-  return __uint_as_float(bits) * 0x1p120f * scale;
+// Values of eight codes, without the scale.
+__device__ __forceinline__ void decode_e4m3x8(uint2 q, float (&v)[kAdamGroup]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? q.x : q.y;
+    const uint16_t pair = static_cast<uint16_t>((i & 1) ? w >> 16 : w);
+    uint32_t halves;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&halves));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
-__device__ __forceinline__ float decode_e5m2(uint32_t code, float scale) {
-  return __uint_as_float(code << 21) * 0x1p112f * scale;
+// An e5m2 is the upper byte of a half.
+__device__ __forceinline__ void decode_e5m2x8(uint2 q, float (&v)[kAdamGroup]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t halves = __byte_perm(i < 2 ? q.x : q.y, 0u, (i & 1) ? 0x3424 : 0x1404);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&halves));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
 // The scale of a block whose largest magnitude has the fp32 bits `peak`, and its inverse; the largest value comes
@@ -131,16 +152,18 @@ __device__ __forceinline__ float2 block_scale(uint32_t peak, uint32_t top) {
   return make_float2(__uint_as_float((field - top) << 23), __uint_as_float((254u + top - field) << 23));
 }
 
-__device__ __forceinline__ uint32_t encode_e4m3(float m, float inverse, uint32_t random16) {
-  const float t = fabsf(m) * inverse * 0x1p-120f;
-  const uint32_t code = (__float_as_uint(t) + (random16 << 4)) >> 20;
-  return (code & 0x7fu) | (__float_as_uint(m) >> 31 << 7);
+// A value brought to where the exponents of the 8-bit type, its subnormal ones too, are those of fp32; then the bits that
+// the type keeps are the upper ones, and random bits added below them round up as often as the rest is large.
+__device__ __forceinline__ uint32_t encode_e4m3(float m, float inverse, uint32_t bits) {
+  const float t = m * inverse * 0x1p-120f;
+  const uint32_t x = (__float_as_uint(t) + ((bits & 0xffffu) << 4)) >> 20;  // sign in bit 11, code in bits 0 to 6
+  return (x & 0x7fu) | ((x >> 4) & 0x80u);
 }
 
-__device__ __forceinline__ uint32_t encode_e5m2(float v, float inverse, uint32_t random16) {
+__device__ __forceinline__ uint32_t encode_e5m2(float v, float inverse, uint32_t bits) {
   const float t = v * inverse * 0x1p-112f;
-  const uint32_t code = (__float_as_uint(t) + (random16 << 5)) >> 21;
-  return max(code, v > 0.0f ? 1u : 0u);
+  const uint32_t code = (__float_as_uint(t) + ((bits >> 16) << 5)) >> 21;
+  return max(code, min(__float_as_uint(v), 1u));
 }
 
 // The tensor that holds a chunk: the last whose first chunk is not behind it.
@@ -155,8 +178,54 @@ __device__ __forceinline__ int find_tensor(const uint32_t (&first)[kCapacity], i
   return lo;
 }
 
-// P: type of the parameters.  A warp takes one block of 256 elements at a time, each thread eight neighbours.
-template <typename P, bool kEight, int kCapacity>
+// Eight elements of one thread; `whole`: all of them exist and are reached by wide accesses.  A group at a tensor's end
+// or of an unaligned tensor goes element by element.
+template <typename T>
+__device__ __forceinline__ void load_group(const T* p, bool whole, int n, float (&v)[kAdamGroup]) {
+  if (whole) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) v[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_group(T* p, bool whole, int n, const float (&v)[kAdamGroup]) {
+  if (whole) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) {
+      if (i < n) p[i] = static_cast<T>(v[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool whole, int n) {
+  if (whole) return load_bytes8(p);
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < kAdamGroup; ++i) {
+    if (i < n) w[i >> 2] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* p, bool whole, int n, uint2 v) {
+  if (whole) {
+    store_bytes8(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kAdamGroup; ++i) {
+    if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
+  }
+}
+
+// P, G: types of parameters and gradients.  A warp takes one block of 256 elements at a time, each thread eight
+// neighbours, so that a block's largest magnitudes are one reduction over the warp.
+template <typename P, typename G, bool kEight, bool kMaster, int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
   const AdamOptions& o = t.opt;
   const AdamRates r = adam_rates(o);
@@ -165,61 +234,73 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
     const AdamTensor& a = t.tensors[k];
+    const bool vector = a.numel >= 0;
+    const long long numel = vector ? a.numel : ~a.numel;
     const long long base = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk;
-    for (int part = 0; part < 2; ++part) {
+#pragma unroll 1
+    for (int part = 0; part < kAdamChunk / (kAdamThreads * kAdamGroup); ++part) {
       const long long at = base + (part * kAdamThreads + threadIdx.x) * kAdamGroup;
-      const long long block = at / kAdamBlock;
-      float m[kAdamGroup], v[kAdamGroup];
-      uint32_t peak_m = 0, peak_v = 0;
+      if (numel <= at / kAdamBlock * kAdamBlock) break;  // the whole warp's block is behind the end
+      const long long left = numel - at;
+      const int n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
+      const bool whole = vector && n == kAdamGroup;
+      float m[kAdamGroup], v[kAdamGroup], p[kAdamGroup], g[kAdamGroup];
+      uint2 qm, qv;
       float sm = 0.0f, sv = 0.0f;
-      if (kEight && at < a.numel) {
-        sm = a.exp_avg_scale[block];
-        sv = a.exp_avg_sq_scale[block];
+      if (kEight) {
+        qm = load_codes(static_cast<const uint8_t*>(a.exp_avg) + at, whole, n);
+        qv = load_codes(static_cast<const uint8_t*>(a.exp_avg_sq) + at, whole, n);
+        if (n > 0) {
+          sm = a.exp_avg_scale[at / kAdamBlock];
+          sv = a.exp_avg_sq_scale[at / kAdamBlock];
+        }
+      } else {
+        load_group(static_cast<const float*>(a.exp_avg) + at, whole, n, m);
+        load_group(static_cast<const float*>(a.exp_avg_sq) + at, whole, n, v);
       }
+      load_group(static_cast<const G*>(a.grad) + at, whole, n, g);
+      if (kMaster) load_group(a.master + at, whole, n, p);
+      else load_group(static_cast<const P*>(a.param) + at, whole, n, p);
+      if (kEight) {
+        decode_e4m3x8(qm, m);
+        decode_e5m2x8(qv, v);
+      }
+      // the scale is a power of two: b times the scale, and that times the code, rounds as b times the value does
+      const float b1 = kEight ? o.beta1 * sm : o.beta1, b2 = kEight ? o.beta2 * sv : o.beta2;
+      uint32_t peak_m = 0, peak_v = 0;
 #pragma unroll
       for (int i = 0; i < kAdamGroup; ++i) {
-        m[i] = v[i] = 0.0f;
-        const long long e = at + i;
-        if (e < a.numel) {
-          if (kEight) {
-            m[i] = decode_e4m3(static_cast<const uint8_t*>(a.exp_avg)[e], sm);
-            v[i] = decode_e5m2(static_cast<const uint8_t*>(a.exp_avg_sq)[e], sv);
-          } else {
-            m[i] = static_cast<const float*>(a.exp_avg)[e];
-            v[i] = static_cast<const float*>(a.exp_avg_sq)[e];
-          }
-          const float g = o.grad_dtype_f32 ? static_cast<const float*>(a.grad)[e]
-                                           : __bfloat162float(static_cast<const __nv_bfloat16*>(a.grad)[e]);
-          float p = a.master != nullptr ? a.master[e] : static_cast<float>(static_cast<const P*>(a.param)[e]);
-          adam_element(o, r, g, m[i], v[i], p);
-          if (a.master != nullptr) a.master[e] = p;
-          static_cast<P*>(a.param)[e] = static_cast<P>(p);
-          if (!kEight) {
-            static_cast<float*>(a.exp_avg)[e] = m[i];
-            static_cast<float*>(a.exp_avg_sq)[e] = v[i];
-          }
+        adam_element(o, r, g[i], __fmul_rn(b1, m[i]), __fmul_rn(b2, v[i]), m[i], v[i], p[i]);
+        if (kEight) {
           peak_m = max(peak_m, __float_as_uint(m[i]) & 0x7fffffffu);
           peak_v = max(peak_v, __float_as_uint(v[i]) & 0x7fffffffu);
         }
       }
+      if (kMaster) store_group(a.master + at, whole, n, p);
+      store_group(static_cast<P*>(a.param) + at, whole, n, p);
       if (kEight) {
         peak_m = __reduce_max_sync(0xffffffffu, peak_m);
         peak_v = __reduce_max_sync(0xffffffffu, peak_v);
-        if (at >= a.numel) continue;
         const float2 cm = block_scale(peak_m, 7), cv = block_scale(peak_v, 14);
-        const unsigned long long group = (t.first_block[k] + block) * (kAdamBlock / kAdamGroup) + (threadIdx.x & 31);
+        const unsigned long long group =
+            (t.first_block[k] + at / kAdamBlock) * (kAdamBlock / kAdamGroup) + (threadIdx.x & 31);
         const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
-        if ((threadIdx.x & 31) == 0) {
-          a.exp_avg_scale[block] = cm.x;
-          a.exp_avg_sq_scale[block] = cv.x;
+        if ((threadIdx.x & 31) == 0 && n > 0) {
+          a.exp_avg_scale[at / kAdamBlock] = cm.x;
+          a.exp_avg_sq_scale[at / kAdamBlock] = cv.x;
         }
+        qm = qv = make_uint2(0u, 0u);
 #pragma unroll
         for (int i = 0; i < kAdamGroup; ++i) {
-          if (at + i >= a.numel) break;
           const uint32_t bits = h * odd_multiplier(i);
-          static_cast<uint8_t*>(a.exp_avg)[at + i] = static_cast<uint8_t>(encode_e4m3(m[i], cm.y, bits & 0xffffu));
-          static_cast<uint8_t*>(a.exp_avg_sq)[at + i] = static_cast<uint8_t>(encode_e5m2(v[i], cv.y, bits >> 16));
+          (i < 4 ? qm.x : qm.y) |= encode_e4m3(m[i], cm.y, bits) << (8 * (i & 3));
+          (i < 4 ? qv.x : qv.y) |= (encode_e5m2(v[i], cv.y, bits) & 0xffu) << (8 * (i & 3));
         }
+        store_codes(static_cast<uint8_t*>(a.exp_avg) + at, whole, n, qm);
+        store_codes(static_cast<uint8_t*>(a.exp_avg_sq) + at, whole, n, qv);
+      } else {
+        store_group(static_cast<float*>(a.exp_avg) + at, whole, n, m);
+        store_group(static_cast<float*>(a.exp_avg_sq) + at, whole, n, v);
       }
     }
   }
@@ -233,6 +314,7 @@ struct GradTensor {
   const void* grad;
   long long numel;
   int f32;
+  int vector;  // aligned to eight elements
 };
 
 template <int kCapacity>
@@ -263,15 +345,22 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_co
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
     const GradTensor& a = t.tensors[k];
-    const long long base = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk;
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < kAdamChunk; i += kAdamThreads) {
-      if (base + i < a.numel) {
-        const float g = a.f32 ? static_cast<const float*>(a.grad)[base + i]
-                              : __bfloat162float(static_cast<const __nv_bfloat16*>(a.grad)[base + i]);
-        s = fmaf(g, g, s);
-      }
+    const long long at = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk + threadIdx.x * kAdamGroup;
+    float g[2][kAdamGroup];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const long long e = at + part * kAdamThreads * kAdamGroup;
+      const long long left = a.numel - e;
+      const int n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
+      const bool whole = a.vector && n == kAdamGroup;
+      if (a.f32) load_group(static_cast<const float*>(a.grad) + e, whole, n, g[part]);
+      else load_group(static_cast<const __nv_bfloat16*>(a.grad) + e, whole, n, g[part]);
     }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) s = fmaf(g[0][i], g[0][i], s);
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) s = fmaf(g[1][i], g[1][i], s);
     sum += static_cast<double>(s);
   }
   sum = block_sum(sum, shared);

@@ -28,7 +28,8 @@ int launched() {
 
 // ---- norms ----
 
-constexpr int64_t kMaxNormWidth = 1 << 24;  // a row's length is exact in fp32
+constexpr int64_t kMaxNormWidth = 1 << 24;                // a row's length is exact in fp32
+constexpr int64_t kMaxNormRows = 0x7fffffff - (1 << 20);  // a row behind the last one is still an int
 constexpr int kMaxNormSplits = 296;         // two thread blocks for each of 148 SMs
 
 int check_rows(const void* p, int64_t M, int64_t d, int64_t ld, int type) {
@@ -39,30 +40,95 @@ int check_rows(const void* p, int64_t M, int64_t d, int64_t ld, int type) {
 
 int check_norm(int64_t M, int64_t d, int x_dtype, int w_dtype) {
   if (M < 0 || d <= 0 || !known_type(x_dtype) || !known_type(w_dtype)) return FSWIGLU_ERR_BAD_ARG;
-  if (M > 0x7fffffffll || d > kMaxNormWidth) return FSWIGLU_ERR_SHAPE;
+  if (M > kMaxNormRows || d > kMaxNormWidth) return FSWIGLU_ERR_SHAPE;
   return FSWIGLU_OK;
 }
 
 int norm_splits(int64_t M) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(M, kMaxNormSplits))); }
 
-template <typename T, bool kLayer>
-int launch_norm_forward(const NormForwardParams& p, int sms, cudaStream_t s) {
-  const int grid = static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8));
-  norm_forward_any_kernel<T, kLayer><<<grid, kNormThreads, 0, s>>>(p);
+// How a width is laid out over threads: groups of `group` threads hold a row, `groups` of them make a block.
+struct RowShape {
+  int vectors;  // of a thread; 0: the width is too large for registers
+  int group, groups;
+};
+
+// Shape for rows of `units` vectors, at most `most` vectors a thread (a power of two) and `threads` threads a block.
+RowShape row_shape(int64_t units, int64_t M, int most, int threads) {
+  RowShape r = {0, 0, 0};
+  int n = 1;
+  while (n < most && units > 32 * n) n *= 2;
+  const int64_t group = (units + 32 * n - 1) / (32 * n) * 32;
+  if (group > threads) return r;
+  r.vectors = n;
+  r.group = static_cast<int>(group);
+  r.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({threads / group, kNormGroups, M})));
+  return r;
+}
+
+template <typename T, bool kLayer, int V, int N>
+int launch_norm_forward_rows(const NormForwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
+  const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
+  const int64_t resident = static_cast<int64_t>(sms) * std::max(1, 1536 / (r.group * r.groups));
+  norm_forward_rows_kernel<T, kLayer, V, N>
+      <<<static_cast<int>(std::min(blocks, resident)), dim3(r.group, r.groups), 0, s>>>(p);
   return launched();
 }
 
 template <typename T, bool kLayer>
-int launch_norm_backward(const NormBackwardParams& p, bool columns, int sms, cudaStream_t s) {
-  const int grid = static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8));
-  norm_backward_any_kernel<T, kLayer><<<grid, kNormThreads, 0, s>>>(p);
+int launch_norm_forward(const NormForwardParams& p, bool wide, int sms, cudaStream_t s) {
+  if (wide) {
+    const RowShape r = row_shape(p.d / 8, p.M, 4, 256);
+    if (r.vectors == 1) return launch_norm_forward_rows<T, kLayer, 8, 1>(p, r, sms, s);
+    if (r.vectors == 2) return launch_norm_forward_rows<T, kLayer, 8, 2>(p, r, sms, s);
+    if (r.vectors == 4) return launch_norm_forward_rows<T, kLayer, 8, 4>(p, r, sms, s);
+  } else {
+    const RowShape r = row_shape(p.d, p.M, 16, 512);
+    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_forward_rows<T, kLayer, 1, 2>(p, r, sms, s);
+    if (r.vectors > 2 && r.vectors <= 8) return launch_norm_forward_rows<T, kLayer, 1, 8>(p, r, sms, s);
+    if (r.vectors == 16) return launch_norm_forward_rows<T, kLayer, 1, 16>(p, r, sms, s);
+  }
+  norm_forward_any_kernel<T, kLayer>
+      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8)), kNormThreads, 0, s>>>(p);
+  return launched();
+}
+
+template <typename T, bool kLayer, int V, int N>
+int launch_norm_backward_rows(NormBackwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
+  const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
+  const int64_t resident = std::min<int64_t>(static_cast<int64_t>(sms) * std::max(1, 512 / (r.group * r.groups)), kMaxNormSplits);
+  const int grid = static_cast<int>(std::min(blocks, resident));
+  p.splits = grid;
+  const size_t shared = r.groups > 1 ? static_cast<size_t>(2) * r.group * V * N * sizeof(float) : 0;
+  norm_backward_rows_kernel<T, kLayer, V, N><<<grid, dim3(r.group, r.groups), shared, s>>>(p);
+  return launched();
+}
+
+template <typename T, bool kLayer>
+int launch_norm_backward(NormBackwardParams& p, bool wide, int sms, cudaStream_t s) {
+  if (wide) {
+    const RowShape r = row_shape(p.d / 8, p.M, 2, 512);
+    if (r.vectors == 1) return launch_norm_backward_rows<T, kLayer, 8, 1>(p, r, sms, s);
+    if (r.vectors == 2) return launch_norm_backward_rows<T, kLayer, 8, 2>(p, r, sms, s);
+  } else {
+    const RowShape r = row_shape(p.d, p.M, 8, 512);
+    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_backward_rows<T, kLayer, 1, 2>(p, r, sms, s);
+    if (r.vectors > 2) return launch_norm_backward_rows<T, kLayer, 1, 8>(p, r, sms, s);
+  }
+  norm_backward_any_kernel<T, kLayer>
+      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8)), kNormThreads, 0, s>>>(p);
   if (int rc = launched()) return rc;
-  if (!columns) return FSWIGLU_OK;
+  if (p.partial == nullptr) return FSWIGLU_OK;
   const int64_t tiles = (p.d + kNormThreads - 1) / kNormThreads * static_cast<int64_t>(p.splits);
   norm_backward_columns_any_kernel<T, kLayer>
       <<<static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(sms) * 32)), kNormThreads, 0, s>>>(p);
   return launched();
 }
+
+// Whether a matrix's rows, or a vector, take the wide accesses of eight elements.
+bool wide_rows(const void* p, int64_t ld, int64_t M, int type) {
+  return aligned(p, type == FSWIGLU_OUT_F32 ? 32 : 16) && (ld % 8 == 0 || M == 1);
+}
+bool wide_vector(const void* p, int type) { return aligned(p, type == FSWIGLU_OUT_F32 ? 32 : 16); }
 
 int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, const void* bias, void* y, int64_t ldy,
                  float* mean, float* rstd, int64_t M, int64_t d, int x_dtype, int w_dtype, float eps, void* stream) {
@@ -89,10 +155,13 @@ int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, con
   p.d = static_cast<int>(d);
   p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
   p.eps = eps;
+  const bool wide = d % 8 == 0 && wide_rows(x, ldx, M, x_dtype) && wide_rows(y, ldy, M, x_dtype) &&
+                    wide_vector(weight, w_dtype) && wide_vector(bias, w_dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  using BF = __nv_bfloat16;
   if (x_dtype == FSWIGLU_OUT_F32)
-    return layer ? launch_norm_forward<float, true>(p, sms, s) : launch_norm_forward<float, false>(p, sms, s);
-  return layer ? launch_norm_forward<__nv_bfloat16, true>(p, sms, s) : launch_norm_forward<__nv_bfloat16, false>(p, sms, s);
+    return layer ? launch_norm_forward<float, true>(p, wide, sms, s) : launch_norm_forward<float, false>(p, wide, sms, s);
+  return layer ? launch_norm_forward<BF, true>(p, wide, sms, s) : launch_norm_forward<BF, false>(p, wide, sms, s);
 }
 
 int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* mean,
@@ -128,7 +197,7 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     p.mean = mean;
     p.rstd = rstd;
     p.dx = dx;
-    p.partial = static_cast<float*>(workspace);
+    p.partial = columns ? static_cast<float*>(workspace) : nullptr;
     p.ld_dout = ld_dout;
     p.ldx = ldx;
     p.ld_res = ld_res;
@@ -137,12 +206,15 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     p.d = static_cast<int>(d);
     p.splits = norm_splits(M);
     p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
+    const bool wide = d % 8 == 0 && wide_rows(dout, ld_dout, M, x_dtype) && wide_rows(x, ldx, M, x_dtype) &&
+                      wide_rows(dx, ld_dx, M, x_dtype) && wide_rows(residual, residual == nullptr ? 0 : ld_res, M, x_dtype) &&
+                      wide_vector(weight, w_dtype);
+    using BF = __nv_bfloat16;
     int rc;
     if (x_dtype == FSWIGLU_OUT_F32)
-      rc = layer ? launch_norm_backward<float, true>(p, columns, sms, s) : launch_norm_backward<float, false>(p, columns, sms, s);
+      rc = layer ? launch_norm_backward<float, true>(p, wide, sms, s) : launch_norm_backward<float, false>(p, wide, sms, s);
     else
-      rc = layer ? launch_norm_backward<__nv_bfloat16, true>(p, columns, sms, s)
-                 : launch_norm_backward<__nv_bfloat16, false>(p, columns, sms, s);
+      rc = layer ? launch_norm_backward<BF, true>(p, wide, sms, s) : launch_norm_backward<BF, false>(p, wide, sms, s);
     if (rc) return rc;
   }
   if (!columns) return FSWIGLU_OK;
@@ -153,7 +225,9 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
   q.d = static_cast<int>(d);
   q.splits = p.splits;
   q.out_f32 = grad_dtype == FSWIGLU_OUT_F32;
-  norm_reduce_kernel<<<static_cast<int>((d + kNormThreads - 1) / kNormThreads), kNormThreads, 0, s>>>(q);
+  const int grid = static_cast<int>((d + 31) / 32);
+  if (dbias != nullptr) norm_reduce_kernel<true><<<grid, dim3(32, kNormReduceRows), 0, s>>>(q);
+  else norm_reduce_kernel<false><<<grid, dim3(32, kNormReduceRows), 0, s>>>(q);
   return launched();
 }
 
@@ -202,16 +276,41 @@ uint32_t chunks_of(int64_t numel) { return static_cast<uint32_t>((numel + kAdamC
 
 constexpr int64_t kMaxNumel = 1ll << 35;  // chunks of a full table are counted in 32 bits
 
-template <typename P, bool kEight, int kCapacity>
+template <typename P, typename G, bool kEight, bool kMaster, int kCapacity>
 int launch_adamw(const AdamTable<kCapacity>& t, int sms, cudaStream_t s) {
   const uint32_t grid = std::min<uint32_t>(t.first_chunk[t.count], static_cast<uint32_t>(sms) * 8u);
-  adamw_kernel<P, kEight, kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
+  adamw_kernel<P, G, kEight, kMaster, kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
   return launched();
 }
 
+struct AdamKind {
+  bool param_f32, grad_f32, eight, master;
+};
+
+template <typename P, typename G, int kCapacity>
+int launch_adamw(const AdamTable<kCapacity>& t, const AdamKind& k, int sms, cudaStream_t s) {
+  if constexpr (sizeof(P) == 2) {
+    if (k.master) return k.eight ? launch_adamw<P, G, true, true>(t, sms, s) : launch_adamw<P, G, false, true>(t, sms, s);
+  }
+  return k.eight ? launch_adamw<P, G, true, false>(t, sms, s) : launch_adamw<P, G, false, false>(t, sms, s);
+}
+
 template <int kCapacity>
-int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const AdamOptions& o, int param_dtype, int state_bits,
-                   int sms, cudaStream_t s) {
+int launch_adamw(const AdamTable<kCapacity>& t, const AdamKind& k, int sms, cudaStream_t s) {
+  using BF = __nv_bfloat16;
+  if (k.param_f32) return k.grad_f32 ? launch_adamw<float, float>(t, k, sms, s) : launch_adamw<float, BF>(t, k, sms, s);
+  return k.grad_f32 ? launch_adamw<BF, float>(t, k, sms, s) : launch_adamw<BF, BF>(t, k, sms, s);
+}
+
+// Whether every pointer of a tensor takes the wide accesses of eight elements.
+bool wide(const fswiglu_adamw_tensor& a, const AdamKind& k) {
+  const size_t p = k.param_f32 ? 32 : 16, g = k.grad_f32 ? 32 : 16, m = k.eight ? 8 : 32;
+  return aligned(a.param, p) && aligned(a.grad, g) && aligned(a.exp_avg, m) && aligned(a.exp_avg_sq, m) && aligned(a.master, 32);
+}
+
+template <int kCapacity>
+int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const AdamOptions& o, AdamKind kind, int sms,
+                   cudaStream_t s) {
   AdamTable<kCapacity> t;
   t.opt = o;
   t.count = 0;
@@ -220,20 +319,22 @@ int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const Ada
   for (int64_t i = 0; i < count; ++i) {
     const fswiglu_adamw_tensor& a = tensors[i];
     if (a.numel > 0) {
+      // one launch's tensors all have a master or none has
+      if (t.count > 0 && (a.master != nullptr) != kind.master) {
+        if (int rc = launch_adamw<kCapacity>(t, kind, sms, s)) return rc;
+        t.count = 0;
+      }
+      kind.master = a.master != nullptr;
+      const long long n = a.numel;
       t.tensors[t.count] = AdamTensor{a.param,  a.grad, a.exp_avg, a.exp_avg_sq, a.master, a.exp_avg_scale,
-                                      a.exp_avg_sq_scale, static_cast<long long>(a.numel)};
+                                      a.exp_avg_sq_scale, wide(a, kind) ? n : ~n};
       t.first_block[t.count] = blocks;
       t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(a.numel);
       blocks += (a.numel + kAdamBlock - 1) / kAdamBlock;
       ++t.count;
     }
     if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
-    int rc;
-    if (param_dtype == FSWIGLU_OUT_F32)
-      rc = state_bits == 8 ? launch_adamw<float, true>(t, sms, s) : launch_adamw<float, false>(t, sms, s);
-    else
-      rc = state_bits == 8 ? launch_adamw<__nv_bfloat16, true>(t, sms, s) : launch_adamw<__nv_bfloat16, false>(t, sms, s);
-    if (rc) return rc;
+    if (int rc = launch_adamw<kCapacity>(t, kind, sms, s)) return rc;
     t.count = 0;
   }
   return FSWIGLU_OK;
@@ -248,8 +349,9 @@ int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double
   t.accumulate = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (tensors[i].numel > 0) {
-      t.tensors[t.count] = GradTensor{tensors[i].grad, static_cast<long long>(tensors[i].numel),
-                                      tensors[i].dtype == FSWIGLU_OUT_F32};
+      const bool f32 = tensors[i].dtype == FSWIGLU_OUT_F32;
+      t.tensors[t.count] = GradTensor{tensors[i].grad, static_cast<long long>(tensors[i].numel), f32,
+                                      aligned(tensors[i].grad, f32 ? 32 : 16)};
       t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(tensors[i].numel);
       ++t.count;
     }
@@ -360,10 +462,10 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
   o.seed_lo = static_cast<uint32_t>(in.seed);
   o.seed_hi = static_cast<uint32_t>(in.seed >> 32);
   o.step_lo = static_cast<uint32_t>(in.step);
-  o.grad_dtype_f32 = grad_dtype == FSWIGLU_OUT_F32;
+  const AdamKind kind = {param_dtype == FSWIGLU_OUT_F32, grad_dtype == FSWIGLU_OUT_F32, state_bits == 8, false};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, param_dtype, state_bits, sms, s)
-                              : adamw_launches<kLargeTable>(tensors, count, o, param_dtype, state_bits, sms, s);
+  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, kind, sms, s)
+                              : adamw_launches<kLargeTable>(tensors, count, o, kind, sms, s);
 }
 
 size_t fswiglu_grad_norm_workspace_bytes(void) { return kGradNormSlots * sizeof(double); }

@@ -860,12 +860,14 @@ int mlp_impl(DeviceState& st, const void* x, int64_t ldx, const void* w_gate, co
 
 namespace fsw {
 
-int current_device_sms(int* num_sms) {
+int current_device(Device* out) {
   DeviceState* st = nullptr;
   if (int rc = device_state(&st)) return rc;
-  *num_sms = st->num_sms;
+  *out = Device{static_cast<int>(st - g_dev), st->num_sms, st->status, g_wait_limit_ns.load(std::memory_order_relaxed)};
   return FSWIGLU_OK;
 }
+
+bool take_withhold() { return g_withhold_one_copy.exchange(0, std::memory_order_relaxed) != 0; }
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 

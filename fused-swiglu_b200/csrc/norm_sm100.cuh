@@ -10,9 +10,18 @@
 #include <cuda_bf16.h>
 #include <cstdint>
 
+#include "ptx_sm100.cuh"
 #include "vector_io_sm100.cuh"
 
 namespace fsw {
+
+// Of the kernels that wait for rows on their way (below).
+struct RingParams {
+  uint32_t* status;  // where a wait that gave up is recorded
+  unsigned long long wait_limit_ns;
+  int places;
+  int withhold;  // test aid: the first row of all is never copied
+};
 
 struct NormForwardParams {
   const void* x;
@@ -25,6 +34,8 @@ struct NormForwardParams {
   int M, d;
   int w_f32;  // weight and bias are fp32, not bf16
   float eps;
+  long long y_step;  // bytes from a group's row to its next
+  RingParams ring;
 };
 
 struct NormBackwardParams {
@@ -39,6 +50,8 @@ struct NormBackwardParams {
   long long ld_dout, ldx, ld_res, ld_dx;
   int M, d, splits;
   int w_f32;
+  long long dx_step;  // bytes from a group's row to its next
+  RingParams ring;
 };
 
 struct NormReduceParams {
@@ -151,6 +164,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_any_kernel(const N
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_backward_columns_any_kernel(const NormBackwardParams p) {
   const long long tiles = (p.d + kNormThreads - 1) / kNormThreads;
+  let_next_start();
   for (long long t = blockIdx.x; t < tiles * p.splits; t += gridDim.x) {
     const int split = static_cast<int>(t / tiles);
     const int i = static_cast<int>(t % tiles) * kNormThreads + threadIdx.x;
@@ -172,117 +186,89 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_columns_any_kernel
 
 // ---- rows held in registers ----
 //
-// blockDim.x threads (a multiple of 32) hold one row, N vectors of V values each, and blockDim.y such groups of a block
-// take rows of their own; a group's next row is on its way while the present one is reduced.  A row is read once.
+// For rows that start on no 16-byte boundary: element by element.  blockDim.x threads (a multiple of 32) hold one row, N
+// values each, and blockDim.y such groups of a block take rows of their own; a group's next row is on its way while the
+// present one is reduced.  A row is read once.
 
-// Sum over a group, in a fixed order, known to its threads.  A group has two sets of slots and takes them in turn: who
-// writes one again has passed the barrier of the other, which all reached after they had read the first.
-__device__ __forceinline__ float2 group_sum(float2 v, float2* slots) {
+constexpr int kNarrowGroups = 8;     // most groups of a block: each has a barrier of its own
+constexpr int kNarrowThreads = 512;  // most threads of a block
+
+__device__ __forceinline__ void group_barrier() {
+  asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+}
+
+// Two sums over a group, in a fixed order, known to its threads; kPair: of both parts, else of y alone.  `span`: the group's
+// warps, rounded up to a power of two.  A group has two sets of slots and takes them in turn: who writes one again has
+// passed the barrier of the other, which all reached after they had read the first.
+template <bool kPair>
+__device__ __forceinline__ float2 group_sums(float2 v, float2* slots, int span) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    if (kPair) v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
-  float2 s = slots[0];
-  for (int w = 1; w < warps; ++w) {
-    s.x += slots[w].x;
-    s.y += slots[w].y;
+  if (span == 1) return v;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) slots[threadIdx.x >> 5] = v;
+  group_barrier();
+  const int at = lane & (span - 1);
+  v = at < warps ? slots[at] : make_float2(0.0f, 0.0f);
+  for (int o = span >> 1; o > 0; o >>= 1) {
+    if (kPair) v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  return s;
+  return v;
 }
 
-constexpr int kNormGroups = 8;       // most groups of a block
-constexpr int kNormRowThreads = 512;  // most threads of a block
+__device__ __forceinline__ int round_up_pow2(int v) { return v <= 1 ? 1 : 1 << (32 - __clz(v - 1)); }
 
-template <typename T, int V, int N>
-__device__ __forceinline__ void load_row(RawVector<T, V> (&raw)[N], const T* row, int d) {
+template <typename T, bool kLayer, int N>
+__global__ void __launch_bounds__(kNarrowThreads) norm_forward_narrow_kernel(const NormForwardParams p) {
+  __shared__ float2 slots[kNarrowGroups][2][32];
+  float w[N], b[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-    if (c < d) raw[j].load(row + c);
+    const int c = j * blockDim.x + threadIdx.x;
+    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
+    b[j] = kLayer && c < p.d ? load_vector(p.bias, c, p.w_f32, 0.0f) : 0.0f;
   }
-}
-
-// A weight or bias vector's values of this thread, and `none` where there are none.
-template <int V, int N>
-__device__ __forceinline__ void load_columns(float (&v)[N * V], const void* p, int f32, int d, float none) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[j * V + i] = none;
-    if (p != nullptr && c < d) {
-      if (f32) {
-        RawVector<float, V> r;
-        r.load(static_cast<const float*>(p) + c);
-        r.get(v + j * V);
-      } else {
-        RawVector<__nv_bfloat16, V> r;
-        r.load(static_cast<const __nv_bfloat16*>(p) + c);
-        r.get(v + j * V);
-      }
-    }
-  }
-}
-
-template <typename T, bool kLayer, int V, int N>
-__global__ void __launch_bounds__(kNormRowThreads) norm_forward_rows_kernel(const NormForwardParams p) {
-  __shared__ float2 slots[kNormGroups][2][kNormRowThreads / 32];
-  float w[N * V], b[N * V];
-  load_columns<V, N>(w, p.weight, p.w_f32, p.d, 1.0f);
-  if (kLayer) load_columns<V, N>(b, p.bias, p.w_f32, p.d, 0.0f);
   const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int stride = gridDim.x * blockDim.y;
+  const int span = round_up_pow2(blockDim.x >> 5), stride = gridDim.x * blockDim.y;
+  float2(&mine)[2][32] = slots[span > 1 ? threadIdx.y : 0];
   int row = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  RawVector<T, V> raw[N];
-  if (row < p.M) load_row<T, V, N>(raw, static_cast<const T*>(p.x) + row * p.ldx, p.d);
-  for (; row < p.M; row += stride) {
-    float x[N * V];
+  T raw[N];
+  auto fetch = [&](int r) {
+    const T* x = static_cast<const T*>(p.x) + r * p.ldx;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[j * V + i] = 0.0f;
-      if ((j * blockDim.x + threadIdx.x) * V < p.d) raw[j].get(x + j * V);
+      const int c = j * blockDim.x + threadIdx.x;
+      raw[j] = c < p.d ? x[c] : from_float<T>(0.0f);
     }
-    if (row < p.M - stride) load_row<T, V, N>(raw, static_cast<const T*>(p.x) + (row + stride) * p.ldx, p.d);
-    float mean = 0.0f;
-    if (kLayer) {
-      float s = 0.0f;
+  };
+  if (row < p.M) fetch(row);
+  for (; row < p.M; row += stride) {
+    float x[N], s = 0.0f, ss = 0.0f, mean = 0.0f;
 #pragma unroll
-      for (int i = 0; i < N * V; ++i) s += x[i];
-      mean = group_sum(make_float2(s, 0.0f), slots[threadIdx.y][turn]).x * inv_d;
+    for (int j = 0; j < N; ++j) x[j] = to_float<T>(raw[j]);
+    if (row < p.M - stride) fetch(row + stride);
+    if (kLayer) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += x[j];
+      mean = group_sums<false>(make_float2(0.0f, s), mine[turn], span).y * inv_d;
       turn ^= 1;
     }
-    float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if ((j * blockDim.x + threadIdx.x) * V < p.d) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[j * V + i] -= mean;
-          ss = fmaf(x[j * V + i], x[j * V + i], ss);
-        }
-      }
+      x[j] = static_cast<int>(j * blockDim.x + threadIdx.x) < p.d ? x[j] - mean : 0.0f;
+      ss = fmaf(x[j], x[j], ss);
     }
-    const float rstd = rsqrtf(fmaf(group_sum(make_float2(ss, 0.0f), slots[threadIdx.y][turn]).x, inv_d, p.eps));
+    const float rstd = rsqrtf(fmaf(group_sums<false>(make_float2(0.0f, ss), mine[turn], span).y, inv_d, p.eps));
     turn ^= 1;
     T* y = static_cast<T*>(p.y) + row * p.ldy;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c < p.d) {
-        float out[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float z = x[j * V + i] * rstd;
-          out[i] = kLayer ? fmaf(z, w[j * V + i], b[j * V + i]) : z * w[j * V + i];
-        }
-        store_vector<V, T>(y + c, out);
-      }
+      const int c = j * blockDim.x + threadIdx.x;
+      if (c < p.d) y[c] = from_float<T>(fmaf(x[j] * rstd, w[j], b[j]));
     }
     if (threadIdx.x == 0) {
       if (kLayer) p.mean[row] = mean;
@@ -293,105 +279,638 @@ __global__ void __launch_bounds__(kNormRowThreads) norm_forward_rows_kernel(cons
 
 // dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
 // block are joined in shared memory, and the blocks by norm_reduce_kernel.
-template <typename T, bool kLayer, int V, int N>
-__global__ void __launch_bounds__(kNormRowThreads) norm_backward_rows_kernel(const NormBackwardParams p) {
-  __shared__ float2 slots[kNormGroups][2][kNormRowThreads / 32];
+template <typename T, bool kLayer, int N>
+__global__ void __launch_bounds__(kNarrowThreads) norm_backward_narrow_kernel(const NormBackwardParams p) {
+  __shared__ float2 slots[kNarrowGroups][2][32];
   extern __shared__ float joined[];  // [2][columns of a group], more than one group only
-  float w[N * V], dw[N * V], db[kLayer ? N * V : 1];
-  load_columns<V, N>(w, p.weight, p.w_f32, p.d, 1.0f);
+  let_next_start();
+  float w[N], dw[N], db[kLayer ? N : 1];
 #pragma unroll
-  for (int i = 0; i < N * V; ++i) dw[i] = 0.0f;
-  if (kLayer) {
-#pragma unroll
-    for (int i = 0; i < N * V; ++i) db[i] = 0.0f;
+  for (int j = 0; j < N; ++j) {
+    const int c = j * blockDim.x + threadIdx.x;
+    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
+    dw[j] = 0.0f;
+    if (kLayer) db[j] = 0.0f;
   }
   const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int stride = gridDim.x * blockDim.y;
+  const int span = round_up_pow2(blockDim.x >> 5), stride = gridDim.x * blockDim.y;
+  float2(&mine)[2][32] = slots[span > 1 ? threadIdx.y : 0];
   int row = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  RawVector<T, V> raw_x[N], raw_dy[N], raw_res[N];
+  T raw_x[N], raw_dy[N], raw_res[N];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch = [&](int r) {
-    load_row<T, V, N>(raw_x, static_cast<const T*>(p.x) + r * p.ldx, p.d);
-    load_row<T, V, N>(raw_dy, static_cast<const T*>(p.dout) + r * p.ld_dout, p.d);
-    if (p.residual != nullptr) load_row<T, V, N>(raw_res, static_cast<const T*>(p.residual) + r * p.ld_res, p.d);
+    const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+    const T* dy = static_cast<const T*>(p.dout) + r * p.ld_dout;
+    const T* res = p.residual != nullptr ? static_cast<const T*>(p.residual) + r * p.ld_res : nullptr;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      raw_x[j] = c < p.d ? x[c] : from_float<T>(0.0f);
+      raw_dy[j] = c < p.d ? dy[c] : from_float<T>(0.0f);
+      raw_res[j] = c < p.d && res != nullptr ? res[c] : from_float<T>(0.0f);
+    }
     if (kLayer) next_mean = p.mean[r];
     next_rstd = p.rstd[r];
   };
   if (row < p.M) fetch(row);
   for (; row < p.M; row += stride) {
-    float z[N * V], a[N * V];
+    float z[N], a[N], res[N];
     const float mean = next_mean, rstd = next_rstd;
-    RawVector<T, V> res[N];
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) z[j * V + i] = a[j * V + i] = 0.0f;
-      if ((j * blockDim.x + threadIdx.x) * V < p.d) {
-        raw_x[j].get(z + j * V);
-        raw_dy[j].get(a + j * V);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int k = j * V + i;
-          z[k] = (z[k] - mean) * rstd;
-          dw[k] = fmaf(a[k], z[k], dw[k]);
-          if (kLayer) db[k] += a[k];
-          a[k] *= w[k];
-          s.x += a[k];
-          s.y = fmaf(a[k], z[k], s.y);
-        }
-      }
-      res[j] = raw_res[j];
+      // behind the row's end a is zero, and with it all that is summed
+      z[j] = (to_float<T>(raw_x[j]) - mean) * rstd;
+      a[j] = to_float<T>(raw_dy[j]);
+      res[j] = to_float<T>(raw_res[j]);
+      dw[j] = fmaf(a[j], z[j], dw[j]);
+      if (kLayer) db[j] += a[j];
+      a[j] *= w[j];
+      s.x += a[j];
+      s.y = fmaf(a[j], z[j], s.y);
     }
     if (row < p.M - stride) fetch(row + stride);
-    s = group_sum(s, slots[threadIdx.y][turn]);
+    s = group_sums<kLayer>(s, mine[turn], span);
     turn ^= 1;
     const float c1 = kLayer ? s.x * inv_d : 0.0f, c2 = s.y * inv_d;
     T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * V;
-      if (c < p.d) {
-        float out[V], add[V];
-        if (p.residual != nullptr) res[j].get(add);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int k = j * V + i;
-          const float t = fmaf(-z[k], c2, kLayer ? a[k] - c1 : a[k]);
-          out[i] = p.residual != nullptr ? fmaf(t, rstd, add[i]) : t * rstd;
-        }
-        store_vector<V, T>(dx + c, out);
-      }
+      const int c = j * blockDim.x + threadIdx.x;
+      if (c < p.d) dx[c] = from_float<T>(fmaf(fmaf(-z[j], c2, a[j] - c1), rstd, res[j]));
     }
   }
   if (p.partial == nullptr) return;
   float* part = p.partial + 2ll * blockIdx.x * p.d;
-  const int columns = blockDim.x * N * V;
+  const int columns = blockDim.x * N;
   for (int g = 0; g < static_cast<int>(blockDim.y); ++g) {
     if (static_cast<int>(threadIdx.y) == g) {
       const bool last = g + 1 == static_cast<int>(blockDim.y);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int c = (j * blockDim.x + threadIdx.x) * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int k = j * V + i;
-          if (g > 0) {
-            dw[k] += joined[c + i];
-            if (kLayer) db[k] += joined[columns + c + i];
-          }
-          if (!last) {
-            joined[c + i] = dw[k];
-            if (kLayer) joined[columns + c + i] = db[k];
-          }
+        const int c = j * blockDim.x + threadIdx.x;
+        if (g > 0) {
+          dw[j] += joined[c];
+          if (kLayer) db[j] += joined[columns + c];
         }
-        if (last && c < p.d) {
-          store_vector<V, float>(part + c, dw + j * V);
-          if (kLayer) store_vector<V, float>(part + p.d + c, db + j * V);
+        if (!last) {
+          joined[c] = dw[j];
+          if (kLayer) joined[columns + c] = db[j];
+        } else if (c < p.d) {
+          part[c] = dw[j];
+          if (kLayer) part[p.d + c] = db[j];
         }
       }
     }
     if (blockDim.y > 1) __syncthreads();
+  }
+}
+
+// ---- rows through shared memory ----
+//
+// The wide form.  A group of blockDim.x threads (a multiple of 32) takes one row at a time, a block has blockDim.y groups, and
+// a group's rows to come are on their way into its ring of S places: one thread asks for a row's arrays by bulk copies, S - 1
+// rows ahead, and all wait for their bytes on the place's barrier.  The bytes on the way cost neither registers, which the sums
+// over rows need, nor instructions of the threads that compute.  A place is free again once the group has met in the next
+// row's reduction.
+
+constexpr int kWideGroups = 24;       // most groups of a block, those of one warp
+constexpr int kWideMultiGroups = 8;   // most groups of more than one warp: each has a barrier of its own
+constexpr int kWidePlaces = 4;         // most places of a ring
+
+struct WideShared {
+  __align__(16) unsigned long long full[kWideGroups][kWidePlaces];
+  float2 slots[kWideMultiGroups][2][32];  // of each warp of a group, in turn
+  uint32_t abort_flag;
+};
+
+// A group's ring: `places` places of kArrays rows of `row_bytes`.  The present row's place and its barrier's phase advance
+// row by row.
+template <int kArrays>
+struct RowRing {
+  uint32_t data, bars, place_bytes, array_bytes, row_bytes;
+  int places, at;
+  uint32_t phase;
+  Watchdog wd;
+
+  __device__ __forceinline__ RowRing(WideShared& sh, unsigned char* ring, uint32_t slot_bytes, uint32_t bytes, const RingParams& p)
+      : array_bytes(slot_bytes), row_bytes(bytes), places(p.places), at(0), phase(0),
+        wd{&sh.abort_flag, p.status, p.wait_limit_ns} {
+    place_bytes = kArrays * slot_bytes;
+    data = smem_u32(ring) + threadIdx.y * places * place_bytes;
+    bars = smem_u32(&sh.full[threadIdx.y][0]);
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < places; ++s) mbar_init(bars + 8 * s, 1);
+    }
+    if (threadIdx.x + threadIdx.y == 0) sh.abort_flag = 0;
+  }
+  // Where the present row lies.
+  __device__ __forceinline__ uint32_t here() const { return data + at * place_bytes; }
+  // The place that the row before the present one had, and the row `places - 1` ahead gets.
+  __device__ __forceinline__ int before() const { return at == 0 ? places - 1 : at - 1; }
+  __device__ __forceinline__ void advance() {
+    if (++at == places) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+  // One thread of the group: ask for a row into a place.
+  __device__ __forceinline__ void ask(int place, const void* const (&src)[kArrays], int arrays, bool withhold) const {
+    if (wd.aborted()) return;
+    const uint32_t bar = bars + 8 * place;
+    mbar_arrive_expect_tx(bar, row_bytes * arrays);
+    if (withhold) return;
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) {
+      if (i < arrays) bulk_row(data + place * place_bytes + i * array_bytes, src[i], row_bytes, bar);
+    }
+  }
+  __device__ __forceinline__ void wait() const { wd.wait(bars + 8 * at, phase, kSiteRowRing); }
+  // After a wait that gave up, behind the last row: what was asked for may still be on its way.
+  __device__ __noinline__ void drain(int rows) const {
+    const unsigned long long t0 = global_timer_ns();
+    for (int n = max(0, rows - places); n < rows; ++n) {
+      while (!mbar_try_wait(bars + 8 * (n % places), (n / places) & 1) && global_timer_ns() - t0 < kDrainLimitNs) {
+      }
+    }
+  }
+  static __device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+  }
+};
+
+// What a thread keeps of a weight or bias vector: bf16 values as they are, and few fp32 ones; many fp32 ones come from the L1
+// cache row by row.  A missing vector is bf16 ones or zeros.
+template <typename W, int N, int P, bool kKeep = true>
+struct Columns;
+template <int N, int P>
+struct Columns<float, N, P, true> {
+  Pair w[N][P / 2];
+  __device__ __forceinline__ void init(const void* p, uint32_t, int d) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * blockDim.x + threadIdx.x) * P;
+#pragma unroll
+      for (int i = 0; i < P / 4; ++i) {
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c < d) f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c) + i);
+        w[j][2 * i] = make_pair(f.x, f.y);
+        w[j][2 * i + 1] = make_pair(f.z, f.w);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(int j, bool, Pair (&v)[P / 2]) const {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) v[i] = w[j][i];
+  }
+};
+template <int N, int P, bool kKeep>
+struct Columns<__nv_bfloat16, N, P, kKeep> {
+  uint32_t w[N][P / 2];
+  __device__ __forceinline__ void init(const void* p, uint32_t none, int d) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * blockDim.x + threadIdx.x) * P;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p) + c);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) w[j][i] = p != nullptr && c < d ? __ldg(q + i) : none;
+    }
+  }
+  __device__ __forceinline__ void get(int j, bool, Pair (&v)[P / 2]) const {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) v[i] = unpack_bf16x2(w[j][i]);
+  }
+};
+template <int N, int P>
+struct Columns<float, N, P, false> {
+  const float* q;
+  __device__ __forceinline__ void init(const void* p, uint32_t, int) { q = static_cast<const float*>(p) + threadIdx.x * P; }
+  __device__ __forceinline__ void get(int j, bool valid, Pair (&v)[P / 2]) const {
+#pragma unroll
+    for (int i = 0; i < P / 4; ++i) {
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (valid) f = __ldg(reinterpret_cast<const float4*>(q + j * blockDim.x * P) + i);
+      v[2 * i] = make_pair(f.x, f.y);
+      v[2 * i + 1] = make_pair(f.z, f.w);
+    }
+  }
+};
+
+// Most threads of a block by the columns that a thread holds: what registers allow.  A scheduler holds a quarter of the
+// warps, so that 12 of them have 168 registers each, and 16 have 128.
+constexpr int wide_forward_threads(int) { return 512; }
+constexpr int wide_backward_threads(int columns) { return columns <= 24 ? 512 : 384; }
+
+// T: type of the rows, W: type of weight and bias.  Places of the ring behind a row's end stay zero.
+template <typename T, typename W, bool kLayer, int N>
+__global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_forward_wide_kernel(const NormForwardParams p) {
+  constexpr int P = kPerVector<T>;
+  __shared__ WideShared shared;
+  extern __shared__ __align__(128) unsigned char ring_memory[];  // [groups][places][N * blockDim.x][16 bytes]
+  const int stride = gridDim.x * blockDim.y, row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int rows = row < p.M ? (p.M - 1 - row) / stride + 1 : 0;  // of this group
+  const uint32_t jump = blockDim.x * 16;                          // bytes from a thread's vector to its next
+  RowRing<1> ring(shared, ring_memory, N * jump, p.d * static_cast<uint32_t>(sizeof(T)), p.ring);
+  bool valid[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    valid[j] = static_cast<int>(j * blockDim.x + threadIdx.x) * P < p.d;
+    if (!valid[j]) {
+      for (int k = 0; k < ring.places; ++k) clear16(ring.here() + threadIdx.x * 16 + (k * N + j) * jump);
+    }
+  }
+  fence_mbar_init();
+  __syncthreads();
+  auto ask = [&](int place, int n) {
+    const void* const src[1] = {static_cast<const T*>(p.x) + (row + n * stride) * p.ldx};
+    ring.ask(place, src, 1, p.ring.withhold && row + n == 0);
+  };
+  const int ahead = ring.places - 1;
+  if (threadIdx.x == 0) {
+    for (int n = 0; n < ahead && n < rows; ++n) ask(n, n);
+  }
+  Columns<W, N, P, (N * P <= 16)> weight, bias;
+  weight.init(p.weight, 0x3f803f80u, p.d);
+  if (kLayer) bias.init(p.bias, 0u, p.d);
+  const int span = round_up_pow2(blockDim.x >> 5);
+  float2* const slots = shared.slots[span > 1 ? threadIdx.y : 0][0];
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  char* out = static_cast<char*>(p.y) + row * p.ldy * static_cast<long long>(sizeof(T)) + threadIdx.x * 16;
+  int turn = 0;
+  for (int n = 0; n < rows; ++n) {
+    ring.wait();
+    const uint32_t here = ring.here() + threadIdx.x * 16;
+    Pair x[N][P / 2];
+#pragma unroll
+    for (int j = 0; j < N; ++j) unpack16(read16(here + j * jump), x[j]);
+    float mean = 0.0f;
+    if (kLayer) {
+      Pair s = both(0.0f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+#pragma unroll
+        for (int i = 0; i < P / 2; ++i) s = s + x[j][i];
+      }
+      mean = group_sums<false>(make_float2(0.0f, sum(s)), slots + 32 * turn, span).y * inv_d;
+      turn ^= 1;
+    }
+    const Pair away = both(-mean);
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      Pair q = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        if (kLayer) x[j][i] = x[j][i] + away;
+        q = fma2(x[j][i], x[j][i], q);
+      }
+      if (!kLayer || valid[j]) ss += sum(q);
+    }
+    const float rstd = rsqrtf(fmaf(group_sums<false>(make_float2(0.0f, ss), slots + 32 * turn, span).y, inv_d, p.eps));
+    turn ^= 1;
+    // the group has read this row, and the one before it long ago: its place takes another
+    if (threadIdx.x == 0 && n + ahead < rows) ask(ring.before(), n + ahead);
+    const Pair by = both(rstd);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      Pair w[P / 2], b[P / 2];
+      weight.get(j, valid[j], w);
+      if (kLayer) bias.get(j, valid[j], b);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        const Pair f = w[i] * by;
+        x[j][i] = kLayer ? fma2(x[j][i], f, b[i]) : x[j][i] * f;
+      }
+      if (valid[j]) store16(out + j * jump, x[j]);
+    }
+    out += p.y_step;
+    ring.advance();
+    if (threadIdx.x == 0) {
+      if (kLayer) p.mean[row + n * stride] = mean;
+      p.rstd[row + n * stride] = rstd;
+    }
+  }
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(rows);
+}
+
+// dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
+// block are joined in the ring's memory at the end, and the blocks by norm_reduce_kernel.
+template <typename T, typename W, bool kLayer, int N>
+__global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm_backward_wide_kernel(const NormBackwardParams p) {
+  constexpr int P = kPerVector<T>;
+  constexpr long long kSize = sizeof(T);
+  // many columns' two sums leave no room for a row's z and a: they are computed again from shared memory
+  constexpr bool kAgain = kLayer && N * P > 16;
+  __shared__ WideShared shared;
+  extern __shared__ __align__(128) unsigned char ring_memory[];  // [groups][places][x, dy, res][N * blockDim.x][16 bytes]
+  const int stride = gridDim.x * blockDim.y, row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int rows = row < p.M ? (p.M - 1 - row) / stride + 1 : 0;  // of this group
+  const uint32_t jump = blockDim.x * 16;                          // bytes from a thread's vector to its next
+  const bool residual = p.residual != nullptr;
+  RowRing<3> ring(shared, ring_memory, N * jump, p.d * static_cast<uint32_t>(kSize), p.ring);
+  bool valid[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    valid[j] = static_cast<int>(j * blockDim.x + threadIdx.x) * P < p.d;
+    if (!valid[j]) {
+      for (int k = 0; k < 3 * ring.places; ++k) clear16(ring.here() + threadIdx.x * 16 + (k * N + j) * jump);
+    }
+  }
+  fence_mbar_init();
+  __syncthreads();
+  auto ask = [&](int place, int n) {
+    const long long r = row + n * stride;
+    const void* const src[3] = {static_cast<const T*>(p.x) + r * p.ldx, static_cast<const T*>(p.dout) + r * p.ld_dout,
+                                static_cast<const T*>(p.residual) + (residual ? r * p.ld_res : 0)};
+    ring.ask(place, src, residual ? 3 : 2, p.ring.withhold && row + n == 0);
+  };
+  const int ahead = ring.places - 1;
+  if (threadIdx.x == 0) {
+    for (int n = 0; n < ahead && n < rows; ++n) ask(n, n);
+  }
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  if (rows > 0) {
+    if (kLayer) next_mean = p.mean[row];
+    next_rstd = p.rstd[row];
+  }
+  Columns<W, N, P, (N * P <= 8)> weight;
+  weight.init(p.weight, 0x3f803f80u, p.d);
+  Pair dw[N][P / 2], db[kLayer ? N : 1][P / 2];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      dw[j][i] = both(0.0f);
+      if (kLayer) db[j][i] = both(0.0f);
+    }
+  }
+  const int span = round_up_pow2(blockDim.x >> 5);
+  float2* const slots = shared.slots[span > 1 ? threadIdx.y : 0][0];
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  let_next_start();
+  char* out = static_cast<char*>(p.dx) + row * p.ld_dx * kSize + threadIdx.x * 16;
+  for (int n = 0; n < rows; ++n) {
+    const float rstd = next_rstd;
+    const Pair by = both(rstd), away = both(-next_mean * rstd);
+    if (n + 1 < rows) {
+      if (kLayer) next_mean = p.mean[row + (n + 1) * stride];
+      next_rstd = p.rstd[row + (n + 1) * stride];
+    }
+    ring.wait();
+    const uint32_t here = ring.here() + threadIdx.x * 16;
+    Pair z[kAgain ? 1 : N][P / 2], a[kAgain ? 1 : N][P / 2];
+    Pair s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      constexpr int kOne = kAgain ? 0 : 1;
+      Pair(&zj)[P / 2] = z[j * kOne];
+      Pair(&aj)[P / 2] = a[j * kOne];
+      Pair w[P / 2];
+      unpack16(read16(here + j * jump), zj);
+      unpack16(read16(here + (N + j) * jump), aj);
+      weight.get(j, valid[j], w);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        zj[i] = kLayer ? fma2(zj[i], by, away) : zj[i] * by;
+        dw[j][i] = fma2(aj[i], zj[i], dw[j][i]);
+        if (kLayer) {
+          db[j][i] = db[j][i] + aj[i];
+          s1 = fma2(aj[i], w[i], s1);
+        }
+        aj[i] = aj[i] * w[i];
+        s2 = fma2(aj[i], zj[i], s2);
+      }
+    }
+    const float2 s = group_sums<kLayer>(make_float2(kLayer ? sum(s1) : 0.0f, sum(s2)), slots + 32 * (n & 1), span);
+    // all have read the row before this one to its end: its place takes another
+    if (threadIdx.x == 0 && n + ahead < rows) ask(ring.before(), n + ahead);
+    // dx = a rstd - c1 rstd - z c2 rstd (+ res)
+    const Pair k1 = both(-s.x * inv_d * rstd), k2 = both(-s.y * inv_d * rstd);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      Pair add[P / 2], zj[P / 2], aj[P / 2];
+      if (kAgain) {
+        Pair w[P / 2];
+        unpack16(read16(here + j * jump), zj);
+        unpack16(read16(here + (N + j) * jump), aj);
+        weight.get(j, valid[j], w);
+#pragma unroll
+        for (int i = 0; i < P / 2; ++i) {
+          zj[i] = fma2(zj[i], by, away);
+          aj[i] = aj[i] * w[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < P / 2; ++i) {
+          zj[i] = z[kAgain ? 0 : j][i];
+          aj[i] = a[kAgain ? 0 : j][i];
+        }
+      }
+      if (residual) unpack16(read16(here + (2 * N + j) * jump), add);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        const Pair t = fma2(zj[i], k2, kLayer ? fma2(aj[i], by, k1) : aj[i] * by);
+        zj[i] = residual ? t + add[i] : t;
+      }
+      if (valid[j]) store16(out + j * jump, zj);
+    }
+    out += p.dx_step;
+    ring.advance();
+  }
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(rows);
+  if (p.partial == nullptr) return;
+  // [group][2][columns]: the groups' sums side by side, joined in the order of the groups
+  const int columns = blockDim.x * N * P, group_floats = 2 * columns;
+  const int threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+  float* joined = reinterpret_cast<float*>(ring_memory);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * blockDim.x + threadIdx.x) * P;
+#pragma unroll
+    for (int i = 0; i < P / 2; i += 2) {
+      float* at = joined + threadIdx.y * group_floats + c + 2 * i;
+      const Pair pair_w[2] = {dw[j][i], dw[j][i + 1]};
+      store16(at, pair_w);
+      if (kLayer) {
+        const Pair pair_b[2] = {db[kLayer ? j : 0][i], db[kLayer ? j : 0][i + 1]};
+        store16(at + columns, pair_b);
+      }
+    }
+  }
+  __syncthreads();
+  float* part = p.partial + 2ll * blockIdx.x * p.d;
+  for (int i = thread * 4; i < (kLayer ? 2 * columns : columns); i += threads * 4) {
+    const int which = i >= columns, c = i - which * columns;
+    if (c >= p.d) continue;
+    float4 total = *reinterpret_cast<const float4*>(joined + i);
+    for (int g = 1; g < static_cast<int>(blockDim.y); ++g) {
+      const float4 q = *reinterpret_cast<const float4*>(joined + g * group_floats + i);
+      total.x += q.x;
+      total.y += q.y;
+      total.z += q.z;
+      total.w += q.w;
+    }
+    *reinterpret_cast<float4*>(part + which * p.d + c) = total;
+  }
+}
+
+// ---- short rows ----
+//
+// Rows of at most 32 vectors: a part of a warp, blockDim.x = 8, 16 or 32 lanes, takes a row, one vector a lane, and several rows
+// at a time, since one row's loads would not keep the memory busy.  Nothing but shuffles joins the lanes.
+
+constexpr int kShortThreads = 256;
+
+__device__ __forceinline__ float part_sum(float v) {
+  for (int o = blockDim.x >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p) {
+  uint4 w;
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p));
+  return w;
+}
+
+template <typename T, typename W, bool kLayer>
+__global__ void __launch_bounds__(kShortThreads) norm_forward_short_kernel(const NormForwardParams p) {
+  constexpr int P = kPerVector<T>, R = 4;
+  const int c = threadIdx.x * P;
+  const bool valid = c < p.d;
+  Columns<W, 1, P> weight, bias;
+  weight.init(p.weight, 0x3f803f80u, p.d);
+  if (kLayer) bias.init(p.bias, 0u, p.d);
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  const int stride = gridDim.x * blockDim.y;
+  // all lanes of a warp go round as often: `first` is the row of the block's first part
+  for (int first = blockIdx.x * blockDim.y; first < p.M; first += R * stride) {
+    uint4 raw[R];
+    int row[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      row[k] = first + k * stride + threadIdx.y;
+      raw[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (valid && row[k] < p.M) raw[k] = load16(static_cast<const T*>(p.x) + row[k] * p.ldx + c);
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      Pair x[P / 2];
+      unpack16(raw[k], x);
+      float mean = 0.0f;
+      if (kLayer) {
+        Pair s = x[0];
+#pragma unroll
+        for (int i = 1; i < P / 2; ++i) s = s + x[i];
+        mean = part_sum(sum(s)) * inv_d;
+      }
+      const Pair away = both(-mean);
+      Pair q = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        if (kLayer) x[i] = x[i] + away;
+        q = fma2(x[i], x[i], q);
+      }
+      const float rstd = rsqrtf(fmaf(part_sum(!kLayer || valid ? sum(q) : 0.0f), inv_d, p.eps));
+      if (row[k] >= p.M) continue;
+      const Pair by = both(rstd);
+      Pair w[P / 2], b[P / 2];
+      weight.get(0, valid, w);
+      if (kLayer) bias.get(0, valid, b);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        const Pair f = w[i] * by;
+        x[i] = kLayer ? fma2(x[i], f, b[i]) : x[i] * f;
+      }
+      if (valid) store16(static_cast<T*>(p.y) + row[k] * p.ldy + c, x);
+      if (threadIdx.x == 0) {
+        if (kLayer) p.mean[row[k]] = mean;
+        p.rstd[row[k]] = rstd;
+      }
+    }
+  }
+}
+
+template <typename T, typename W, bool kLayer>
+__global__ void __launch_bounds__(kShortThreads) norm_backward_short_kernel(const NormBackwardParams p) {
+  constexpr int P = kPerVector<T>, R = 2;
+  let_next_start();
+  __shared__ float joined[2][kShortThreads * P];  // [parts][columns]
+  const int c = threadIdx.x * P;
+  const bool valid = c < p.d, residual = p.residual != nullptr;
+  Columns<W, 1, P> weight;
+  weight.init(p.weight, 0x3f803f80u, p.d);
+  Pair dw[P / 2], db[P / 2];
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) dw[i] = db[i] = both(0.0f);
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  const int stride = gridDim.x * blockDim.y;
+  for (int first = blockIdx.x * blockDim.y; first < p.M; first += R * stride) {
+    uint4 raw_x[R], raw_dy[R], raw_res[R];
+    float mean[R], rstd[R];
+    int row[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      row[k] = first + k * stride + threadIdx.y;
+      raw_x[k] = raw_dy[k] = raw_res[k] = make_uint4(0u, 0u, 0u, 0u);
+      mean[k] = rstd[k] = 0.0f;
+      if (row[k] < p.M) {
+        if (kLayer) mean[k] = p.mean[row[k]];
+        rstd[k] = p.rstd[row[k]];
+        if (valid) {
+          raw_x[k] = load16(static_cast<const T*>(p.x) + row[k] * p.ldx + c);
+          raw_dy[k] = load16(static_cast<const T*>(p.dout) + row[k] * p.ld_dout + c);
+          if (residual) raw_res[k] = load16(static_cast<const T*>(p.residual) + row[k] * p.ld_res + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      Pair z[P / 2], a[P / 2], w[P / 2], add[P / 2];
+      unpack16(raw_x[k], z);
+      unpack16(raw_dy[k], a);
+      unpack16(raw_res[k], add);
+      weight.get(0, valid, w);
+      const Pair by = both(rstd[k]), away = both(-mean[k] * rstd[k]);
+      Pair s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        z[i] = kLayer ? fma2(z[i], by, away) : z[i] * by;
+        dw[i] = fma2(a[i], z[i], dw[i]);
+        if (kLayer) db[i] = db[i] + a[i];
+        a[i] = a[i] * w[i];
+        if (kLayer) s1 = s1 + a[i];
+        s2 = fma2(a[i], z[i], s2);
+      }
+      const float c1 = kLayer ? part_sum(sum(s1)) * inv_d : 0.0f, c2 = part_sum(sum(s2)) * inv_d;
+      const Pair k1 = both(-c1 * rstd[k]), k2 = both(-c2 * rstd[k]);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        const Pair t = fma2(z[i], k2, kLayer ? fma2(a[i], by, k1) : a[i] * by);
+        z[i] = residual ? t + add[i] : t;
+      }
+      if (valid && row[k] < p.M) store16(static_cast<T*>(p.dx) + row[k] * p.ld_dx + c, z);
+    }
+  }
+  if (p.partial == nullptr) return;
+  const int columns = blockDim.x * P, thread = threadIdx.y * blockDim.x + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < P / 2; i += 2) {
+    const Pair pair_w[2] = {dw[i], dw[i + 1]}, pair_b[2] = {db[i], db[i + 1]};
+    store16(&joined[0][thread * P + 2 * i], pair_w);
+    if (kLayer) store16(&joined[1][thread * P + 2 * i], pair_b);
+  }
+  __syncthreads();
+  float* part = p.partial + 2ll * blockIdx.x * p.d;
+  for (int i = thread; i < (kLayer ? 2 * columns : columns); i += kShortThreads) {
+    const int which = i >= columns, column = i - which * columns;
+    if (column >= p.d) continue;
+    float total = 0.0f;
+    for (int g = 0; g < static_cast<int>(blockDim.y); ++g) total += joined[which][g * columns + column];
+    part[which * p.d + column] = total;
   }
 }
 
@@ -402,6 +921,7 @@ __global__ void __launch_bounds__(32 * kNormReduceRows) norm_reduce_kernel(const
   __shared__ float shared[kBias ? 2 : 1][kNormReduceRows][33];
   const int i = blockIdx.x * 32 + threadIdx.x;
   float dw = 0.0f, db = 0.0f;
+  wait_for_previous();
   if (i < p.d) {
     for (int s = threadIdx.y; s < p.splits; s += kNormReduceRows) {
       dw += p.partial[2ll * s * p.d + i];

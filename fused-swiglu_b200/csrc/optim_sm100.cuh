@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "ptx_sm100.cuh"
 #include "vector_io_sm100.cuh"
@@ -223,85 +224,151 @@ __device__ __forceinline__ void store_codes(uint8_t* p, bool whole, int n, uint2
   }
 }
 
-// P, G: types of parameters and gradients.  A warp takes one block of 256 elements at a time, each thread eight
-// neighbours, so that a block's largest magnitudes are one reduction over the warp.
+// Where a warp is in a launch's tensors: at one block of 256 elements, this thread at its eight.
+template <int kCapacity>
+struct AdamCursor {
+  const AdamTable<kCapacity>& t;
+  uint32_t chunk;
+  int part = 0, k = 0, n = 0;  // n: elements of this thread that exist
+  long long at = 0;
+  bool whole = false;
+
+  // To the first block from (chunk, part) on that has elements; false behind the last.  The same for all lanes of a warp.
+  __device__ __forceinline__ bool seek() {
+    const uint32_t chunks = t.first_chunk[t.count];
+    for (; chunk < chunks; chunk += gridDim.x, part = 0) {
+      if (part == 0) k = find_tensor(t.first_chunk, t.count, chunk);
+      const long long numel = t.tensors[k].numel >= 0 ? t.tensors[k].numel : ~t.tensors[k].numel;
+      at = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk + (part * kAdamThreads + threadIdx.x) * kAdamGroup;
+      if (part < kAdamChunk / (kAdamThreads * kAdamGroup) && numel > at / kAdamBlock * kAdamBlock) {
+        const long long left = numel - at;
+        n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
+        whole = t.tensors[k].numel >= 0 && n == kAdamGroup;
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+// Eight values as they lie in memory.
+template <typename T>
+struct RawGroup;
+template <>
+struct RawGroup<float> {
+  float v[kAdamGroup];
+  __device__ __forceinline__ void load(const float* p, bool whole, int n) { load_group(p, whole, n, v); }
+  __device__ __forceinline__ void get(float (&out)[kAdamGroup]) const {
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) out[i] = v[i];
+  }
+};
+template <>
+struct RawGroup<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool whole, int n) {
+    if (whole) {
+      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "l"(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = 2 * i < n ? __bfloat16_as_ushort(p[2 * i]) : 0, hi = 2 * i + 1 < n ? __bfloat16_as_ushort(p[2 * i + 1]) : 0;
+        w[i] = lo | hi << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&out)[kAdamGroup]) const { unpack_bf16x8(w, out); }
+};
+
+// P, G: types of parameters and gradients; kEight: 8-bit moments, else fp32 ones.  A warp takes one block of 256 elements at a
+// time, each thread eight neighbours, so that a block's largest magnitudes are one reduction over the warp.  With 8-bit
+// moments there is as much to compute as to move: the next block's values are on their way meanwhile.
 template <typename P, typename G, bool kEight, bool kMaster, int kCapacity>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
+__global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 4) adamw_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
+  using Weight = typename std::conditional<kMaster, float, P>::type;
   const AdamOptions& o = t.opt;
   const AdamRates r = adam_rates(o);
   if (r.skip) return;
-  const uint32_t chunks = t.first_chunk[t.count];
-  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int k = find_tensor(t.first_chunk, t.count, chunk);
-    const AdamTensor& a = t.tensors[k];
-    const bool vector = a.numel >= 0;
-    const long long numel = vector ? a.numel : ~a.numel;
-    const long long base = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk;
-#pragma unroll 1
-    for (int part = 0; part < kAdamChunk / (kAdamThreads * kAdamGroup); ++part) {
-      const long long at = base + (part * kAdamThreads + threadIdx.x) * kAdamGroup;
-      if (numel <= at / kAdamBlock * kAdamBlock) break;  // the whole warp's block is behind the end
-      const long long left = numel - at;
-      const int n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
-      const bool whole = vector && n == kAdamGroup;
-      float m[kAdamGroup], v[kAdamGroup], p[kAdamGroup], g[kAdamGroup];
-      uint2 qm, qv;
-      float sm = 0.0f, sv = 0.0f;
-      if (kEight) {
-        qm = load_codes(static_cast<const uint8_t*>(a.exp_avg) + at, whole, n);
-        qv = load_codes(static_cast<const uint8_t*>(a.exp_avg_sq) + at, whole, n);
-        if (n > 0) {
-          sm = a.exp_avg_scale[at / kAdamBlock];
-          sv = a.exp_avg_sq_scale[at / kAdamBlock];
-        }
-      } else {
-        load_group(static_cast<const float*>(a.exp_avg) + at, whole, n, m);
-        load_group(static_cast<const float*>(a.exp_avg_sq) + at, whole, n, v);
+  AdamCursor<kCapacity> c{t, blockIdx.x};
+  RawGroup<Weight> raw_p;
+  RawGroup<G> raw_g;
+  RawGroup<float> raw_m, raw_v;
+  uint2 codes_m = make_uint2(0u, 0u), codes_v = codes_m;
+  float scale_m = 0.0f, scale_v = 0.0f;
+  auto fetch = [&]() {
+    const AdamTensor& a = t.tensors[c.k];
+    if (kEight) {
+      codes_m = load_codes(static_cast<const uint8_t*>(a.exp_avg) + c.at, c.whole, c.n);
+      codes_v = load_codes(static_cast<const uint8_t*>(a.exp_avg_sq) + c.at, c.whole, c.n);
+      if (c.n > 0) {
+        scale_m = a.exp_avg_scale[c.at / kAdamBlock];
+        scale_v = a.exp_avg_sq_scale[c.at / kAdamBlock];
       }
-      load_group(static_cast<const G*>(a.grad) + at, whole, n, g);
-      if (kMaster) load_group(a.master + at, whole, n, p);
-      else load_group(static_cast<const P*>(a.param) + at, whole, n, p);
+    } else {
+      raw_m.load(static_cast<const float*>(a.exp_avg) + c.at, c.whole, c.n);
+      raw_v.load(static_cast<const float*>(a.exp_avg_sq) + c.at, c.whole, c.n);
+    }
+    raw_g.load(static_cast<const G*>(a.grad) + c.at, c.whole, c.n);
+    raw_p.load(kMaster ? reinterpret_cast<const Weight*>(a.master) + c.at : static_cast<const Weight*>(a.param) + c.at, c.whole, c.n);
+  };
+  bool more = c.seek();
+  if (kEight && more) fetch();
+  while (more) {
+    if (!kEight) fetch();
+    const AdamTensor& a = t.tensors[c.k];
+    const long long at = c.at, block = at / kAdamBlock;
+    const unsigned long long group = (t.first_block[c.k] + block) * (kAdamBlock / kAdamGroup) + (threadIdx.x & 31);
+    const int n = c.n;
+    const bool whole = c.whole;
+    float m[kAdamGroup], v[kAdamGroup], p[kAdamGroup], g[kAdamGroup];
+    if (kEight) {
+      decode_e4m3x8(codes_m, m);
+      decode_e5m2x8(codes_v, v);
+    } else {
+      raw_m.get(m);
+      raw_v.get(v);
+    }
+    raw_g.get(g);
+    raw_p.get(p);
+    // the scale is a power of two: b times the scale, and that times the code, rounds as b times the value does
+    const float b1 = kEight ? o.beta1 * scale_m : o.beta1, b2 = kEight ? o.beta2 * scale_v : o.beta2;
+    ++c.part;
+    more = c.seek();
+    if (kEight && more) fetch();
+    uint32_t peak_m = 0, peak_v = 0;
+#pragma unroll
+    for (int i = 0; i < kAdamGroup; ++i) {
+      adam_element(o, r, g[i], __fmul_rn(b1, m[i]), __fmul_rn(b2, v[i]), m[i], v[i], p[i]);
       if (kEight) {
-        decode_e4m3x8(qm, m);
-        decode_e5m2x8(qv, v);
+        peak_m = max(peak_m, __float_as_uint(m[i]) & 0x7fffffffu);
+        peak_v = max(peak_v, __float_as_uint(v[i]) & 0x7fffffffu);
       }
-      // the scale is a power of two: b times the scale, and that times the code, rounds as b times the value does
-      const float b1 = kEight ? o.beta1 * sm : o.beta1, b2 = kEight ? o.beta2 * sv : o.beta2;
-      uint32_t peak_m = 0, peak_v = 0;
+    }
+    if (kMaster) store_group(a.master + at, whole, n, p);
+    store_group(static_cast<P*>(a.param) + at, whole, n, p);
+    if (kEight) {
+      peak_m = __reduce_max_sync(0xffffffffu, peak_m);
+      peak_v = __reduce_max_sync(0xffffffffu, peak_v);
+      const float2 cm = block_scale(peak_m, 7), cv = block_scale(peak_v, 14);
+      const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
+      if ((threadIdx.x & 31) == 0) {
+        a.exp_avg_scale[block] = cm.x;
+        a.exp_avg_sq_scale[block] = cv.x;
+      }
+      uint2 qm = make_uint2(0u, 0u), qv = qm;
 #pragma unroll
       for (int i = 0; i < kAdamGroup; ++i) {
-        adam_element(o, r, g[i], __fmul_rn(b1, m[i]), __fmul_rn(b2, v[i]), m[i], v[i], p[i]);
-        if (kEight) {
-          peak_m = max(peak_m, __float_as_uint(m[i]) & 0x7fffffffu);
-          peak_v = max(peak_v, __float_as_uint(v[i]) & 0x7fffffffu);
-        }
+        const uint32_t bits = h * odd_multiplier(i);
+        (i < 4 ? qm.x : qm.y) |= encode_e4m3(m[i], cm.y, bits) << (8 * (i & 3));
+        (i < 4 ? qv.x : qv.y) |= (encode_e5m2(v[i], cv.y, bits) & 0xffu) << (8 * (i & 3));
       }
-      if (kMaster) store_group(a.master + at, whole, n, p);
-      store_group(static_cast<P*>(a.param) + at, whole, n, p);
-      if (kEight) {
-        peak_m = __reduce_max_sync(0xffffffffu, peak_m);
-        peak_v = __reduce_max_sync(0xffffffffu, peak_v);
-        const float2 cm = block_scale(peak_m, 7), cv = block_scale(peak_v, 14);
-        const unsigned long long group =
-            (t.first_block[k] + at / kAdamBlock) * (kAdamBlock / kAdamGroup) + (threadIdx.x & 31);
-        const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
-        if ((threadIdx.x & 31) == 0 && n > 0) {
-          a.exp_avg_scale[at / kAdamBlock] = cm.x;
-          a.exp_avg_sq_scale[at / kAdamBlock] = cv.x;
-        }
-        qm = qv = make_uint2(0u, 0u);
-#pragma unroll
-        for (int i = 0; i < kAdamGroup; ++i) {
-          const uint32_t bits = h * odd_multiplier(i);
-          (i < 4 ? qm.x : qm.y) |= encode_e4m3(m[i], cm.y, bits) << (8 * (i & 3));
-          (i < 4 ? qv.x : qv.y) |= (encode_e5m2(v[i], cv.y, bits) & 0xffu) << (8 * (i & 3));
-        }
-        store_codes(static_cast<uint8_t*>(a.exp_avg) + at, whole, n, qm);
-        store_codes(static_cast<uint8_t*>(a.exp_avg_sq) + at, whole, n, qv);
-      } else {
-        store_group(static_cast<float*>(a.exp_avg) + at, whole, n, m);
-        store_group(static_cast<float*>(a.exp_avg_sq) + at, whole, n, v);
-      }
+      store_codes(static_cast<uint8_t*>(a.exp_avg) + at, whole, n, qm);
+      store_codes(static_cast<uint8_t*>(a.exp_avg_sq) + at, whole, n, qv);
+    } else {
+      store_group(static_cast<float*>(a.exp_avg) + at, whole, n, m);
+      store_group(static_cast<float*>(a.exp_avg_sq) + at, whole, n, v);
     }
   }
 }
@@ -341,6 +408,7 @@ template <int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradTable<kCapacity> t) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
+  let_next_start();
   const uint32_t chunks = t.first_chunk[t.count];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
@@ -372,6 +440,7 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const do
                                                                        float* out) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
+  wait_for_previous();
   for (int i = threadIdx.x; i < count; i += kAdamThreads) sum += slots[i];
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) {

@@ -23,6 +23,7 @@ enum WaitSite : uint32_t {
   kSiteDrainMma = 6,        // teardown waiting for MMAs in flight
   kSiteDecode = 7,          // decode kernels
   kSitePeer = 8,            // 2-CTA pair handshakes
+  kSiteRowRing = 9,         // norms waiting for a row
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s: default limit of every device-side wait
@@ -43,6 +44,12 @@ __device__ __forceinline__ uint32_t lane_id() {
   asm volatile("mov.u32 %0, %%laneid;" : "=r"(l));
   return l;
 }
+
+// ------------------- kernels that follow one another -----------------------
+// The stream's next kernel, where it was launched so, may start once all blocks have said this or ended ...
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// ... and waits here until this one has ended and what it wrote can be read.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ----------------------------- mbarrier ------------------------------------
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {

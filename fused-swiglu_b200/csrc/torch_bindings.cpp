@@ -9,6 +9,7 @@
 // raw pointers to the C ABI in include/fswiglu.h.  A non-zero status becomes a c10::Error
 // (RuntimeError in Python), like the reference's TORCH_CHECKs (csrc/SwiGLU/swiglu.cu:475-480).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -229,7 +230,12 @@ const float* norm_statistic(const at::Tensor& t, const char* name, const at::Ten
   return t.data_ptr<float>();
 }
 
-at::Tensor like_rows(const at::Tensor& x) { return at::empty({x.size(0), x.size(1)}, x.options()); }
+// What a call allocates, without the dispatcher's round: these calls may take less time on the GPU than on the host.
+at::Tensor empty_beside(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, x.device(), std::nullopt));
+}
+
+at::Tensor like_rows(const at::Tensor& x) { return empty_beside(x, {x.size(0), x.size(1)}, x.scalar_type()); }
 
 struct NormGradients {
   at::Tensor dx, dweight, dbias;
@@ -248,16 +254,16 @@ NormGradients norm_backward(bool layer, at::Tensor const& dout, at::Tensor const
   const int64_t M = x.size(0), d = x.size(1);
   const c10::cuda::OptionalCUDAGuard guard(device_of(x));
   const int gt = fp32_grads ? FSWIGLU_OUT_F32 : wt;
-  const auto grads = x.options().dtype(gt == FSWIGLU_OUT_F32 ? at::kFloat : at::kBFloat16);
+  const at::ScalarType grads = gt == FSWIGLU_OUT_F32 ? at::kFloat : at::kBFloat16;
   NormGradients g;
   g.dx = like_rows(x);
-  if (w != nullptr && weight_grad) g.dweight = at::empty({d}, grads);
-  if (bias_grad) g.dbias = at::empty({d}, grads);
+  if (w != nullptr && weight_grad) g.dweight = empty_beside(x, {d}, grads);
+  if (bias_grad) g.dbias = empty_beside(x, {d}, grads);
   at::Tensor ws;
   size_t bytes = 0;
   if ((g.dweight.defined() || g.dbias.defined()) && M > 0) {
     bytes = fswiglu_norm_backward_workspace_bytes(M, d);
-    ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+    ws = empty_beside(x, {static_cast<int64_t>(bytes)}, at::kByte);
   }
   void* dw = g.dweight.defined() ? g.dweight.data_ptr() : nullptr;
   void* db = g.dbias.defined() ? g.dbias.data_ptr() : nullptr;
@@ -284,8 +290,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward(at::Tensor con
   const void* w = norm_vector(weight, "weight", x);
   const void* b = norm_vector(bias, "bias", x);
   const c10::cuda::OptionalCUDAGuard guard(device_of(x));
-  at::Tensor y = like_rows(x), mean = at::empty({M}, x.options().dtype(at::kFloat)),
-             rstd = at::empty({M}, x.options().dtype(at::kFloat));
+  at::Tensor y = like_rows(x), mean = empty_beside(x, {M}, at::kFloat), rstd = empty_beside(x, {M}, at::kFloat);
   check_status(fswiglu_layer_norm_forward(x.data_ptr(), ldx, w, b, y.data_ptr(), d, mean.data_ptr<float>(),
                                           rstd.data_ptr<float>(), M, d, xt, wt, static_cast<float>(eps), current_stream(x)),
                "layer_norm_forward");
@@ -297,7 +302,7 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_forward(at::Tensor const& x, std::op
   const int xt = element_type(x, "x"), wt = norm_vector_type(weight, std::nullopt, x);
   const void* w = norm_vector(weight, "weight", x);
   const c10::cuda::OptionalCUDAGuard guard(device_of(x));
-  at::Tensor y = like_rows(x), rstd = at::empty({M}, x.options().dtype(at::kFloat));
+  at::Tensor y = like_rows(x), rstd = empty_beside(x, {M}, at::kFloat);
   check_status(fswiglu_rms_norm_forward(x.data_ptr(), ldx, w, y.data_ptr(), d, rstd.data_ptr<float>(), M, d, xt, wt,
                                         static_cast<float>(eps), current_stream(x)),
                "rms_norm_forward");
@@ -323,14 +328,37 @@ std::tuple<at::Tensor, at::Tensor> rms_norm_backward(at::Tensor const& dout, at:
 
 namespace {
 
+// The tensors of a list, by reference: what a step over many of them has to touch one by one.
+using Refs = std::vector<const at::Tensor*>;
+
+Refs refs_of(at::TensorList list) {
+  Refs r;
+  r.reserve(list.size());
+  for (const at::Tensor& t : list) r.push_back(&t);
+  return r;
+}
+
+// The same from a Python list or tuple, which the caller holds.
+Refs refs_of(const pybind11::handle& list, const char* name) {
+  TORCH_CHECK(PyList_Check(list.ptr()) || PyTuple_Check(list.ptr()), name, " must be a list of tensors");
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+  PyObject** items = PySequence_Fast_ITEMS(list.ptr());
+  Refs r(static_cast<size_t>(n));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    TORCH_CHECK(THPVariable_Check(items[i]), name, " must be a list of tensors");
+    r[static_cast<size_t>(i)] = &THPVariable_Unpack(items[i]);
+  }
+  return r;
+}
+
 // One list of a step over many tensors: as many entries as parameters, each contiguous, of one type, on one device.
-void check_list(at::TensorList list, at::TensorList params, at::ScalarType type, const char* name) {
+void check_list(const Refs& list, const Refs& params, at::ScalarType type, const char* name) {
   TORCH_CHECK(list.size() == params.size(), name, " must have one tensor for each parameter");
-  const auto device = params[0].device();
-  for (size_t i = 0; i < list.size(); ++i) {
-    TORCH_CHECK(list[i].scalar_type() == type, name, " must all be ", type, " tensors");
-    TORCH_CHECK(list[i].device() == device, name, " must all be on the device of the parameters");
-    TORCH_CHECK(list[i].is_contiguous(), name, " must all be contiguous");
+  const auto device = params[0]->device();
+  for (const at::Tensor* t : list) {
+    TORCH_CHECK(t->scalar_type() == type, name, " must all be ", type, " tensors");
+    TORCH_CHECK(t->device() == device, name, " must all be on the device of the parameters");
+    TORCH_CHECK(t->is_contiguous(), name, " must all be contiguous");
   }
 }
 
@@ -341,23 +369,21 @@ const void* scalar_on_device(const std::optional<at::Tensor>& t, at::ScalarType 
   return t->data_ptr();
 }
 
-}  // namespace
-
-void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs, int64_t step,
-                double lr, double beta1, double beta2, double eps, double weight_decay, at::TensorList masters,
-                at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, std::optional<at::Tensor> const& grad_scale,
-                int64_t seed, std::optional<at::Tensor> const& lr_tensor, std::optional<at::Tensor> const& step_tensor) {
+void adamw_step_refs(const Refs& params, const Refs& grads, const Refs& exp_avgs, const Refs& exp_avg_sqs, int64_t step,
+                     double lr, double beta1, double beta2, double eps, double weight_decay, const Refs& masters,
+                     const Refs& exp_avg_scales, const Refs& exp_avg_sq_scales, std::optional<at::Tensor> const& grad_scale,
+                     int64_t seed, std::optional<at::Tensor> const& lr_tensor, std::optional<at::Tensor> const& step_tensor) {
   if (params.empty()) {
     TORCH_CHECK(grads.empty() && exp_avgs.empty() && exp_avg_sqs.empty(), "the lists must be of one length");
     return;
   }
-  const at::Tensor& p0 = params[0];
+  const at::Tensor& p0 = *params[0];
   TORCH_CHECK(p0.is_cuda(), "params must be CUDA tensors");
   TORCH_CHECK(grads.size() == params.size() && exp_avgs.size() == params.size(), "the lists must be of one length");
-  const int pt = element_type(p0, "params"), gt = element_type(grads[0], "grads");
-  const bool eight = exp_avgs[0].scalar_type() == at::kFloat8_e4m3fn;
+  const int pt = element_type(p0, "params"), gt = element_type(*grads[0], "grads");
+  const bool eight = exp_avgs[0]->scalar_type() == at::kFloat8_e4m3fn;
   check_list(params, params, p0.scalar_type(), "params");
-  check_list(grads, params, grads[0].scalar_type(), "grads");
+  check_list(grads, params, grads[0]->scalar_type(), "grads");
   check_list(exp_avgs, params, eight ? at::kFloat8_e4m3fn : at::kFloat, "exp_avgs");
   check_list(exp_avg_sqs, params, eight ? at::kFloat8_e5m2 : at::kFloat, "exp_avg_sqs");
   if (!masters.empty()) {
@@ -372,21 +398,21 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   }
   std::vector<fswiglu_adamw_tensor> table(params.size());
   for (size_t i = 0; i < params.size(); ++i) {
-    const int64_t n = params[i].numel();
-    TORCH_CHECK(grads[i].numel() == n && exp_avgs[i].numel() == n && exp_avg_sqs[i].numel() == n &&
-                    (masters.empty() || masters[i].numel() == n),
+    const int64_t n = params[i]->numel();
+    TORCH_CHECK(grads[i]->numel() == n && exp_avgs[i]->numel() == n && exp_avg_sqs[i]->numel() == n &&
+                    (masters.empty() || masters[i]->numel() == n),
                 "tensor ", i, ": parameter, gradient, moments and master must have as many elements");
     if (eight) {
-      TORCH_CHECK(exp_avg_scales[i].numel() == (n + 255) / 256 && exp_avg_sq_scales[i].numel() == (n + 255) / 256, "tensor ",
+      TORCH_CHECK(exp_avg_scales[i]->numel() == (n + 255) / 256 && exp_avg_sq_scales[i]->numel() == (n + 255) / 256, "tensor ",
                   i, ": scales must have one element for each 256 of the parameter");
     }
-    table[i] = {params[i].data_ptr(),
-                grads[i].data_ptr(),
-                exp_avgs[i].data_ptr(),
-                exp_avg_sqs[i].data_ptr(),
-                masters.empty() ? nullptr : masters[i].data_ptr<float>(),
-                eight ? exp_avg_scales[i].data_ptr<float>() : nullptr,
-                eight ? exp_avg_sq_scales[i].data_ptr<float>() : nullptr,
+    table[i] = {params[i]->data_ptr(),
+                grads[i]->data_ptr(),
+                exp_avgs[i]->data_ptr(),
+                exp_avg_sqs[i]->data_ptr(),
+                masters.empty() ? nullptr : masters[i]->data_ptr<float>(),
+                eight ? exp_avg_scales[i]->data_ptr<float>() : nullptr,
+                eight ? exp_avg_sq_scales[i]->data_ptr<float>() : nullptr,
                 n};
   }
   fswiglu_adamw_options o = {};
@@ -404,31 +430,44 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   check_status(fswiglu_adamw_step(table.data(), static_cast<int64_t>(table.size()), pt, gt, eight ? 8 : 32, &o, current_stream(p0)),
                "adamw_step");
   // written through raw pointers: what a graph saved of a parameter is known to be stale
-  for (const at::Tensor& p : params) {
-    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  for (const at::Tensor* p : params) {
+    if (!p->is_inference()) p->unsafeGetTensorImpl()->bump_version();
   }
 }
 
-// [norm, factor]: the 2-norm over all gradients, and min(1, max_norm / (norm + 1e-6)) for adamw_step's grad_scale.
-at::Tensor grad_norm_clip(at::TensorList grads, double max_norm) {
+at::Tensor grad_norm_clip_refs(const Refs& grads, double max_norm) {
   TORCH_CHECK(!grads.empty(), "grads must not be empty");
-  const at::Tensor& g0 = grads[0];
+  const at::Tensor& g0 = *grads[0];
   std::vector<fswiglu_grad_tensor> table(grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor& g = grads[i];
+    const at::Tensor& g = *grads[i];
     TORCH_CHECK(g.is_cuda() && g.device() == g0.device(), "grads must all be CUDA tensors of one device");
     TORCH_CHECK(g.is_contiguous(), "grads must all be contiguous");
     table[i] = {g.data_ptr(), g.numel(), element_type(g, "grads")};
   }
   const c10::cuda::OptionalCUDAGuard guard(device_of(g0));
-  at::Tensor out = at::empty({2}, g0.options().dtype(at::kFloat));
+  at::Tensor out = empty_beside(g0, {2}, at::kFloat);
   const size_t bytes = fswiglu_grad_norm_workspace_bytes();
-  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, g0.options().dtype(at::kByte));
+  at::Tensor ws = empty_beside(g0, {static_cast<int64_t>(bytes)}, at::kByte);
   check_status(fswiglu_grad_norm_clip(table.data(), static_cast<int64_t>(table.size()), static_cast<float>(max_norm),
                                       out.data_ptr<float>(), ws.data_ptr(), bytes, current_stream(g0)),
                "grad_norm_clip");
   return out;
 }
+
+}  // namespace
+
+void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs, int64_t step,
+                double lr, double beta1, double beta2, double eps, double weight_decay, at::TensorList masters,
+                at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, std::optional<at::Tensor> const& grad_scale,
+                int64_t seed, std::optional<at::Tensor> const& lr_tensor, std::optional<at::Tensor> const& step_tensor) {
+  adamw_step_refs(refs_of(params), refs_of(grads), refs_of(exp_avgs), refs_of(exp_avg_sqs), step, lr, beta1, beta2, eps,
+                  weight_decay, refs_of(masters), refs_of(exp_avg_scales), refs_of(exp_avg_sq_scales), grad_scale, seed,
+                  lr_tensor, step_tensor);
+}
+
+// [norm, factor]: the 2-norm over all gradients, and min(1, max_norm / (norm + 1e-6)) for adamw_step's grad_scale.
+at::Tensor grad_norm_clip(at::TensorList grads, double max_norm) { return grad_norm_clip_refs(refs_of(grads), max_norm); }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward_meta(at::Tensor const& x, std::optional<at::Tensor> const&,
                                                                        std::optional<at::Tensor> const&, double) {
@@ -487,21 +526,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_backward", &rms_norm_backward, "(dx, dweight); residual is added to dx", py::arg("dout"), py::arg("x"),
         py::arg("rstd"), py::arg("weight") = py::none(), py::arg("residual") = py::none(), py::arg("fp32_grads") = false,
         py::arg("weight_grad") = true);
-  using Tensors = std::vector<at::Tensor>;
   m.def("adamw_step",
-        [](const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs, int64_t step,
-           double lr, double beta1, double beta2, double eps, double weight_decay, const Tensors& masters,
-           const Tensors& exp_avg_scales, const Tensors& exp_avg_sq_scales, const std::optional<at::Tensor>& grad_scale,
-           int64_t seed, const std::optional<at::Tensor>& lr_tensor, const std::optional<at::Tensor>& step_tensor) {
-          adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales,
-                     exp_avg_sq_scales, grad_scale, seed, lr_tensor, step_tensor);
+        [](py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs, int64_t step, double lr,
+           double beta1, double beta2, double eps, double weight_decay, py::handle masters, py::handle exp_avg_scales,
+           py::handle exp_avg_sq_scales, const std::optional<at::Tensor>& grad_scale, int64_t seed,
+           const std::optional<at::Tensor>& lr_tensor, const std::optional<at::Tensor>& step_tensor) {
+          adamw_step_refs(refs_of(params, "params"), refs_of(grads, "grads"), refs_of(exp_avgs, "exp_avgs"),
+                          refs_of(exp_avg_sqs, "exp_avg_sqs"), step, lr, beta1, beta2, eps, weight_decay,
+                          refs_of(masters, "masters"), refs_of(exp_avg_scales, "exp_avg_scales"),
+                          refs_of(exp_avg_sq_scales, "exp_avg_sq_scales"), grad_scale, seed, lr_tensor, step_tensor);
         },
         "one AdamW step over many tensors, in place", py::arg("params"), py::arg("grads"), py::arg("exp_avgs"),
         py::arg("exp_avg_sqs"), py::arg("step"), py::arg("lr"), py::arg("beta1") = 0.9, py::arg("beta2") = 0.999,
-        py::arg("eps") = 1e-8, py::arg("weight_decay") = 0.01, py::arg("masters") = Tensors(),
-        py::arg("exp_avg_scales") = Tensors(), py::arg("exp_avg_sq_scales") = Tensors(), py::arg("grad_scale") = py::none(),
+        py::arg("eps") = 1e-8, py::arg("weight_decay") = 0.01, py::arg("masters") = py::tuple(),
+        py::arg("exp_avg_scales") = py::tuple(), py::arg("exp_avg_sq_scales") = py::tuple(), py::arg("grad_scale") = py::none(),
         py::arg("seed") = 0, py::arg("lr_tensor") = py::none(), py::arg("step_tensor") = py::none());
-  m.def("grad_norm_clip", [](const Tensors& grads, double max_norm) { return grad_norm_clip(grads, max_norm); },
+  m.def("grad_norm_clip",
+        [](py::handle grads, double max_norm) { return grad_norm_clip_refs(refs_of(grads, "grads"), max_norm); },
         "[2-norm over all gradients, min(1, max_norm / (norm + 1e-6))]", py::arg("grads"), py::arg("max_norm"));
 }
 

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <memory>
@@ -26,6 +27,24 @@ int launched() {
   return cudaGetLastError() == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
 }
 
+// A launch that may start while the stream's previous kernel ends; the kernel itself waits for what that one wrote
+// (wait_for_previous).
+template <typename... Params, typename... Args>
+int launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = s;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+  count_launch();
+  return e == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
+}
+
 // ---- norms ----
 
 constexpr int64_t kMaxNormWidth = 1 << 24;                // a row's length is exact in fp32
@@ -46,6 +65,8 @@ int check_norm(int64_t M, int64_t d, int x_dtype, int w_dtype) {
 
 int norm_splits(int64_t M) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(M, kMaxNormSplits))); }
 
+constexpr size_t kRingBytes = 216 * 1024;  // of the 227 KB of a block
+
 // How a width is laid out over threads: groups of `group` threads hold a row, `groups` of them make a block.
 struct RowShape {
   int vectors;  // of a thread; 0: the width is too large for registers
@@ -61,74 +82,221 @@ RowShape row_shape(int64_t units, int64_t M, int most, int threads) {
   if (group > threads) return r;
   r.vectors = n;
   r.group = static_cast<int>(group);
-  r.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({threads / group, kNormGroups, M})));
+  r.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({threads / group, kNarrowGroups, M})));
   return r;
 }
 
-template <typename T, bool kLayer, int V, int N>
-int launch_norm_forward_rows(const NormForwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
+template <typename T, bool kLayer, int N>
+int launch_norm_forward_narrow(const NormForwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
   const int64_t resident = static_cast<int64_t>(sms) * std::max(1, 1536 / (r.group * r.groups));
-  norm_forward_rows_kernel<T, kLayer, V, N>
+  norm_forward_narrow_kernel<T, kLayer, N>
       <<<static_cast<int>(std::min(blocks, resident)), dim3(r.group, r.groups), 0, s>>>(p);
   return launched();
 }
 
-template <typename T, bool kLayer>
-int launch_norm_forward(const NormForwardParams& p, bool wide, int sms, cudaStream_t s) {
-  if (wide) {
-    const RowShape r = row_shape(p.d / 8, p.M, 4, 256);
-    if (r.vectors == 1) return launch_norm_forward_rows<T, kLayer, 8, 1>(p, r, sms, s);
-    if (r.vectors == 2) return launch_norm_forward_rows<T, kLayer, 8, 2>(p, r, sms, s);
-    if (r.vectors == 4) return launch_norm_forward_rows<T, kLayer, 8, 4>(p, r, sms, s);
-  } else {
-    const RowShape r = row_shape(p.d, p.M, 16, 512);
-    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_forward_rows<T, kLayer, 1, 2>(p, r, sms, s);
-    if (r.vectors > 2 && r.vectors <= 8) return launch_norm_forward_rows<T, kLayer, 1, 8>(p, r, sms, s);
-    if (r.vectors == 16) return launch_norm_forward_rows<T, kLayer, 1, 16>(p, r, sms, s);
+// How the wide kernels lay a row out: each thread holds `columns` of it.
+struct WidePlan {
+  int columns, group, groups, places;
+  size_t ring;  // bytes of shared memory
+  int threads() const { return group * groups; }
+};
+
+// The plan for rows of d values of `size` bytes, `arrays` of them on their way, in blocks of at most `most_threads`;
+// columns == 0 where a row does not fit.
+WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_threads, int arrays, int most_places, int sms) {
+  WidePlan w = {0, 0, 0, 0, 0};
+  const int64_t group = (d + 32 * columns - 1) / (32 * columns) * 32;
+  if (group > most_threads) return w;
+  // no more groups than leave every SM a block
+  const int64_t spread = std::max<int64_t>(1, (M + sms - 1) / sms);
+  int64_t groups = std::min<int64_t>({most_threads / group, group > 32 ? kWideMultiGroups : kWideGroups, spread});
+  for (; groups >= 1; --groups) {
+    const size_t place = static_cast<size_t>(arrays) * static_cast<size_t>(group * groups * columns) * size;
+    const size_t places = std::min<size_t>(static_cast<size_t>(most_places), kRingBytes / place);
+    // two places keep one row of each group on its way: enough where that is 64 KB
+    if (places < 2 || (places == 2 && most_places > 2 && groups > 1 && place < 64 * 1024)) continue;
+    w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), places * place};
+    break;
   }
-  norm_forward_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8)), kNormThreads, 0, s>>>(p);
+  return w;
+}
+
+// Lets a kernel have a whole ring of shared memory; once for each device.
+template <typename Kernel>
+int opt_in(Kernel k, std::atomic<uint64_t>* done, const Device& dev) {
+  const uint64_t bit = 1ull << dev.index;
+  if (done->load(std::memory_order_relaxed) & bit) return FSWIGLU_OK;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingBytes)) != cudaSuccess)
+    return FSWIGLU_ERR_CUDA;
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return FSWIGLU_OK;
+}
+
+// Blocks of a kernel that an SM holds; the last answer is kept with what it was for.
+template <typename Kernel>
+int64_t resident_blocks(Kernel k, std::atomic<uint64_t>* known, int threads, size_t shared) {
+  const uint64_t key = static_cast<uint64_t>(threads) << 40 | static_cast<uint64_t>(shared) << 8;
+  const uint64_t seen = known->load(std::memory_order_relaxed);
+  if ((seen & ~0xffull) == key && (seen & 0xffu) != 0) return static_cast<int64_t>(seen & 0xffu);
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, threads, shared) != cudaSuccess || n < 1) n = 1;
+  known->store(key | static_cast<uint64_t>(n), std::memory_order_relaxed);
+  return n;
+}
+
+// Wide kernels take weights of the rows' type or fp32 ones (bf16 rows), and stand-ins for missing ones in bf16.
+template <typename T, typename W, bool kLayer, int kColumns>
+int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  constexpr auto kernel = norm_forward_wide_kernel<T, W, kLayer, kColumns / kPerVector<T>>;
+  static std::atomic<uint64_t> done{0}, known{0};
+  if (int rc = opt_in(kernel, &done, dev)) return rc;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
+  const int64_t resident = dev.sms * resident_blocks(kernel, &known, w.threads(), w.ring);
+  const int grid = static_cast<int>(std::min(blocks, resident));
+  p.y_step = static_cast<long long>(grid) * w.groups * p.ldy * static_cast<long long>(sizeof(T));
+  p.ring.places = w.places;
+  p.ring.withhold = take_withhold();
+  kernel<<<grid, dim3(w.group, w.groups), w.ring, s>>>(p);
   return launched();
 }
 
-template <typename T, bool kLayer, int V, int N>
-int launch_norm_backward_rows(NormBackwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
+// Forward: 32 columns a thread, since a row's reductions cost every warp the same; 16 where a warp holds a whole row with
+// them, where fp32 weights are kept in registers, and for fp32 rows, whose places would take twice the shared memory.
+WidePlan forward_plan(const NormForwardParams& p, bool layer, size_t size, int sms) {
+  const bool few = p.d <= 512 || ((p.w_f32 || size == 4) && p.d <= 16 * wide_forward_threads(16));
+  const int columns = few ? 16 : 32, group = (p.d + 32 * columns - 1) / (32 * columns) * 32;
+  if (group > wide_forward_threads(columns)) return WidePlan{0, 0, 0, 0, 0};
+  return wide_plan(p.d, p.M, size, columns, std::max(256, group), 1, layer ? 4 : 3, sms);
+}
+
+template <typename T, typename W, bool kLayer>
+int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  if (w.columns == 16) return launch_norm_forward_wide<T, W, kLayer, 16>(p, w, dev, s);
+  return launch_norm_forward_wide<T, W, kLayer, 32>(p, w, dev, s);
+}
+
+// Lanes that take a short row.
+int short_lanes(int d, int per_vector) { return d <= 8 * per_vector ? 8 : d <= 16 * per_vector ? 16 : 32; }
+
+template <typename T, typename W, bool kLayer>
+int launch_norm_forward_short(const NormForwardParams& p, const Device& dev, cudaStream_t s) {
+  const int lanes = short_lanes(p.d, kPerVector<T>), parts = kShortThreads / lanes;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + parts - 1) / parts;
+  norm_forward_short_kernel<T, W, kLayer>
+      <<<static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(dev.sms) * 8)), dim3(lanes, parts), 0, s>>>(p);
+  return launched();
+}
+
+template <typename T, bool kLayer>
+int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cudaStream_t s) {
+  if (wide) {
+    if (p.d <= 32 * kPerVector<T>) {
+      if (p.w_f32) return launch_norm_forward_short<T, float, kLayer>(p, dev, s);
+      return launch_norm_forward_short<T, __nv_bfloat16, kLayer>(p, dev, s);
+    }
+    const WidePlan w = forward_plan(p, kLayer, sizeof(T), dev.sms);
+    if (w.columns > 0) {
+      if (p.w_f32) return launch_norm_forward_wide<T, float, kLayer>(p, w, dev, s);
+      return launch_norm_forward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
+    }
+  } else {
+    const RowShape r = row_shape(p.d, p.M, 16, 512);
+    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_forward_narrow<T, kLayer, 2>(p, r, dev.sms, s);
+    if (r.vectors > 2 && r.vectors <= 8) return launch_norm_forward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
+    if (r.vectors == 16) return launch_norm_forward_narrow<T, kLayer, 16>(p, r, dev.sms, s);
+  }
+  norm_forward_any_kernel<T, kLayer>
+      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8)), kNormThreads, 0, s>>>(p);
+  return launched();
+}
+
+template <typename T, bool kLayer, int N>
+int launch_norm_backward_narrow(NormBackwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
   const int64_t resident = std::min<int64_t>(static_cast<int64_t>(sms) * std::max(1, 512 / (r.group * r.groups)), kMaxNormSplits);
   const int grid = static_cast<int>(std::min(blocks, resident));
   p.splits = grid;
-  const size_t shared = r.groups > 1 ? static_cast<size_t>(2) * r.group * V * N * sizeof(float) : 0;
-  norm_backward_rows_kernel<T, kLayer, V, N><<<grid, dim3(r.group, r.groups), shared, s>>>(p);
+  const size_t shared = r.groups > 1 ? static_cast<size_t>(2) * r.group * N * sizeof(float) : 0;
+  norm_backward_narrow_kernel<T, kLayer, N><<<grid, dim3(r.group, r.groups), shared, s>>>(p);
+  return launched();
+}
+
+template <typename T, typename W, bool kLayer, int kColumns>
+int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  constexpr auto kernel = norm_backward_wide_kernel<T, W, kLayer, kColumns / kPerVector<T>>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = opt_in(kernel, &done, dev)) return rc;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
+  const int grid = static_cast<int>(std::min<int64_t>({blocks, dev.sms, kMaxNormSplits}));
+  p.splits = grid;
+  p.dx_step = static_cast<long long>(grid) * w.groups * p.ld_dx * static_cast<long long>(sizeof(T));
+  p.ring.places = w.places;
+  p.ring.withhold = take_withhold();
+  kernel<<<grid, dim3(w.group, w.groups), w.ring, s>>>(p);
+  return launched();
+}
+
+// Backward: one block an SM, its registers full of the sums over rows.  Of the columns a thread may hold, those that keep most
+// warps busy.
+WidePlan backward_plan(const NormBackwardParams& p, size_t size, int sms) {
+  WidePlan best = {0, 0, 0, 0, 0};
+  for (int columns = 16; columns <= 32; columns += 8) {
+    const WidePlan w = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns), 3, 4, sms);
+    if (w.threads() > best.threads()) best = w;
+  }
+  return best;
+}
+
+template <typename T, typename W, bool kLayer>
+int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  switch (w.columns) {
+    case 16: return launch_norm_backward_wide<T, W, kLayer, 16>(p, w, dev, s);
+    case 24: return launch_norm_backward_wide<T, W, kLayer, 24>(p, w, dev, s);
+    default: return launch_norm_backward_wide<T, W, kLayer, 32>(p, w, dev, s);
+  }
+}
+
+template <typename T, typename W, bool kLayer>
+int launch_norm_backward_short(NormBackwardParams& p, const Device& dev, cudaStream_t s) {
+  const int lanes = short_lanes(p.d, kPerVector<T>), parts = kShortThreads / lanes;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + parts - 1) / parts;
+  p.splits = static_cast<int>(std::min<int64_t>({blocks, static_cast<int64_t>(dev.sms) * 2, kMaxNormSplits}));
+  norm_backward_short_kernel<T, W, kLayer><<<p.splits, dim3(lanes, parts), 0, s>>>(p);
   return launched();
 }
 
 template <typename T, bool kLayer>
-int launch_norm_backward(NormBackwardParams& p, bool wide, int sms, cudaStream_t s) {
+int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cudaStream_t s) {
   if (wide) {
-    const RowShape r = row_shape(p.d / 8, p.M, 2, 512);
-    if (r.vectors == 1) return launch_norm_backward_rows<T, kLayer, 8, 1>(p, r, sms, s);
-    if (r.vectors == 2) return launch_norm_backward_rows<T, kLayer, 8, 2>(p, r, sms, s);
+    if (p.d <= 32 * kPerVector<T>) {
+      if (p.w_f32) return launch_norm_backward_short<T, float, kLayer>(p, dev, s);
+      return launch_norm_backward_short<T, __nv_bfloat16, kLayer>(p, dev, s);
+    }
+    const WidePlan w = backward_plan(p, sizeof(T), dev.sms);
+    if (w.columns > 0) {
+      if (p.w_f32) return launch_norm_backward_wide<T, float, kLayer>(p, w, dev, s);
+      return launch_norm_backward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
+    }
   } else {
     const RowShape r = row_shape(p.d, p.M, 8, 512);
-    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_backward_rows<T, kLayer, 1, 2>(p, r, sms, s);
-    if (r.vectors > 2) return launch_norm_backward_rows<T, kLayer, 1, 8>(p, r, sms, s);
+    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_backward_narrow<T, kLayer, 2>(p, r, dev.sms, s);
+    if (r.vectors > 2) return launch_norm_backward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
   }
   norm_backward_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8)), kNormThreads, 0, s>>>(p);
+      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8)), kNormThreads, 0, s>>>(p);
   if (int rc = launched()) return rc;
   if (p.partial == nullptr) return FSWIGLU_OK;
   const int64_t tiles = (p.d + kNormThreads - 1) / kNormThreads * static_cast<int64_t>(p.splits);
   norm_backward_columns_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(sms) * 32)), kNormThreads, 0, s>>>(p);
+      <<<static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * 32)), kNormThreads, 0, s>>>(p);
   return launched();
 }
 
-// Whether a matrix's rows, or a vector, take the wide accesses of eight elements.
+// Whether a matrix's rows all start on 16 bytes.
 bool wide_rows(const void* p, int64_t ld, int64_t M, int type) {
-  return aligned(p, type == FSWIGLU_OUT_F32 ? 32 : 16) && (ld % 8 == 0 || M == 1);
+  return aligned(p, 16) && (M == 1 || ld * static_cast<int64_t>(type_bytes(type)) % 16 == 0);
 }
-bool wide_vector(const void* p, int type) { return aligned(p, type == FSWIGLU_OUT_F32 ? 32 : 16); }
 
 int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, const void* bias, void* y, int64_t ldy,
                  float* mean, float* rstd, int64_t M, int64_t d, int x_dtype, int w_dtype, float eps, void* stream) {
@@ -140,8 +308,8 @@ int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, con
   if (rstd == nullptr || (layer && mean == nullptr)) return FSWIGLU_ERR_BAD_ARG;
   if (!aligned(weight, type_bytes(w_dtype)) || !aligned(bias, type_bytes(w_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4))
     return FSWIGLU_ERR_ALIGNMENT;
-  int sms = 0;
-  if (int rc = current_device_sms(&sms)) return rc;
+  Device dev;
+  if (int rc = current_device(&dev)) return rc;
   NormForwardParams p = {};
   p.x = x;
   p.weight = weight;
@@ -153,15 +321,18 @@ int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, con
   p.ldy = ldy;
   p.M = static_cast<int>(M);
   p.d = static_cast<int>(d);
-  p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
+  p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0};
+  p.w_f32 = w_dtype == FSWIGLU_OUT_F32 && (weight != nullptr || bias != nullptr);
   p.eps = eps;
-  const bool wide = d % 8 == 0 && wide_rows(x, ldx, M, x_dtype) && wide_rows(y, ldy, M, x_dtype) &&
-                    wide_vector(weight, w_dtype) && wide_vector(bias, w_dtype);
+  // fp32 vectors are read where they are: one without the other goes the narrow way
+  const bool wide = !(layer && p.w_f32 && (weight == nullptr || bias == nullptr)) &&
+                    d * type_bytes(x_dtype) % 16 == 0 && wide_rows(x, ldx, M, x_dtype) && wide_rows(y, ldy, M, x_dtype) &&
+                    aligned(weight, 16) && aligned(bias, 16);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   using BF = __nv_bfloat16;
   if (x_dtype == FSWIGLU_OUT_F32)
-    return layer ? launch_norm_forward<float, true>(p, wide, sms, s) : launch_norm_forward<float, false>(p, wide, sms, s);
-  return layer ? launch_norm_forward<BF, true>(p, wide, sms, s) : launch_norm_forward<BF, false>(p, wide, sms, s);
+    return layer ? launch_norm_forward<float, true>(p, wide, dev, s) : launch_norm_forward<float, false>(p, wide, dev, s);
+  return layer ? launch_norm_forward<BF, true>(p, wide, dev, s) : launch_norm_forward<BF, false>(p, wide, dev, s);
 }
 
 int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, int64_t ldx, const float* mean,
@@ -187,8 +358,8 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     if (columns && (workspace == nullptr || workspace_bytes < fswiglu_norm_backward_workspace_bytes(M, d) || !aligned(workspace, 256)))
       return FSWIGLU_ERR_WORKSPACE;
   }
-  int sms = 0;
-  if (int rc = current_device_sms(&sms)) return rc;
+  Device dev;
+  if (int rc = current_device(&dev)) return rc;
   if (M > 0) {
     p.dout = dout;
     p.x = x;
@@ -205,16 +376,17 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     p.M = static_cast<int>(M);
     p.d = static_cast<int>(d);
     p.splits = norm_splits(M);
-    p.w_f32 = w_dtype == FSWIGLU_OUT_F32;
-    const bool wide = d % 8 == 0 && wide_rows(dout, ld_dout, M, x_dtype) && wide_rows(x, ldx, M, x_dtype) &&
+    p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0};
+    p.w_f32 = w_dtype == FSWIGLU_OUT_F32 && weight != nullptr;
+    const bool wide = d * type_bytes(x_dtype) % 16 == 0 && wide_rows(dout, ld_dout, M, x_dtype) && wide_rows(x, ldx, M, x_dtype) &&
                       wide_rows(dx, ld_dx, M, x_dtype) && wide_rows(residual, residual == nullptr ? 0 : ld_res, M, x_dtype) &&
-                      wide_vector(weight, w_dtype);
+                      aligned(weight, 16);
     using BF = __nv_bfloat16;
     int rc;
     if (x_dtype == FSWIGLU_OUT_F32)
-      rc = layer ? launch_norm_backward<float, true>(p, wide, sms, s) : launch_norm_backward<float, false>(p, wide, sms, s);
+      rc = layer ? launch_norm_backward<float, true>(p, wide, dev, s) : launch_norm_backward<float, false>(p, wide, dev, s);
     else
-      rc = layer ? launch_norm_backward<BF, true>(p, wide, sms, s) : launch_norm_backward<BF, false>(p, wide, sms, s);
+      rc = layer ? launch_norm_backward<BF, true>(p, wide, dev, s) : launch_norm_backward<BF, false>(p, wide, dev, s);
     if (rc) return rc;
   }
   if (!columns) return FSWIGLU_OK;
@@ -225,10 +397,9 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
   q.d = static_cast<int>(d);
   q.splits = p.splits;
   q.out_f32 = grad_dtype == FSWIGLU_OUT_F32;
-  const int grid = static_cast<int>((d + 31) / 32);
-  if (dbias != nullptr) norm_reduce_kernel<true><<<grid, dim3(32, kNormReduceRows), 0, s>>>(q);
-  else norm_reduce_kernel<false><<<grid, dim3(32, kNormReduceRows), 0, s>>>(q);
-  return launched();
+  const dim3 grid(static_cast<unsigned>((d + 31) / 32)), block(32, kNormReduceRows);
+  return dbias != nullptr ? launch_after(norm_reduce_kernel<true>, grid, block, s, q)
+                          : launch_after(norm_reduce_kernel<false>, grid, block, s, q);
 }
 
 // ---- many tensors ----
@@ -438,8 +609,8 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
   if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg_sq, tensors[i].numel * static_cast<int64_t>(sb)); })))
     return rc;
   if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].master, tensors[i].numel * 4); }))) return rc;
-  int sms = 0;
-  if ((rc = current_device_sms(&sms))) return rc;
+  Device dev;
+  if ((rc = current_device(&dev))) return rc;
   AdamOptions o = {};
   o.log_beta1 = std::log(in.beta1);
   o.log_beta2 = std::log(in.beta2);
@@ -464,8 +635,8 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
   o.step_lo = static_cast<uint32_t>(in.step);
   const AdamKind kind = {param_dtype == FSWIGLU_OUT_F32, grad_dtype == FSWIGLU_OUT_F32, state_bits == 8, false};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, kind, sms, s)
-                              : adamw_launches<kLargeTable>(tensors, count, o, kind, sms, s);
+  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, kind, dev.sms, s)
+                              : adamw_launches<kLargeTable>(tensors, count, o, kind, dev.sms, s);
 }
 
 size_t fswiglu_grad_norm_workspace_bytes(void) { return kGradNormSlots * sizeof(double); }
@@ -484,16 +655,16 @@ int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, fl
     if (a.grad == nullptr) return FSWIGLU_ERR_BAD_ARG;
     if (!aligned(a.grad, type_bytes(a.dtype))) return FSWIGLU_ERR_ALIGNMENT;
   }
-  int sms = 0;
-  if (int rc = current_device_sms(&sms)) return rc;
+  Device dev;
+  if (int rc = current_device(&dev)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   double* slots = static_cast<double*>(workspace);
   int used = 0;
-  const int rc = count <= kSmallTable ? grad_norm_launches<kSmallTable>(tensors, count, slots, &used, sms, s)
-                                      : grad_norm_launches<kLargeTable>(tensors, count, slots, &used, sms, s);
+  const int rc = count <= kSmallTable ? grad_norm_launches<kSmallTable>(tensors, count, slots, &used, dev.sms, s)
+                                      : grad_norm_launches<kLargeTable>(tensors, count, slots, &used, dev.sms, s);
   if (rc) return rc;
-  grad_norm_finish_kernel<<<1, kAdamThreads, 0, s>>>(slots, used, max_norm, out);
-  return launched();
+  return launch_after(grad_norm_finish_kernel, dim3(1), dim3(kAdamThreads), s, static_cast<const double*>(slots), used,
+                      max_norm, out);
 }
 
 }  // extern "C"

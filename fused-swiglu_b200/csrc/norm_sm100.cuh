@@ -105,6 +105,8 @@ __device__ __forceinline__ float2 block_sum2(float2 v, float2* shared) {
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_forward_any_kernel(const NormForwardParams p) {
   __shared__ float2 shared[kNormThreads / 32];
+  let_next_start();
+  wait_for_previous();
   for (int row = blockIdx.x; row < p.M; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     T* y = static_cast<T*>(p.y) + row * p.ldy;
@@ -135,6 +137,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_any_kernel(const No
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_backward_any_kernel(const NormBackwardParams p) {
   __shared__ float2 shared[kNormThreads / 32];
+  let_next_start();
+  wait_for_previous();
   for (int row = blockIdx.x; row < p.M; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* dy = static_cast<const T*>(p.dout) + row * p.ld_dout;
@@ -165,6 +169,7 @@ template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_backward_columns_any_kernel(const NormBackwardParams p) {
   const long long tiles = (p.d + kNormThreads - 1) / kNormThreads;
   let_next_start();
+  wait_for_previous();
   for (long long t = blockIdx.x; t < tiles * p.splits; t += gridDim.x) {
     const int split = static_cast<int>(t / tiles);
     const int i = static_cast<int>(t % tiles) * kNormThreads + threadIdx.x;
@@ -225,6 +230,8 @@ __device__ __forceinline__ int round_up_pow2(int v) { return v <= 1 ? 1 : 1 << (
 template <typename T, bool kLayer, int N>
 __global__ void __launch_bounds__(kNarrowThreads) norm_forward_narrow_kernel(const NormForwardParams p) {
   __shared__ float2 slots[kNarrowGroups][2][32];
+  let_next_start();
+  wait_for_previous();
   float w[N], b[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -284,6 +291,7 @@ __global__ void __launch_bounds__(kNarrowThreads) norm_backward_narrow_kernel(co
   __shared__ float2 slots[kNarrowGroups][2][32];
   extern __shared__ float joined[];  // [2][columns of a group], more than one group only
   let_next_start();
+  wait_for_previous();
   float w[N], dw[N], db[kLayer ? N : 1];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -523,6 +531,8 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
   }
   fence_mbar_init();
   __syncthreads();
+  let_next_start();
+  wait_for_previous();
   auto ask = [&](int place, int n) {
     const void* const src[1] = {static_cast<const T*>(p.x) + (row + n * stride) * p.ldx};
     ring.ask(place, src, 1, p.ring.withhold && row + n == 0);
@@ -620,6 +630,8 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm
   }
   fence_mbar_init();
   __syncthreads();
+  let_next_start();
+  wait_for_previous();
   auto ask = [&](int place, int n) {
     const long long r = row + n * stride;
     const void* const src[3] = {static_cast<const T*>(p.x) + r * p.ldx, static_cast<const T*>(p.dout) + r * p.ld_dout,
@@ -649,7 +661,6 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm
   const int span = round_up_pow2(blockDim.x >> 5);
   float2* const slots = shared.slots[span > 1 ? threadIdx.y : 0][0];
   const float inv_d = 1.0f / static_cast<float>(p.d);
-  let_next_start();
   char* out = static_cast<char*>(p.dx) + row * p.ld_dx * kSize + threadIdx.x * 16;
   for (int n = 0; n < rows; ++n) {
     const float rstd = next_rstd;
@@ -781,6 +792,8 @@ __global__ void __launch_bounds__(kShortThreads) norm_forward_short_kernel(const
   constexpr int P = kPerVector<T>, R = 4;
   const int c = threadIdx.x * P;
   const bool valid = c < p.d;
+  let_next_start();
+  wait_for_previous();
   Columns<W, 1, P> weight, bias;
   weight.init(p.weight, 0x3f803f80u, p.d);
   if (kLayer) bias.init(p.bias, 0u, p.d);
@@ -837,10 +850,11 @@ __global__ void __launch_bounds__(kShortThreads) norm_forward_short_kernel(const
 template <typename T, typename W, bool kLayer>
 __global__ void __launch_bounds__(kShortThreads) norm_backward_short_kernel(const NormBackwardParams p) {
   constexpr int P = kPerVector<T>, R = 2;
-  let_next_start();
   __shared__ float joined[2][kShortThreads * P];  // [parts][columns]
   const int c = threadIdx.x * P;
   const bool valid = c < p.d, residual = p.residual != nullptr;
+  let_next_start();
+  wait_for_previous();
   Columns<W, 1, P> weight;
   weight.init(p.weight, 0x3f803f80u, p.d);
   Pair dw[P / 2], db[P / 2];
@@ -921,6 +935,7 @@ __global__ void __launch_bounds__(32 * kNormReduceRows) norm_reduce_kernel(const
   __shared__ float shared[kBias ? 2 : 1][kNormReduceRows][33];
   const int i = blockIdx.x * 32 + threadIdx.x;
   float dw = 0.0f, db = 0.0f;
+  let_next_start();
   wait_for_previous();
   if (i < p.d) {
     for (int s = threadIdx.y; s < p.splits; s += kNormReduceRows) {

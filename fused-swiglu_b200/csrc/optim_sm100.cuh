@@ -29,7 +29,7 @@ namespace fsw {
 constexpr int kAdamThreads = 256;
 constexpr int kAdamGroup = 8;                              // elements of a thread at a time
 constexpr int kAdamBlock = 256;                            // elements that share a scale: one warp's groups
-constexpr int kAdamChunk = kAdamThreads * kAdamGroup * 2;  // elements of a thread block at a time
+constexpr int kAdamPart = kAdamThreads * kAdamGroup;       // elements of a thread block at a time
 
 struct AdamTensor {
   void* param;
@@ -58,6 +58,10 @@ struct AdamTable {
   uint32_t first_chunk[kCapacity + 1];  // of this launch's chunks; the last entry is their number
   long long first_block[kCapacity];     // of the call's blocks of 256: what the random bits are counted by
   int count;
+  int parts;  // of kAdamPart elements in a chunk
+  uint32_t* status;  // of the bounded waits
+  unsigned long long wait_limit_ns;
+  int withhold;  // test aid: the first part's copies are left out
   AdamOptions opt;
 };
 
@@ -104,24 +108,10 @@ __device__ __forceinline__ AdamRates adam_rates(const AdamOptions& o) {
   return r;
 }
 
-// m, v and p of one element from b1 m, b2 v and the gradient.  The root and the quotient are the fast ones, off by a few
-// units of fp32: p alone depends on them.
-__device__ __forceinline__ void adam_element(const AdamOptions& o, const AdamRates& r, float g, float old_m, float old_v,
-                                             float& m, float& v, float& p) {
-  g = __fmul_rn(g, r.scale);
-  m = __fadd_rn(old_m, __fmul_rn(o.one_minus_beta1, g));
-  v = __fadd_rn(old_v, __fmul_rn(o.one_minus_beta2, __fmul_rn(g, g)));
-  float root, quotient;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  root = fmaf(root, r.inv_sqrt_correction2, o.eps);
-  asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(quotient) : "f"(r.step_size * m), "f"(root));
-  p = fmaf(p, r.decay, -quotient);
-}
-
 // ---- 8-bit floats with a block's scale ----
 
 // Values of eight codes, without the scale.
-__device__ __forceinline__ void decode_e4m3x8(uint2 q, float (&v)[kAdamGroup]) {
+__device__ __forceinline__ void decode_e4m3x8(uint2 q, Pair (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = i < 2 ? q.x : q.y;
@@ -129,42 +119,50 @@ __device__ __forceinline__ void decode_e4m3x8(uint2 q, float (&v)[kAdamGroup]) {
     uint32_t halves;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&halves));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    v[i] = make_pair(f.x, f.y);
   }
 }
 
 // An e5m2 is the upper byte of a half.
-__device__ __forceinline__ void decode_e5m2x8(uint2 q, float (&v)[kAdamGroup]) {
+__device__ __forceinline__ void decode_e5m2x8(uint2 q, Pair (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t halves = __byte_perm(i < 2 ? q.x : q.y, 0u, (i & 1) ? 0x3424 : 0x1404);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&halves));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    v[i] = make_pair(f.x, f.y);
   }
 }
 
-// The scale of a block whose largest magnitude has the fp32 bits `peak`, and its inverse; the largest value comes
-// below 2^(top + 1).  The lower bound on the exponent keeps both normal.
-__device__ __forceinline__ float2 block_scale(uint32_t peak, uint32_t top) {
-  const uint32_t field = max(peak >> 23, top + 1);
-  if (field >= 255u) return make_float2(__uint_as_float(0x7fc00000u), 0.0f);
-  return make_float2(__uint_as_float((field - top) << 23), __uint_as_float((254u + top - field) << 23));
+// How a block whose largest magnitude has the fp32 bits `peak` is encoded: its scale, the power of two that brings its values
+// to where the exponents of the 8-bit type, its subnormal ones too, are those of fp32, and whether they have to come down by
+// 2^-100 first, so that this power is a normal number.  `top`: the type's exponent that the largest value gets; `low`: the
+// difference of the types' biases.
+struct BlockScale {
+  float scale, factor;
+  bool down;
+};
+__device__ __forceinline__ BlockScale block_scale(uint32_t peak, int top, int low) {
+  const int field = max(static_cast<int>(peak >> 23), top + 1);  // keeps the scale normal
+  BlockScale b;
+  b.scale = field < 255 ? __uint_as_float(static_cast<uint32_t>(field - top) << 23) : __uint_as_float(0x7fc00000u);
+  const int exponent = 254 + top - low - field;
+  b.down = exponent < 1;
+  b.factor = __uint_as_float(static_cast<uint32_t>(b.down ? exponent + 100 : exponent) << 23);
+  return b;
 }
 
-// A value brought to where the exponents of the 8-bit type, its subnormal ones too, are those of fp32; then the bits that
-// the type keeps are the upper ones, and random bits added below them round up as often as the rest is large.
-__device__ __forceinline__ uint32_t encode_e4m3(float m, float inverse, uint32_t bits) {
-  const float t = m * inverse * 0x1p-120f;
-  const uint32_t x = (__float_as_uint(t) + ((bits & 0xffffu) << 4)) >> 20;  // sign in bit 11, code in bits 0 to 6
-  return (x & 0x7fu) | ((x >> 4) & 0x80u);
+// The bits that the 8-bit type keeps are the upper ones of t; random bits added below them round up as often as the rest is
+// large.  The code comes in the uppermost byte.
+__device__ __forceinline__ uint32_t encode_e4m3(float t, uint32_t bits) {
+  const uint32_t x = __float_as_uint(t) + ((bits & 0xffffu) << 4);  // sign in bit 31, code in bits 20 to 26
+  return (x << 4) | (x & 0x80000000u);
 }
-
-__device__ __forceinline__ uint32_t encode_e5m2(float v, float inverse, uint32_t bits) {
-  const float t = v * inverse * 0x1p-112f;
-  const uint32_t code = (__float_as_uint(t) + ((bits >> 16) << 5)) >> 21;
-  return max(code, min(__float_as_uint(v), 1u));
+__device__ __forceinline__ uint32_t encode_e5m2(float t, float v, uint32_t bits) {
+  const uint32_t x = (__float_as_uint(t) + ((bits >> 16) << 5)) << 3;  // code in bits 21 to 27
+  return max(x, v > 0.0f ? 1u << 24 : 0u);
+}
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
 // The tensor that holds a chunk: the last whose first chunk is not behind it.
@@ -224,33 +222,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, bool whole, int n, uint2
   }
 }
 
-// Where a warp is in a launch's tensors: at one block of 256 elements, this thread at its eight.
-template <int kCapacity>
-struct AdamCursor {
-  const AdamTable<kCapacity>& t;
-  uint32_t chunk;
-  int part = 0, k = 0, n = 0;  // n: elements of this thread that exist
-  long long at = 0;
-  bool whole = false;
-
-  // To the first block from (chunk, part) on that has elements; false behind the last.  The same for all lanes of a warp.
-  __device__ __forceinline__ bool seek() {
-    const uint32_t chunks = t.first_chunk[t.count];
-    for (; chunk < chunks; chunk += gridDim.x, part = 0) {
-      if (part == 0) k = find_tensor(t.first_chunk, t.count, chunk);
-      const long long numel = t.tensors[k].numel >= 0 ? t.tensors[k].numel : ~t.tensors[k].numel;
-      at = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk + (part * kAdamThreads + threadIdx.x) * kAdamGroup;
-      if (part < kAdamChunk / (kAdamThreads * kAdamGroup) && numel > at / kAdamBlock * kAdamBlock) {
-        const long long left = numel - at;
-        n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
-        whole = t.tensors[k].numel >= 0 && n == kAdamGroup;
-        return true;
-      }
-    }
-    return false;
-  }
-};
-
 // Eight values as they lie in memory.
 template <typename T>
 struct RawGroup;
@@ -258,9 +229,13 @@ template <>
 struct RawGroup<float> {
   float v[kAdamGroup];
   __device__ __forceinline__ void load(const float* p, bool whole, int n) { load_group(p, whole, n, v); }
-  __device__ __forceinline__ void get(float (&out)[kAdamGroup]) const {
+  __device__ __forceinline__ void read(const float* p) {  // shared memory
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  __device__ __forceinline__ void get(Pair (&out)[4]) const {
 #pragma unroll
-    for (int i = 0; i < kAdamGroup; ++i) out[i] = v[i];
+    for (int i = 0; i < 4; ++i) out[i] = make_pair(v[2 * i], v[2 * i + 1]);
   }
 };
 template <>
@@ -279,102 +254,328 @@ struct RawGroup<__nv_bfloat16> {
       }
     }
   }
-  __device__ __forceinline__ void get(float (&out)[kAdamGroup]) const { unpack_bf16x8(w, out); }
+  __device__ __forceinline__ void read(const __nv_bfloat16* p) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+  }
+  __device__ __forceinline__ void get(Pair (&out)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = unpack_bf16x2(w[i]);
+  }
 };
 
-// P, G: types of parameters and gradients; kEight: 8-bit moments, else fp32 ones.  A warp takes one block of 256 elements at a
-// time, each thread eight neighbours, so that a block's largest magnitudes are one reduction over the warp.  With 8-bit
-// moments there is as much to compute as to move: the next block's values are on their way meanwhile.
-template <typename P, typename G, bool kEight, bool kMaster, int kCapacity>
-__global__ void __launch_bounds__(kAdamThreads, kEight ? 3 : 4) adamw_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* p, bool whole, int n, const Pair (&v)[4]) {
+  float f[kAdamGroup];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = split(v[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+  store_group(p, whole, n, f);
+}
+
+// The moments of one element, each product and sum rounded on its own.
+__device__ __forceinline__ void adam_moments(const AdamOptions& o, const AdamRates& r, float b1, float b2, float g, float& m, float& v) {
+  g = __fmul_rn(g, r.scale);
+  m = __fadd_rn(__fmul_rn(b1, m), __fmul_rn(o.one_minus_beta1, g));
+  v = __fadd_rn(__fmul_rn(b2, v), __fmul_rn(o.one_minus_beta2, __fmul_rn(g, g)));
+}
+
+// Fast roots and quotients, off by a unit or two of fp32: p alone depends on them.  Under the root a second moment below the
+// smallest normal number counts as that.
+__device__ __forceinline__ float adam_root(float v) {
+  float root;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(root) : "f"(v), "f"(0x1p-126f));
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(root));
+  return root;
+}
+__device__ __forceinline__ float adam_inverse_root(float root) {
+  float inverse;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(root));
+  return inverse;
+}
+
+// fp32 moments.  P, G: types of parameters and gradients.  A thread has eight neighbours at a time; three blocks an SM
+// keep enough on its way, and more of them are slower (3 x 45 M weights: three 595 us, four 599, five 645).
+template <typename P, typename G, bool kMaster, int kCapacity>
+__global__ void __launch_bounds__(kAdamThreads, 3) adamw32_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
   using Weight = typename std::conditional<kMaster, float, P>::type;
   const AdamOptions& o = t.opt;
+  let_next_start();
+  wait_for_previous();
   const AdamRates r = adam_rates(o);
-  if (r.skip) return;
-  AdamCursor<kCapacity> c{t, blockIdx.x};
-  RawGroup<Weight> raw_p;
-  RawGroup<G> raw_g;
-  RawGroup<float> raw_m, raw_v;
-  uint2 codes_m = make_uint2(0u, 0u), codes_v = codes_m;
-  float scale_m = 0.0f, scale_v = 0.0f;
-  auto fetch = [&]() {
-    const AdamTensor& a = t.tensors[c.k];
-    if (kEight) {
-      codes_m = load_codes(static_cast<const uint8_t*>(a.exp_avg) + c.at, c.whole, c.n);
-      codes_v = load_codes(static_cast<const uint8_t*>(a.exp_avg_sq) + c.at, c.whole, c.n);
-      if (c.n > 0) {
-        scale_m = a.exp_avg_scale[c.at / kAdamBlock];
-        scale_v = a.exp_avg_sq_scale[c.at / kAdamBlock];
-      }
-    } else {
-      raw_m.load(static_cast<const float*>(a.exp_avg) + c.at, c.whole, c.n);
-      raw_v.load(static_cast<const float*>(a.exp_avg_sq) + c.at, c.whole, c.n);
-    }
-    raw_g.load(static_cast<const G*>(a.grad) + c.at, c.whole, c.n);
-    raw_p.load(kMaster ? reinterpret_cast<const Weight*>(a.master) + c.at : static_cast<const Weight*>(a.param) + c.at, c.whole, c.n);
-  };
-  bool more = c.seek();
-  if (kEight && more) fetch();
-  while (more) {
-    if (!kEight) fetch();
-    const AdamTensor& a = t.tensors[c.k];
-    const long long at = c.at, block = at / kAdamBlock;
-    const unsigned long long group = (t.first_block[c.k] + block) * (kAdamBlock / kAdamGroup) + (threadIdx.x & 31);
-    const int n = c.n;
-    const bool whole = c.whole;
-    float m[kAdamGroup], v[kAdamGroup], p[kAdamGroup], g[kAdamGroup];
-    if (kEight) {
-      decode_e4m3x8(codes_m, m);
-      decode_e5m2x8(codes_v, v);
-    } else {
-      raw_m.get(m);
-      raw_v.get(v);
-    }
-    raw_g.get(g);
-    raw_p.get(p);
-    // the scale is a power of two: b times the scale, and that times the code, rounds as b times the value does
-    const float b1 = kEight ? o.beta1 * scale_m : o.beta1, b2 = kEight ? o.beta2 * scale_v : o.beta2;
-    ++c.part;
-    more = c.seek();
-    if (kEight && more) fetch();
-    uint32_t peak_m = 0, peak_v = 0;
-#pragma unroll
-    for (int i = 0; i < kAdamGroup; ++i) {
-      adam_element(o, r, g[i], __fmul_rn(b1, m[i]), __fmul_rn(b2, v[i]), m[i], v[i], p[i]);
-      if (kEight) {
-        peak_m = max(peak_m, __float_as_uint(m[i]) & 0x7fffffffu);
-        peak_v = max(peak_v, __float_as_uint(v[i]) & 0x7fffffffu);
-      }
-    }
-    if (kMaster) store_group(a.master + at, whole, n, p);
-    store_group(static_cast<P*>(a.param) + at, whole, n, p);
-    if (kEight) {
-      peak_m = __reduce_max_sync(0xffffffffu, peak_m);
-      peak_v = __reduce_max_sync(0xffffffffu, peak_v);
-      const float2 cm = block_scale(peak_m, 7), cv = block_scale(peak_v, 14);
-      const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
-      if ((threadIdx.x & 31) == 0) {
-        a.exp_avg_scale[block] = cm.x;
-        a.exp_avg_sq_scale[block] = cv.x;
-      }
-      uint2 qm = make_uint2(0u, 0u), qv = qm;
+  const uint32_t chunks = t.first_chunk[t.count];
+  const int chunk_size = t.parts * kAdamPart;
+  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    const int k = find_tensor(t.first_chunk, t.count, chunk);
+    const AdamTensor& a = t.tensors[k];
+    const bool vector = a.numel >= 0;
+    const long long base = static_cast<long long>(chunk - t.first_chunk[k]) * chunk_size;
+    const int size = static_cast<int>(min((vector ? a.numel : ~a.numel) - base, static_cast<long long>(chunk_size)));
+#pragma unroll 1
+    for (int e = threadIdx.x * kAdamGroup; e < size; e += kAdamPart) {
+      const int n = min(size - e, kAdamGroup);
+      const bool whole = vector && n == kAdamGroup;
+      const long long at = base + e;
+      float m[kAdamGroup], v[kAdamGroup], g[kAdamGroup], p[kAdamGroup];
+      load_group(static_cast<const float*>(a.exp_avg) + at, whole, n, m);
+      load_group(static_cast<const float*>(a.exp_avg_sq) + at, whole, n, v);
+      load_group(static_cast<const G*>(a.grad) + at, whole, n, g);
+      load_group((kMaster ? reinterpret_cast<const Weight*>(a.master) : static_cast<const Weight*>(a.param)) + at, whole, n, p);
+      if (r.skip) return;  // only here, where this is not waited for before the loads
 #pragma unroll
       for (int i = 0; i < kAdamGroup; ++i) {
-        const uint32_t bits = h * odd_multiplier(i);
-        (i < 4 ? qm.x : qm.y) |= encode_e4m3(m[i], cm.y, bits) << (8 * (i & 3));
-        (i < 4 ? qv.x : qv.y) |= (encode_e5m2(v[i], cv.y, bits) & 0xffu) << (8 * (i & 3));
+        adam_moments(o, r, o.beta1, o.beta2, g[i], m[i], v[i]);
+        p[i] = fmaf(-r.step_size * m[i], adam_inverse_root(fmaf(adam_root(v[i]), r.inv_sqrt_correction2, o.eps)), p[i] * r.decay);
       }
-      store_codes(static_cast<uint8_t*>(a.exp_avg) + at, whole, n, qm);
-      store_codes(static_cast<uint8_t*>(a.exp_avg_sq) + at, whole, n, qv);
-    } else {
+      if (kMaster) store_group(a.master + at, whole, n, p);
+      store_group(static_cast<P*>(a.param) + at, whole, n, p);
       store_group(static_cast<float*>(a.exp_avg) + at, whole, n, m);
       store_group(static_cast<float*>(a.exp_avg_sq) + at, whole, n, v);
     }
   }
 }
 
+// ---- 8-bit moments ----
+//
+// There is nearly as much to compute as to move, and a warp that waits for its loads does not compute: a part's values come
+// by bulk copies into a ring of shared memory, asked for by a warp of their own while the eight others work on earlier
+// parts.  A part at a tensor's end, or of a tensor whose pointers are not aligned, is loaded by its threads.
+
+constexpr int kAdam8Places = 3;
+constexpr int kAdam8RingThreads = kAdamThreads + 32;
+constexpr int kAdam8Blocks = 2;  // of an SM
+
+struct Adam8Part {  // of one place: what it holds
+  long long base;   // first element
+  int k, size;      // tensor, elements
+};
+
+template <typename Weight, typename G>
+struct Adam8Place {
+  __align__(128) Weight p[kAdamPart];
+  __align__(16) G g[kAdamPart];
+  __align__(16) uint8_t m[kAdamPart], v[kAdamPart];
+  __align__(16) float scale_m[kAdamPart / kAdamBlock], scale_v[kAdamPart / kAdamBlock];
+};
+
+template <typename Weight, typename G>
+struct Adam8Shared {
+  Adam8Place<Weight, G> place[kAdam8Places];
+  Adam8Part part[kAdam8Places];
+  unsigned long long full[kAdam8Places], empty[kAdam8Places];
+  uint32_t abort_flag;
+};
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// The part of a launch: copied where it is whole and aligned.
+template <bool kRing, int kCapacity>
+__device__ __forceinline__ Adam8Part adam8_part(const AdamTable<kCapacity>& t, uint32_t part) {
+  const int k = find_tensor(t.first_chunk, t.count, part);
+  const long long numel = t.tensors[k].numel, base = static_cast<long long>(part - t.first_chunk[k]) * kAdamPart;
+  const int size = static_cast<int>(min((numel >= 0 ? numel : ~numel) - base, static_cast<long long>(kAdamPart)));
+  return Adam8Part{base, kRing && numel >= 0 && size == kAdamPart ? k : ~k, size};
+}
+
+// One thread asks for this block's parts, a ring ahead of those that work on them.  Behind the last, or where a wait gave up,
+// it sees to it that no copy is on its way any more.
+template <typename Weight, typename G, bool kMaster, int kCapacity>
+__device__ __forceinline__ void adam8_ask(const AdamTable<kCapacity>& t, Adam8Shared<Weight, G>& sh, const Watchdog& wd) {
+  const uint32_t parts = t.first_chunk[t.count];
+  int i = 0;
+  for (uint32_t part = blockIdx.x; part < parts; part += gridDim.x, ++i) {
+    const int at = i % kAdam8Places;
+    const uint32_t full = smem_u32(&sh.full[at]);
+    if (i >= kAdam8Places && !wd.wait(smem_u32(&sh.empty[at]), (i / kAdam8Places - 1) & 1, kSiteAdamRing)) break;
+    const Adam8Part here = adam8_part<true>(t, part);
+    sh.part[at] = here;
+    if (here.k < 0) {
+      mbar_arrive(full);
+      continue;
+    }
+    if (t.withhold && part == 0) {
+      mbar_arrive_expect_tx(full, 16);
+      continue;
+    }
+    const AdamTensor& a = t.tensors[here.k];
+    const long long base = here.base, block = base / kAdamBlock;
+    Adam8Place<Weight, G>& place = sh.place[at];
+    mbar_arrive_expect_tx(full, sizeof(place.p) + sizeof(place.g) + sizeof(place.m) + sizeof(place.v) + sizeof(place.scale_m) +
+                                    sizeof(place.scale_v));
+    bulk_copy(place.p, (kMaster ? reinterpret_cast<const Weight*>(a.master) : static_cast<const Weight*>(a.param)) + base,
+              sizeof(place.p), full);
+    bulk_copy(place.g, static_cast<const G*>(a.grad) + base, sizeof(place.g), full);
+    bulk_copy(place.m, static_cast<const uint8_t*>(a.exp_avg) + base, sizeof(place.m), full);
+    bulk_copy(place.v, static_cast<const uint8_t*>(a.exp_avg_sq) + base, sizeof(place.v), full);
+    bulk_copy(place.scale_m, a.exp_avg_scale + block, sizeof(place.scale_m), full);
+    bulk_copy(place.scale_v, a.exp_avg_sq_scale + block, sizeof(place.scale_v), full);
+  }
+  const unsigned long long t0 = global_timer_ns();
+  for (int j = max(0, i - kAdam8Places); j < i; ++j) {
+    while (!mbar_try_wait(smem_u32(&sh.full[j % kAdam8Places]), (j / kAdam8Places) & 1) &&
+           !(wd.aborted() && global_timer_ns() - t0 > kDrainLimitNs)) {
+      if (global_timer_ns() - t0 > wd.limit_ns) wd.give_up(kSiteAdamRing);
+    }
+  }
+}
+
+// Eight elements of a thread.
+struct AdamGroup {
+  Pair m[4], v[4], p[4], g[4];
+};
+
+// m, v and p from b1 and b2 times m and v, and the gradient, two at a time where that may be (pairs' products and sums may
+// come fused, which the moments' must not).
+__device__ __forceinline__ void adam_step(const AdamOptions& o, const AdamRates& r, float b1, float b2, AdamGroup& a) {
+  const Pair inv = both(r.inv_sqrt_correction2), eps = both(o.eps), rate = both(-r.step_size), decay = both(r.decay);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 g = split(a.g[i]);
+    float2 m = split(a.m[i]), v = split(a.v[i]);
+    adam_moments(o, r, b1, b2, g.x, m.x, v.x);
+    adam_moments(o, r, b1, b2, g.y, m.y, v.y);
+    a.m[i] = make_pair(m.x, m.y);
+    a.v[i] = make_pair(v.x, v.y);
+    const float2 root = split(fma2(make_pair(adam_root(v.x), adam_root(v.y)), inv, eps));
+    a.p[i] = fma2(a.m[i] * rate, make_pair(adam_inverse_root(root.x), adam_inverse_root(root.y)), a.p[i] * decay);
+  }
+}
+
+// P, G: types of parameters and gradients.  A warp takes one block of 256 elements of a part, each thread eight neighbours, so
+// that a block's largest magnitudes are one reduction over the warp.
+template <typename P, typename G, bool kMaster, bool kRing, int kCapacity>
+__global__ void __launch_bounds__(kRing ? kAdam8RingThreads : kAdamThreads, kRing ? kAdam8Blocks : 4) adamw8_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
+  using Weight = typename std::conditional<kMaster, float, P>::type;
+  extern __shared__ __align__(128) unsigned char memory[];
+  Adam8Shared<Weight, G>& sh = *reinterpret_cast<Adam8Shared<Weight, G>*>(memory);
+  const AdamOptions& o = t.opt;
+  const Watchdog wd{&sh.abort_flag, t.status, t.wait_limit_ns};
+  if (kRing) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kAdam8Places; ++i) {
+        mbar_init(smem_u32(&sh.full[i]), 1);
+        mbar_init(smem_u32(&sh.empty[i]), kAdamThreads / 32);
+      }
+      sh.abort_flag = 0;
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  let_next_start();
+  wait_for_previous();
+  const AdamRates r = adam_rates(o);
+  if (kRing && r.skip) return;
+  if (kRing && threadIdx.x >= kAdamThreads) {
+    if (threadIdx.x == kAdamThreads) adam8_ask<Weight, G, kMaster>(t, sh, wd);
+    return;
+  }
+  const uint32_t parts = t.first_chunk[t.count];
+  const int e = threadIdx.x * kAdamGroup, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int at = 0;
+  uint32_t phase = 0;
+  for (uint32_t part = blockIdx.x; part < parts; part += gridDim.x) {
+    // a warp that gives up leaves what it has not read as it was
+    if (kRing && !__all_sync(0xffffffffu, wd.wait(smem_u32(&sh.full[at]), phase, kSiteAdamRing))) return;
+    const Adam8Part here = kRing ? sh.part[at] : adam8_part<false>(t, part);
+    const bool copied = kRing && here.k >= 0;
+    const int k = copied ? here.k : ~here.k;
+    const AdamTensor& a = t.tensors[k];
+    const int n = min(max(here.size - e, 0), kAdamGroup);
+    const bool some = warp * kAdamBlock < here.size;  // of the warp's block
+    const long long first = here.base + e, block = here.base / kAdamBlock + warp;
+    uint2 codes_m, codes_v;
+    float scale_m = 0.0f, scale_v = 0.0f;
+    RawGroup<Weight> raw_p;
+    RawGroup<G> raw_g;
+    bool whole = true;
+    if (copied) {
+      const Adam8Place<Weight, G>& place = sh.place[at];
+      raw_p.read(place.p + e);
+      raw_g.read(place.g + e);
+      codes_m = *reinterpret_cast<const uint2*>(place.m + e);
+      codes_v = *reinterpret_cast<const uint2*>(place.v + e);
+      scale_m = place.scale_m[warp];
+      scale_v = place.scale_v[warp];
+    } else {
+      whole = a.numel >= 0 && n == kAdamGroup;
+      raw_p.load((kMaster ? reinterpret_cast<const Weight*>(a.master) : static_cast<const Weight*>(a.param)) + first, whole, n);
+      raw_g.load(static_cast<const G*>(a.grad) + first, whole, n);
+      codes_m = load_codes(static_cast<const uint8_t*>(a.exp_avg) + first, whole, n);
+      codes_v = load_codes(static_cast<const uint8_t*>(a.exp_avg_sq) + first, whole, n);
+      if (some) {
+        scale_m = a.exp_avg_scale[block];
+        scale_v = a.exp_avg_sq_scale[block];
+      }
+    }
+    if (kRing) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[at]));
+      if (++at == kAdam8Places) {
+        at = 0;
+        phase ^= 1;
+      }
+    }
+    if (!some) continue;
+    if (!kRing && r.skip) return;  // only here, where this is not waited for before the loads
+    AdamGroup q;
+    decode_e4m3x8(codes_m, q.m);
+    decode_e5m2x8(codes_v, q.v);
+    raw_g.get(q.g);
+    raw_p.get(q.p);
+    // the scale is a power of two: b times the scale, and that times the code, rounds as b times the value does
+    adam_step(o, r, o.beta1 * scale_m, o.beta2 * scale_v, q);
+    uint32_t peak_m = 0, peak_v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 m = split(q.m[i]), v = split(q.v[i]);
+      peak_m = max(peak_m, max(__float_as_uint(m.x) & 0x7fffffffu, __float_as_uint(m.y) & 0x7fffffffu));
+      peak_v = max(peak_v, max(__float_as_uint(v.x), __float_as_uint(v.y)));
+    }
+    const BlockScale bm = block_scale(__reduce_max_sync(0xffffffffu, peak_m), 7, 120);
+    const BlockScale bv = block_scale(__reduce_max_sync(0xffffffffu, peak_v), 14, 112);
+    if (kMaster) store_pairs(a.master + first, whole, n, q.p);
+    store_pairs(static_cast<P*>(a.param) + first, whole, n, q.p);
+    if (lane == 0) {
+      a.exp_avg_scale[block] = bm.scale;
+      a.exp_avg_sq_scale[block] = bv.scale;
+    }
+    const unsigned long long group = (t.first_block[k] + block) * (kAdamBlock / kAdamGroup) + lane;
+    const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
+    const Pair fm = both(bm.factor), fv = both(bv.factor);
+    if (bm.down || bv.down) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (bm.down) q.m[i] = q.m[i] * both(0x1p-100f);
+        if (bv.down) q.v[i] = q.v[i] * both(0x1p-100f);
+      }
+    }
+    uint32_t cm[kAdamGroup], cv[kAdamGroup];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 tm = split(q.m[i] * fm), tv = split(q.v[i] * fv), v = split(q.v[i]);
+      const uint32_t b0 = h * odd_multiplier(2 * i), b1 = h * odd_multiplier(2 * i + 1);
+      cm[2 * i] = encode_e4m3(tm.x, b0);
+      cm[2 * i + 1] = encode_e4m3(tm.y, b1);
+      cv[2 * i] = encode_e5m2(tv.x, v.x, b0);
+      cv[2 * i + 1] = encode_e5m2(tv.y, v.y, b1);
+    }
+    store_codes(static_cast<uint8_t*>(a.exp_avg) + first, whole, n,
+                make_uint2(upper_bytes(cm[0], cm[1], cm[2], cm[3]), upper_bytes(cm[4], cm[5], cm[6], cm[7])));
+    store_codes(static_cast<uint8_t*>(a.exp_avg_sq) + first, whole, n,
+                make_uint2(upper_bytes(cv[0], cv[1], cv[2], cv[3]), upper_bytes(cv[4], cv[5], cv[6], cv[7])));
+  }
+}
+
 // ---- 2-norm over many gradients ----
 
+constexpr int kGradChunk = 4 * kAdamPart;  // elements of a thread block at a time
 constexpr int kGradNormSlots = 1184;  // partial sums of squares, one a thread block: eight for each of 148 SMs
 
 struct GradTensor {
@@ -403,33 +604,54 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
   return s;
 }
 
-// Squares are summed in fp32 over a thread's elements of one chunk, and in fp64 from there on.
+// Squares of this thread's elements of kParts parts of a chunk from part `first` on, all loaded before the first is used: in
+// fp32 over two parts, sixteen elements, in fp64 from there on.
+template <int kParts, typename T>
+__device__ __forceinline__ double sum_squares(const T* p, bool vector, int size, int first) {
+  RawGroup<T> raw[kParts];
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const int e = (first + i) * kAdamPart + threadIdx.x * kAdamGroup, n = min(max(size - e, 0), kAdamGroup);
+    raw[i].load(p + e, vector && n == kAdamGroup, n);
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kParts; i += 2) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      Pair v[4];
+      raw[i + j].get(v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = split(v[k]);
+        s = fmaf(f.x, f.x, s);
+        s = fmaf(f.y, f.y, s);
+      }
+    }
+    sum += static_cast<double>(s);
+  }
+  return sum;
+}
+
 template <int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradTable<kCapacity> t) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
   let_next_start();
+  wait_for_previous();
   const uint32_t chunks = t.first_chunk[t.count];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
     const GradTensor& a = t.tensors[k];
-    const long long at = static_cast<long long>(chunk - t.first_chunk[k]) * kAdamChunk + threadIdx.x * kAdamGroup;
-    float g[2][kAdamGroup];
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const long long e = at + part * kAdamThreads * kAdamGroup;
-      const long long left = a.numel - e;
-      const int n = left <= 0 ? 0 : left < kAdamGroup ? static_cast<int>(left) : kAdamGroup;
-      const bool whole = a.vector && n == kAdamGroup;
-      if (a.f32) load_group(static_cast<const float*>(a.grad) + e, whole, n, g[part]);
-      else load_group(static_cast<const __nv_bfloat16*>(a.grad) + e, whole, n, g[part]);
+    const long long base = static_cast<long long>(chunk - t.first_chunk[k]) * kGradChunk;
+    const int size = static_cast<int>(min(a.numel - base, static_cast<long long>(kGradChunk)));
+    if (a.f32) {
+      sum += sum_squares<2>(static_cast<const float*>(a.grad) + base, a.vector, size, 0);
+      sum += sum_squares<2>(static_cast<const float*>(a.grad) + base, a.vector, size, 2);
+    } else {
+      sum += sum_squares<4>(static_cast<const __nv_bfloat16*>(a.grad) + base, a.vector, size, 0);
     }
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kAdamGroup; ++i) s = fmaf(g[0][i], g[0][i], s);
-#pragma unroll
-    for (int i = 0; i < kAdamGroup; ++i) s = fmaf(g[1][i], g[1][i], s);
-    sum += static_cast<double>(s);
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) t.slots[blockIdx.x] = t.accumulate ? t.slots[blockIdx.x] + sum : sum;
@@ -440,6 +662,7 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const do
                                                                        float* out) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
+  let_next_start();
   wait_for_previous();
   for (int i = threadIdx.x; i < count; i += kAdamThreads) sum += slots[i];
   sum = block_sum(sum, shared);

@@ -24,6 +24,7 @@ enum WaitSite : uint32_t {
   kSiteDecode = 7,          // decode kernels
   kSitePeer = 8,            // 2-CTA pair handshakes
   kSiteRowRing = 9,         // norms waiting for a row
+  kSiteAdamRing = 10,       // 8-bit AdamW waiting for a part, or for a place to put one
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s: default limit of every device-side wait

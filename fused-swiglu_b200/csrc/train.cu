@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <memory>
 #include <new>
+#include <type_traits>
 
 #include "../../include/fswiglu.h"
 #include "host_state.h"
@@ -22,25 +23,21 @@ bool known_type(int t) { return t == FSWIGLU_OUT_BF16 || t == FSWIGLU_OUT_F32; }
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 size_t type_bytes(int t) { return t == FSWIGLU_OUT_F32 ? 4u : 2u; }
 
-int launched() {
-  count_launch();
-  return cudaGetLastError() == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
-}
-
-// A launch that may start while the stream's previous kernel ends; the kernel itself waits for what that one wrote
-// (wait_for_previous).
+// A launch that may start while the stream's previous kernel ends: its blocks come up, and wait (wait_for_previous) before
+// they touch memory.
 template <typename... Params, typename... Args>
-int launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
+int launch(void (*kernel)(Params...), int64_t grid, dim3 block, size_t shared, cudaStream_t s, const Args&... args) {
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
+  config.gridDim = dim3(static_cast<unsigned>(grid));
   config.blockDim = block;
+  config.dynamicSmemBytes = shared;
   config.stream = s;
   config.attrs = &early;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<const std::decay_t<Params>&>(args)...);
   count_launch();
   return e == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
 }
@@ -90,9 +87,7 @@ template <typename T, bool kLayer, int N>
 int launch_norm_forward_narrow(const NormForwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
   const int64_t resident = static_cast<int64_t>(sms) * std::max(1, 1536 / (r.group * r.groups));
-  norm_forward_narrow_kernel<T, kLayer, N>
-      <<<static_cast<int>(std::min(blocks, resident)), dim3(r.group, r.groups), 0, s>>>(p);
-  return launched();
+  return launch(norm_forward_narrow_kernel<T, kLayer, N>, std::min(blocks, resident), dim3(r.group, r.groups), 0, s, p);
 }
 
 // How the wide kernels lay a row out: each thread holds `columns` of it.
@@ -157,8 +152,7 @@ int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Devi
   p.y_step = static_cast<long long>(grid) * w.groups * p.ldy * static_cast<long long>(sizeof(T));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  kernel<<<grid, dim3(w.group, w.groups), w.ring, s>>>(p);
-  return launched();
+  return launch(kernel, grid, dim3(w.group, w.groups), w.ring, s, p);
 }
 
 // Forward: 32 columns a thread, since a row's reductions cost every warp the same; 16 where a warp holds a whole row with
@@ -183,9 +177,8 @@ template <typename T, typename W, bool kLayer>
 int launch_norm_forward_short(const NormForwardParams& p, const Device& dev, cudaStream_t s) {
   const int lanes = short_lanes(p.d, kPerVector<T>), parts = kShortThreads / lanes;
   const int64_t blocks = (static_cast<int64_t>(p.M) + parts - 1) / parts;
-  norm_forward_short_kernel<T, W, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(dev.sms) * 8)), dim3(lanes, parts), 0, s>>>(p);
-  return launched();
+  return launch(norm_forward_short_kernel<T, W, kLayer>, std::min<int64_t>(blocks, static_cast<int64_t>(dev.sms) * 8),
+                dim3(lanes, parts), 0, s, p);
 }
 
 template <typename T, bool kLayer>
@@ -206,9 +199,8 @@ int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cuda
     if (r.vectors > 2 && r.vectors <= 8) return launch_norm_forward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
     if (r.vectors == 16) return launch_norm_forward_narrow<T, kLayer, 16>(p, r, dev.sms, s);
   }
-  norm_forward_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8)), kNormThreads, 0, s>>>(p);
-  return launched();
+  return launch(norm_forward_any_kernel<T, kLayer>, std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8),
+                dim3(kNormThreads), 0, s, p);
 }
 
 template <typename T, bool kLayer, int N>
@@ -218,8 +210,7 @@ int launch_norm_backward_narrow(NormBackwardParams& p, const RowShape& r, int sm
   const int grid = static_cast<int>(std::min(blocks, resident));
   p.splits = grid;
   const size_t shared = r.groups > 1 ? static_cast<size_t>(2) * r.group * N * sizeof(float) : 0;
-  norm_backward_narrow_kernel<T, kLayer, N><<<grid, dim3(r.group, r.groups), shared, s>>>(p);
-  return launched();
+  return launch(norm_backward_narrow_kernel<T, kLayer, N>, grid, dim3(r.group, r.groups), shared, s, p);
 }
 
 template <typename T, typename W, bool kLayer, int kColumns>
@@ -233,8 +224,7 @@ int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const De
   p.dx_step = static_cast<long long>(grid) * w.groups * p.ld_dx * static_cast<long long>(sizeof(T));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  kernel<<<grid, dim3(w.group, w.groups), w.ring, s>>>(p);
-  return launched();
+  return launch(kernel, grid, dim3(w.group, w.groups), w.ring, s, p);
 }
 
 // Backward: one block an SM, its registers full of the sums over rows.  Of the columns a thread may hold, those that keep most
@@ -262,8 +252,7 @@ int launch_norm_backward_short(NormBackwardParams& p, const Device& dev, cudaStr
   const int lanes = short_lanes(p.d, kPerVector<T>), parts = kShortThreads / lanes;
   const int64_t blocks = (static_cast<int64_t>(p.M) + parts - 1) / parts;
   p.splits = static_cast<int>(std::min<int64_t>({blocks, static_cast<int64_t>(dev.sms) * 2, kMaxNormSplits}));
-  norm_backward_short_kernel<T, W, kLayer><<<p.splits, dim3(lanes, parts), 0, s>>>(p);
-  return launched();
+  return launch(norm_backward_short_kernel<T, W, kLayer>, p.splits, dim3(lanes, parts), 0, s, p);
 }
 
 template <typename T, bool kLayer>
@@ -283,14 +272,13 @@ int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cu
     if (r.vectors > 0 && r.vectors <= 2) return launch_norm_backward_narrow<T, kLayer, 2>(p, r, dev.sms, s);
     if (r.vectors > 2) return launch_norm_backward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
   }
-  norm_backward_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8)), kNormThreads, 0, s>>>(p);
-  if (int rc = launched()) return rc;
+  if (int rc = launch(norm_backward_any_kernel<T, kLayer>, std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8),
+                      dim3(kNormThreads), 0, s, p))
+    return rc;
   if (p.partial == nullptr) return FSWIGLU_OK;
   const int64_t tiles = (p.d + kNormThreads - 1) / kNormThreads * static_cast<int64_t>(p.splits);
-  norm_backward_columns_any_kernel<T, kLayer>
-      <<<static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * 32)), kNormThreads, 0, s>>>(p);
-  return launched();
+  return launch(norm_backward_columns_any_kernel<T, kLayer>, std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * 32),
+                dim3(kNormThreads), 0, s, p);
 }
 
 // Whether a matrix's rows all start on 16 bytes.
@@ -397,9 +385,9 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
   q.d = static_cast<int>(d);
   q.splits = p.splits;
   q.out_f32 = grad_dtype == FSWIGLU_OUT_F32;
-  const dim3 grid(static_cast<unsigned>((d + 31) / 32)), block(32, kNormReduceRows);
-  return dbias != nullptr ? launch_after(norm_reduce_kernel<true>, grid, block, s, q)
-                          : launch_after(norm_reduce_kernel<false>, grid, block, s, q);
+  const dim3 block(32, kNormReduceRows);
+  return dbias != nullptr ? launch(norm_reduce_kernel<true>, (d + 31) / 32, block, 0, s, q)
+                          : launch(norm_reduce_kernel<false>, (d + 31) / 32, block, 0, s, q);
 }
 
 // ---- many tensors ----
@@ -443,48 +431,61 @@ Range range_of(const void* p, int64_t bytes) {
   return Range{b, b + static_cast<uintptr_t>(p == nullptr ? 0 : bytes)};
 }
 
-uint32_t chunks_of(int64_t numel) { return static_cast<uint32_t>((numel + kAdamChunk - 1) / kAdamChunk); }
+uint32_t chunks_of(int64_t numel, int64_t chunk) { return static_cast<uint32_t>((numel + chunk - 1) / chunk); }
 
-constexpr int64_t kMaxNumel = 1ll << 35;  // chunks of a full table are counted in 32 bits
-
-template <typename P, typename G, bool kEight, bool kMaster, int kCapacity>
-int launch_adamw(const AdamTable<kCapacity>& t, int sms, cudaStream_t s) {
-  const uint32_t grid = std::min<uint32_t>(t.first_chunk[t.count], static_cast<uint32_t>(sms) * 8u);
-  adamw_kernel<P, G, kEight, kMaster, kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
-  return launched();
-}
+constexpr int64_t kMaxNumel = 1ll << 34;  // chunks of a full table are counted in 32 bits
 
 struct AdamKind {
   bool param_f32, grad_f32, eight, master;
 };
 
-template <typename P, typename G, int kCapacity>
-int launch_adamw(const AdamTable<kCapacity>& t, const AdamKind& k, int sms, cudaStream_t s) {
-  if constexpr (sizeof(P) == 2) {
-    if (k.master) return k.eight ? launch_adamw<P, G, true, true>(t, sms, s) : launch_adamw<P, G, false, true>(t, sms, s);
+template <typename P, typename G, bool kMaster, int kCapacity>
+int launch_adamw(AdamTable<kCapacity>& t, const AdamKind& k, const Device& dev, cudaStream_t s) {
+  const int64_t chunks = t.first_chunk[t.count];
+  if (k.eight) {
+    // a ring pays where each block has several parts
+    const int64_t resident = static_cast<int64_t>(dev.sms) * kAdam8Blocks;
+    if (chunks >= 4 * resident) {
+      constexpr auto kernel = adamw8_kernel<P, G, kMaster, true, kCapacity>;
+      static_assert(sizeof(Adam8Shared<typename std::conditional<kMaster, float, P>::type, G>) <= kRingBytes / kAdam8Blocks,
+                    "the blocks of an SM share its memory");
+      static std::atomic<uint64_t> done{0};
+      if (int rc = opt_in(kernel, &done, dev)) return rc;
+      t.withhold = take_withhold();
+      // all of the SM's memory for its two blocks: a third one, of a launch that starts early, would leave other SMs one
+      return launch(kernel, resident, dim3(kAdam8RingThreads), kRingBytes / kAdam8Blocks, s, t);
+    }
+    return launch(adamw8_kernel<P, G, kMaster, false, kCapacity>, chunks, dim3(kAdamThreads), 0, s, t);
   }
-  return k.eight ? launch_adamw<P, G, true, false>(t, sms, s) : launch_adamw<P, G, false, false>(t, sms, s);
+  // a block for each chunk: SMs that are done take the next (3 x 45 M weights: 559 us; 16 blocks an SM that stay: 584)
+  return launch(adamw32_kernel<P, G, kMaster, kCapacity>, std::min<int64_t>(chunks, 1 << 30), dim3(kAdamThreads), 0, s, t);
 }
 
 template <int kCapacity>
-int launch_adamw(const AdamTable<kCapacity>& t, const AdamKind& k, int sms, cudaStream_t s) {
+int launch_adamw(AdamTable<kCapacity>& t, const AdamKind& k, const Device& dev, cudaStream_t s) {
   using BF = __nv_bfloat16;
-  if (k.param_f32) return k.grad_f32 ? launch_adamw<float, float>(t, k, sms, s) : launch_adamw<float, BF>(t, k, sms, s);
-  return k.grad_f32 ? launch_adamw<BF, float>(t, k, sms, s) : launch_adamw<BF, BF>(t, k, sms, s);
+  if (k.param_f32) return k.grad_f32 ? launch_adamw<float, float, false>(t, k, dev, s) : launch_adamw<float, BF, false>(t, k, dev, s);
+  if (k.master) return k.grad_f32 ? launch_adamw<BF, float, true>(t, k, dev, s) : launch_adamw<BF, BF, true>(t, k, dev, s);
+  return k.grad_f32 ? launch_adamw<BF, float, false>(t, k, dev, s) : launch_adamw<BF, BF, false>(t, k, dev, s);
 }
 
-// Whether every pointer of a tensor takes the wide accesses of eight elements.
+// Whether every pointer of a tensor takes the wide accesses of eight elements, and bulk copies.
 bool wide(const fswiglu_adamw_tensor& a, const AdamKind& k) {
-  const size_t p = k.param_f32 ? 32 : 16, g = k.grad_f32 ? 32 : 16, m = k.eight ? 8 : 32;
-  return aligned(a.param, p) && aligned(a.grad, g) && aligned(a.exp_avg, m) && aligned(a.exp_avg_sq, m) && aligned(a.master, 32);
+  const size_t p = k.param_f32 ? 32 : 16, g = k.grad_f32 ? 32 : 16, m = k.eight ? 16 : 32;
+  return aligned(a.param, p) && aligned(a.grad, g) && aligned(a.exp_avg, m) && aligned(a.exp_avg_sq, m) && aligned(a.master, 32) &&
+         aligned(a.exp_avg_scale, 16) && aligned(a.exp_avg_sq_scale, 16);
 }
 
 template <int kCapacity>
-int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const AdamOptions& o, AdamKind kind, int sms,
-                   cudaStream_t s) {
+int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const AdamOptions& o, AdamKind kind, int parts,
+                   const Device& dev, cudaStream_t s) {
   AdamTable<kCapacity> t;
   t.opt = o;
   t.count = 0;
+  t.parts = parts;
+  t.status = dev.status;
+  t.wait_limit_ns = dev.wait_limit_ns;
+  t.withhold = 0;
   t.first_chunk[0] = 0;
   long long blocks = 0;
   for (int64_t i = 0; i < count; ++i) {
@@ -492,7 +493,7 @@ int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const Ada
     if (a.numel > 0) {
       // one launch's tensors all have a master or none has
       if (t.count > 0 && (a.master != nullptr) != kind.master) {
-        if (int rc = launch_adamw<kCapacity>(t, kind, sms, s)) return rc;
+        if (int rc = launch_adamw<kCapacity>(t, kind, dev, s)) return rc;
         t.count = 0;
       }
       kind.master = a.master != nullptr;
@@ -500,12 +501,12 @@ int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const Ada
       t.tensors[t.count] = AdamTensor{a.param,  a.grad, a.exp_avg, a.exp_avg_sq, a.master, a.exp_avg_scale,
                                       a.exp_avg_sq_scale, wide(a, kind) ? n : ~n};
       t.first_block[t.count] = blocks;
-      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(a.numel);
+      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(a.numel, static_cast<int64_t>(t.parts) * kAdamPart);
       blocks += (a.numel + kAdamBlock - 1) / kAdamBlock;
       ++t.count;
     }
     if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
-    if (int rc = launch_adamw<kCapacity>(t, kind, sms, s)) return rc;
+    if (int rc = launch_adamw<kCapacity>(t, kind, dev, s)) return rc;
     t.count = 0;
   }
   return FSWIGLU_OK;
@@ -523,14 +524,13 @@ int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double
       const bool f32 = tensors[i].dtype == FSWIGLU_OUT_F32;
       t.tensors[t.count] = GradTensor{tensors[i].grad, static_cast<long long>(tensors[i].numel), f32,
                                       aligned(tensors[i].grad, f32 ? 32 : 16)};
-      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(tensors[i].numel);
+      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(tensors[i].numel, kGradChunk);
       ++t.count;
     }
     if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
     // every launch of a call has the same thread blocks: a later one adds to the slots of the first
     const int grid = std::min(kGradNormSlots, sms * 8);
-    grad_norm_kernel<kCapacity><<<grid, kAdamThreads, 0, s>>>(t);
-    if (int rc = launched()) return rc;
+    if (int rc = launch(grad_norm_kernel<kCapacity>, grid, dim3(kAdamThreads), 0, s, t)) return rc;
     *used = grid;
     t.accumulate = 1;
     t.count = 0;
@@ -634,9 +634,13 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
   o.seed_hi = static_cast<uint32_t>(in.seed >> 32);
   o.step_lo = static_cast<uint32_t>(in.step);
   const AdamKind kind = {param_dtype == FSWIGLU_OUT_F32, grad_dtype == FSWIGLU_OUT_F32, state_bits == 8, false};
+  // with fp32 moments two parts to a chunk where each SM has chunks enough
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += tensors[i].numel;
+  const int parts = state_bits == 32 && total / (2 * kAdamPart) >= 8 * dev.sms ? 2 : 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, kind, dev.sms, s)
-                              : adamw_launches<kLargeTable>(tensors, count, o, kind, dev.sms, s);
+  return count <= kSmallTable ? adamw_launches<kSmallTable>(tensors, count, o, kind, parts, dev, s)
+                              : adamw_launches<kLargeTable>(tensors, count, o, kind, parts, dev, s);
 }
 
 size_t fswiglu_grad_norm_workspace_bytes(void) { return kGradNormSlots * sizeof(double); }
@@ -663,8 +667,7 @@ int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, fl
   const int rc = count <= kSmallTable ? grad_norm_launches<kSmallTable>(tensors, count, slots, &used, dev.sms, s)
                                       : grad_norm_launches<kLargeTable>(tensors, count, slots, &used, dev.sms, s);
   if (rc) return rc;
-  return launch_after(grad_norm_finish_kernel, dim3(1), dim3(kAdamThreads), s, static_cast<const double*>(slots), used,
-                      max_norm, out);
+  return launch(grad_norm_finish_kernel, 1, dim3(kAdamThreads), 0, s, static_cast<const double*>(slots), used, max_norm, out);
 }
 
 }  // extern "C"

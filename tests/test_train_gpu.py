@@ -491,6 +491,27 @@ def test_adamw_step_of_long_lists(lib, cuda_dev, count, bits):
     canaries_hold(buffers)
 
 
+@pytest.mark.parametrize("bits,pt,gt,master", [(8, BF, BF, True), (8, F32, F32, False), (8, BF, F32, False), (32, BF, F32, True)])
+def test_adamw_step_of_tensors_that_go_round_every_block(lib, cuda_dev, bits, pt, gt, master):
+    """More parts than the blocks of a launch have room for at once, whole and ragged and unaligned ones among them."""
+    tensors, buffers = adam_inputs([6_000_013, 300_000, 2048 * 900, 77], pt, gt, bits, master, cuda_dev, 8, lead=[0, 1, 0, 0])
+    before = snapshot(tensors)
+    take_step(lib, tensors)
+    check_step(before, tensors, 7, 1e-2, 1.0, 11)
+    canaries_hold(buffers)
+
+
+def test_adamw_8bit_second_moments_too_large_for_fp32_say_so(lib, cuda_dev):
+    t = {"p": torch.ones(512), "g": torch.ones(512), "m": torch.zeros(512).to(torch.float8_e4m3fn),
+         "v": torch.zeros(512).to(torch.float8_e5m2), "ms": torch.zeros(2), "vs": torch.zeros(2)}
+    t["g"][5] = 1e25
+    tensors = [{k: v.to(cuda_dev) for k, v in t.items()}]
+    take_step(lib, tensors, step=1)
+    assert bool(torch.isfinite(tensors[0]["p"]).all()) and torch.isnan(tensors[0]["vs"]).tolist() == [True, False]
+    take_step(lib, tensors, step=2)
+    assert bool(torch.isnan(tensors[0]["p"][:256]).all()) and bool(torch.isfinite(tensors[0]["p"][256:]).all())
+
+
 def test_adamw_step_at_first_from_zero_state(lib, cuda_dev):
     for bits in (32, 8):
         tensors, _ = adam_inputs([1000], BF, BF, bits, True, cuda_dev, 1)

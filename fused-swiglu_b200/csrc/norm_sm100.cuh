@@ -422,22 +422,23 @@ struct RowRing {
       phase ^= 1;
     }
   }
-  // One thread of the group: ask for a row into a place.
-  __device__ __forceinline__ void ask(int place, const void* const (&src)[kArrays], int arrays, bool withhold) const {
-    if (wd.aborted()) return;
+  // One thread of the group: ask for a row into a place; whether it did.
+  __device__ __forceinline__ bool ask(int place, const void* const (&src)[kArrays], int arrays, bool withhold) const {
+    if (wd.aborted()) return false;
     const uint32_t bar = bars + 8 * place;
     mbar_arrive_expect_tx(bar, row_bytes * arrays);
-    if (withhold) return;
+    if (withhold) return true;
 #pragma unroll
     for (int i = 0; i < kArrays; ++i) {
       if (i < arrays) bulk_row(data + place * place_bytes + i * array_bytes, src[i], row_bytes, bar);
     }
+    return true;
   }
   __device__ __forceinline__ void wait() const { wd.wait(bars + 8 * at, phase, kSiteRowRing); }
-  // After a wait that gave up, behind the last row: what was asked for may still be on its way.
-  __device__ __noinline__ void drain(int rows) const {
+  // After a wait that gave up: the last of the `asked` rows may still be on their way.
+  __device__ __noinline__ void drain(int asked) const {
     const unsigned long long t0 = global_timer_ns();
-    for (int n = max(0, rows - places); n < rows; ++n) {
+    for (int n = max(0, asked - places); n < asked; ++n) {
       while (!mbar_try_wait(bars + 8 * (n % places), (n / places) & 1) && global_timer_ns() - t0 < kDrainLimitNs) {
       }
     }
@@ -533,9 +534,10 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
   __syncthreads();
   let_next_start();
   wait_for_previous();
+  int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const void* const src[1] = {static_cast<const T*>(p.x) + (row + n * stride) * p.ldx};
-    ring.ask(place, src, 1, p.ring.withhold && row + n == 0);
+    asked += ring.ask(place, src, 1, p.ring.withhold && row + n == 0);
   };
   const int ahead = ring.places - 1;
   if (threadIdx.x == 0) {
@@ -602,7 +604,7 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
       p.rstd[row + n * stride] = rstd;
     }
   }
-  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(rows);
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(asked);
 }
 
 // dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
@@ -632,11 +634,12 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm
   __syncthreads();
   let_next_start();
   wait_for_previous();
+  int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const long long r = row + n * stride;
     const void* const src[3] = {static_cast<const T*>(p.x) + r * p.ldx, static_cast<const T*>(p.dout) + r * p.ld_dout,
                                 static_cast<const T*>(p.residual) + (residual ? r * p.ld_res : 0)};
-    ring.ask(place, src, residual ? 3 : 2, p.ring.withhold && row + n == 0);
+    asked += ring.ask(place, src, residual ? 3 : 2, p.ring.withhold && row + n == 0);
   };
   const int ahead = ring.places - 1;
   if (threadIdx.x == 0) {
@@ -730,7 +733,7 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm
     out += p.dx_step;
     ring.advance();
   }
-  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(rows);
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(asked);
   if (p.partial == nullptr) return;
   // [group][2][columns]: the groups' sums side by side, joined in the order of the groups
   const int columns = blockDim.x * N * P, group_floats = 2 * columns;

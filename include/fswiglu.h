@@ -381,9 +381,10 @@ int64_t fswiglu_set_wait_limit_us(int64_t limit_us);
 
 /*
  * Test aid for the time-out path, no counterpart in the reference.  After fswiglu_test_expire_next_wait(1)
- * the NEXT kernel launch of this library (one launch, then the switch is off again) is made so that one of
- * its bounded waits cannot be satisfied: the first CTA of a tiled GEMM leaves out one operand copy, the
- * small-batch kernel expects one more CTA at its hand-over than exists.  Nothing faults, traps or spins
+ * the NEXT launch of a kernel that has such waits (one launch, then the switch is off again) is made so that one of
+ * them cannot be satisfied: the first CTA of a tiled GEMM leaves out one operand copy, the small-batch kernel expects
+ * one more CTA at its hand-over than exists, a norm leaves out its first row's copies and an AdamW step with 8-bit
+ * moments its first part's.  Nothing faults, traps or spins
  * without bound: the wait runs out after the limit above, the kernel unwinds and returns, the launch's
  * output is undefined and fswiglu_device_status() reports FSWIGLU_ERR_WATCHDOG with the site of the wait.
  * Use it with a limit of a few milliseconds.

@@ -276,3 +276,110 @@ def test_a_whole_training_step_from_a_captured_graph(fsw, cuda_dev, bits):
         assert int(replayed[-1]) == int(start[-1]) + 1
         for a, b in zip(state(), replayed):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---------------------------------------------------------------- waits, launches that overlap
+
+@pytest.mark.parametrize("which", ["layer_forward", "rms_forward", "layer_backward", "rms_backward", "adamw_8bit"])
+def test_a_copy_that_never_comes_is_reported_and_leaves_the_device_usable(fsw, cuda_dev, which):
+    """One launch whose first copy is left out, with a limit of a few milliseconds: the kernel ends by itself, the host reads
+    where a wait gave up, and the next call is right."""
+    import fused_mlp_module as lib
+
+    capi = fsw.capi
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn((900, 1024), generator=g).to(BF).to(cuda_dev)
+    w = torch.randn(1024, generator=g).to(BF).to(cuda_dev)
+    n = 6_000_000
+
+    def call():
+        if which == "layer_forward":
+            return lib.layer_norm_forward(x, w, w)
+        if which == "rms_forward":
+            return lib.rms_norm_forward(x, w)
+        stats = [v.float() for v in (x.float().mean(1), torch.rsqrt(x.float().var(1, unbiased=False) + 1e-5))]
+        if which == "layer_backward":
+            return lib.layer_norm_backward(x, x, *stats, w, True, x)
+        if which == "rms_backward":
+            return lib.rms_norm_backward(x, x, stats[1], w, x)
+        t = {"p": torch.zeros(n, device=cuda_dev), "g": torch.ones(n, device=cuda_dev),
+             "m": torch.zeros(n, dtype=torch.uint8, device=cuda_dev).view(torch.float8_e4m3fn),
+             "v": torch.zeros(n, dtype=torch.uint8, device=cuda_dev).view(torch.float8_e5m2),
+             "ms": torch.zeros((n + 255) // 256, device=cuda_dev), "vs": torch.zeros((n + 255) // 256, device=cuda_dev)}
+        lib.adamw_step([t["p"]], [t["g"]], [t["m"]], [t["v"]], 1, 1e-3, exp_avg_scales=[t["ms"]], exp_avg_sq_scales=[t["vs"]])
+        return t["p"], t["m"].view(torch.uint8), t["v"].view(torch.uint8), t["ms"]
+
+    want = call()
+    torch.cuda.synchronize()
+    assert capi.device_status() == 0
+    before = capi.lib.fswiglu_set_wait_limit_us(3000)
+    try:
+        capi.lib.fswiglu_test_expire_next_wait(1)
+        call()
+        torch.cuda.synchronize()
+        word = capi.device_status()
+    finally:
+        capi.lib.fswiglu_test_expire_next_wait(0)
+        capi.lib.fswiglu_set_wait_limit_us(before)
+    assert word & 0xFF == (10 if which == "adamw_8bit" else 9) and (word >> 8) - 1 == 0
+    assert capi.device_status() == 0
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+def test_launches_that_overlap_wait_for_what_was_written_before(fsw, cuda_dev):
+    """Every operator right behind a kernel, a copy, a fill and another stream's work that writes what it reads, many times over,
+    eagerly and captured."""
+    import fused_mlp_module as lib
+
+    g = torch.Generator().manual_seed(0)
+    source = [torch.randn((1500, 2048), generator=g).to(BF).to(cuda_dev) for _ in range(4)]
+    x, dy, w = torch.empty_like(source[0]), torch.empty_like(source[0]), source[3][0].clone()
+    p, m, v = (torch.empty(1500 * 2048, device=cuda_dev) for _ in range(3))
+    other = torch.cuda.Stream()
+
+    def chain(k):
+        x.copy_(source[k % 3])  # a copy
+        dy.zero_()  # a fill
+        dy.add_(source[(k + 1) % 3])  # a kernel
+        y, mean, rstd = lib.layer_norm_forward(x, w, w)
+        dx, dw, db = lib.layer_norm_backward(dy, x, mean, rstd, w, True, y)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            p.copy_(source[2].view(-1))
+            m.zero_()
+            v.fill_(1.0)
+        torch.cuda.current_stream().wait_stream(other)
+        clip = lib.grad_norm_clip([dx, dw, db], 1.0)
+        lib.adamw_step([p], [dx.view(-1)], [m], [v], 3, 1e-2, grad_scale=clip[1:])
+        lib.adamw_step([p], [dx.view(-1)], [m], [v], 4, 1e-2, grad_scale=clip[1:])
+        z = lib.rms_norm_forward(p.view(1500, 2048), None)[0]
+        x.zero_()  # behind the readers
+        dx_out = dx.clone()
+        dx.zero_()
+        return [y, dx_out, dw, db, clip, p.clone(), m.clone(), v.clone(), z]
+
+    want = []
+    for k in range(3):
+        torch.cuda.synchronize()
+        out = chain(k)
+        torch.cuda.synchronize()
+        want.append(out)
+    # against the plain formulas once, so that all agreeing on something wrong does not pass
+    x64 = source[0].double()
+    z64 = (x64 - x64.mean(1, keepdim=True)) / (x64.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    assert rel(want[0][0], z64 * w.double() + w.double()) <= 5e-3
+    assert rel(want[0][3], source[1].double().sum(0)) <= 5e-3
+    for k in range(60):
+        for a, b in zip(chain(k), want[k % 3]):
+            assert torch.equal(a, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [chain(k) for k in range(3)]
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    for out, ref in zip(outs, want):
+        for a, b in zip(out, ref):
+            assert torch.equal(a, b)

@@ -15,6 +15,12 @@
 
 namespace fsw {
 
+__device__ __forceinline__ void store_shared(uint32_t at, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void store_shared(uint32_t at, __nv_bfloat16 v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__bfloat16_as_ushort(v)) : "memory");
+}
 // Of the kernels that wait for rows on their way (below).
 struct RingParams {
   uint32_t* status;  // where a wait that gave up is recorded
@@ -189,14 +195,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_columns_any_kernel
   }
 }
 
-// ---- rows held in registers ----
+// ---- a group of threads a row ----
 //
-// For rows that start on no 16-byte boundary: element by element.  blockDim.x threads (a multiple of 32) hold one row, N
-// values each, and blockDim.y such groups of a block take rows of their own; a group's next row is on its way while the
-// present one is reduced.  A row is read once.
-
-constexpr int kNarrowGroups = 8;     // most groups of a block: each has a barrier of its own
-constexpr int kNarrowThreads = 512;  // most threads of a block
+// blockDim.x threads (a multiple of 32) take one row at a time, and blockDim.y such groups of a block rows of their own.
 
 __device__ __forceinline__ void group_barrier() {
   asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
@@ -227,157 +228,9 @@ __device__ __forceinline__ float2 group_sums(float2 v, float2* slots, int span) 
 
 __device__ __forceinline__ int round_up_pow2(int v) { return v <= 1 ? 1 : 1 << (32 - __clz(v - 1)); }
 
-template <typename T, bool kLayer, int N>
-__global__ void __launch_bounds__(kNarrowThreads) norm_forward_narrow_kernel(const NormForwardParams p) {
-  __shared__ float2 slots[kNarrowGroups][2][32];
-  let_next_start();
-  wait_for_previous();
-  float w[N], b[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = j * blockDim.x + threadIdx.x;
-    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
-    b[j] = kLayer && c < p.d ? load_vector(p.bias, c, p.w_f32, 0.0f) : 0.0f;
-  }
-  const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int span = round_up_pow2(blockDim.x >> 5), stride = gridDim.x * blockDim.y;
-  float2(&mine)[2][32] = slots[span > 1 ? threadIdx.y : 0];
-  int row = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  T raw[N];
-  auto fetch = [&](int r) {
-    const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = j * blockDim.x + threadIdx.x;
-      raw[j] = c < p.d ? x[c] : from_float<T>(0.0f);
-    }
-  };
-  if (row < p.M) fetch(row);
-  for (; row < p.M; row += stride) {
-    float x[N], s = 0.0f, ss = 0.0f, mean = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = to_float<T>(raw[j]);
-    if (row < p.M - stride) fetch(row + stride);
-    if (kLayer) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) s += x[j];
-      mean = group_sums<false>(make_float2(0.0f, s), mine[turn], span).y * inv_d;
-      turn ^= 1;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      x[j] = static_cast<int>(j * blockDim.x + threadIdx.x) < p.d ? x[j] - mean : 0.0f;
-      ss = fmaf(x[j], x[j], ss);
-    }
-    const float rstd = rsqrtf(fmaf(group_sums<false>(make_float2(0.0f, ss), mine[turn], span).y, inv_d, p.eps));
-    turn ^= 1;
-    T* y = static_cast<T*>(p.y) + row * p.ldy;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = j * blockDim.x + threadIdx.x;
-      if (c < p.d) y[c] = from_float<T>(fmaf(x[j] * rstd, w[j], b[j]));
-    }
-    if (threadIdx.x == 0) {
-      if (kLayer) p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-  }
-}
-
-// dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
-// block are joined in shared memory, and the blocks by norm_reduce_kernel.
-template <typename T, bool kLayer, int N>
-__global__ void __launch_bounds__(kNarrowThreads) norm_backward_narrow_kernel(const NormBackwardParams p) {
-  __shared__ float2 slots[kNarrowGroups][2][32];
-  extern __shared__ float joined[];  // [2][columns of a group], more than one group only
-  let_next_start();
-  wait_for_previous();
-  float w[N], dw[N], db[kLayer ? N : 1];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = j * blockDim.x + threadIdx.x;
-    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
-    dw[j] = 0.0f;
-    if (kLayer) db[j] = 0.0f;
-  }
-  const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int span = round_up_pow2(blockDim.x >> 5), stride = gridDim.x * blockDim.y;
-  float2(&mine)[2][32] = slots[span > 1 ? threadIdx.y : 0];
-  int row = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  T raw_x[N], raw_dy[N], raw_res[N];
-  float next_mean = 0.0f, next_rstd = 0.0f;
-  auto fetch = [&](int r) {
-    const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-    const T* dy = static_cast<const T*>(p.dout) + r * p.ld_dout;
-    const T* res = p.residual != nullptr ? static_cast<const T*>(p.residual) + r * p.ld_res : nullptr;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = j * blockDim.x + threadIdx.x;
-      raw_x[j] = c < p.d ? x[c] : from_float<T>(0.0f);
-      raw_dy[j] = c < p.d ? dy[c] : from_float<T>(0.0f);
-      raw_res[j] = c < p.d && res != nullptr ? res[c] : from_float<T>(0.0f);
-    }
-    if (kLayer) next_mean = p.mean[r];
-    next_rstd = p.rstd[r];
-  };
-  if (row < p.M) fetch(row);
-  for (; row < p.M; row += stride) {
-    float z[N], a[N], res[N];
-    const float mean = next_mean, rstd = next_rstd;
-    float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      // behind the row's end a is zero, and with it all that is summed
-      z[j] = (to_float<T>(raw_x[j]) - mean) * rstd;
-      a[j] = to_float<T>(raw_dy[j]);
-      res[j] = to_float<T>(raw_res[j]);
-      dw[j] = fmaf(a[j], z[j], dw[j]);
-      if (kLayer) db[j] += a[j];
-      a[j] *= w[j];
-      s.x += a[j];
-      s.y = fmaf(a[j], z[j], s.y);
-    }
-    if (row < p.M - stride) fetch(row + stride);
-    s = group_sums<kLayer>(s, mine[turn], span);
-    turn ^= 1;
-    const float c1 = kLayer ? s.x * inv_d : 0.0f, c2 = s.y * inv_d;
-    T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = j * blockDim.x + threadIdx.x;
-      if (c < p.d) dx[c] = from_float<T>(fmaf(fmaf(-z[j], c2, a[j] - c1), rstd, res[j]));
-    }
-  }
-  if (p.partial == nullptr) return;
-  float* part = p.partial + 2ll * blockIdx.x * p.d;
-  const int columns = blockDim.x * N;
-  for (int g = 0; g < static_cast<int>(blockDim.y); ++g) {
-    if (static_cast<int>(threadIdx.y) == g) {
-      const bool last = g + 1 == static_cast<int>(blockDim.y);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int c = j * blockDim.x + threadIdx.x;
-        if (g > 0) {
-          dw[j] += joined[c];
-          if (kLayer) db[j] += joined[columns + c];
-        }
-        if (!last) {
-          joined[c] = dw[j];
-          if (kLayer) joined[columns + c] = db[j];
-        } else if (c < p.d) {
-          part[c] = dw[j];
-          if (kLayer) part[p.d + c] = db[j];
-        }
-      }
-    }
-    if (blockDim.y > 1) __syncthreads();
-  }
-}
-
 // ---- rows through shared memory ----
 //
-// The wide form.  A group of blockDim.x threads (a multiple of 32) takes one row at a time, a block has blockDim.y groups, and
-// a group's rows to come are on their way into its ring of S places: one thread asks for a row's arrays by bulk copies, S - 1
+// A group's rows to come are on their way into its ring of S places: one thread asks for a row's arrays by bulk copies, S - 1
 // rows ahead, and all wait for their bytes on the place's barrier.  The bytes on the way cost neither registers, which the sums
 // over rows need, nor instructions of the threads that compute.  A place is free again once the group has met in the next
 // row's reduction.
@@ -391,6 +244,9 @@ struct WideShared {
   float2 slots[kWideMultiGroups][2][32];  // of each warp of a group, in turn
   uint32_t abort_flag;
 };
+
+// Bytes from the start of its 16-byte granule to an address.
+__device__ __forceinline__ uint32_t behind(const void* p) { return static_cast<uint32_t>(reinterpret_cast<uint64_t>(p)) & 15u; }
 
 // A group's ring: `places` places of kArrays rows of `row_bytes`.  The present row's place and its barrier's phase advance
 // row by row.
@@ -431,6 +287,56 @@ struct RowRing {
 #pragma unroll
     for (int i = 0; i < kArrays; ++i) {
       if (i < arrays) bulk_row(data + place * place_bytes + i * array_bytes, src[i], row_bytes, bar);
+    }
+    return true;
+  }
+  // The same for rows that start anywhere: whole granules of 16 bytes, so that a row lies in its place as far behind a granule's
+  // start as in memory.  What the granules hold beyond the row belongs to its neighbours.
+  template <typename T>
+  __device__ __forceinline__ bool ask_granules(int place, const T* const (&src)[kArrays], int arrays) const {
+    if (wd.aborted()) return false;
+    const uint32_t bar = bars + 8 * place;
+    uint32_t size[kArrays], bytes = 0;
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) {
+      size[i] = i < arrays ? (behind(src[i]) + row_bytes + 15u) & ~15u : 0u;
+      bytes += size[i];
+    }
+    mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) {
+      if (i < arrays) bulk_row(data + place * place_bytes + i * array_bytes, reinterpret_cast<const char*>(src[i]) - behind(src[i]), size[i], bar);
+    }
+    return true;
+  }
+  // The first row of all or the last has no neighbours on one side: the elements of its granule there, fewer than 16 bytes, are
+  // copied one by one.
+  template <typename T>
+  __device__ __noinline__ bool ask_edge(int place, const T* x, const T* dy, const T* res, int arrays, int d, bool first, bool last,
+                                        bool withhold) const {
+    if (wd.aborted()) return false;
+    const uint32_t bar = bars + 8 * place;
+    const T* const src[3] = {x, dy, res};
+    uint32_t bytes = withhold ? 16 : 0;
+    for (int turn = 0; turn < 2; ++turn) {  // what a barrier is to expect it is told before the copies begin
+      if (turn == 1) mbar_arrive_expect_tx(bar, bytes);
+      for (int i = 0; i < arrays; ++i) {
+        const uint64_t begin = reinterpret_cast<uint64_t>(src[i]), end = begin + static_cast<uint64_t>(d) * sizeof(T);
+        const uint64_t granule = begin & ~15ull;
+        const uint64_t lo = first ? (begin + 15) & ~15ull : granule, hi = last ? end & ~15ull : (end + 15) & ~15ull;
+        const uint32_t here = data + place * place_bytes + i * array_bytes, size = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+        if (turn == 1) {
+          if (size > 0 && !withhold) bulk_row(here + static_cast<uint32_t>(lo - granule), reinterpret_cast<const void*>(lo), size, bar);
+          continue;
+        }
+        if (!withhold) bytes += size;
+        for (uint64_t q = begin; first && q < lo && q < end; q += sizeof(T)) {
+          store_shared(here + static_cast<uint32_t>(q - granule), *reinterpret_cast<const T*>(q));
+        }
+        for (uint64_t q = hi < begin ? begin : hi; last && q < end; q += sizeof(T)) {
+          store_shared(here + static_cast<uint32_t>(q - granule), *reinterpret_cast<const T*>(q));
+        }
+      }
     }
     return true;
   }
@@ -768,6 +674,244 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm
       total.w += q.w;
     }
     *reinterpret_cast<float4*>(part + which * p.d + c) = total;
+  }
+}
+
+// ---- rows that start anywhere ----
+//
+// The same rings for rows that are not whole granules of 16 bytes, or not all on granules' starts.  A thread takes every
+// blockDim.x-th column, element by element, so that neighbours still read and write next to one another.
+
+constexpr int kOddThreads = 512;  // most threads of a block
+
+// Elements of two bytes go through shared memory on their way out: stored one by one they took most of the time.
+template <typename T>
+constexpr bool kStaged = sizeof(T) == 2;
+
+// Bytes of a place for one array: the granules that a row of a group's `columns` touches.
+__host__ __device__ constexpr uint32_t odd_array_bytes(int columns, int size) {
+  return static_cast<uint32_t>(columns) * size + 16u;  // columns are a multiple of 32
+}
+
+// A group's row from its staging memory, where it lies as far behind a granule's start as its target: whole granules by wide
+// stores, the elements before and behind them one by one.
+template <typename T>
+__device__ __forceinline__ void store_staged(T* target, const unsigned char* staging, int d, int span) {
+  if (span > 1) group_barrier();
+  else __syncwarp();
+  const int size = sizeof(T);
+  const int begin = static_cast<int>(reinterpret_cast<uint64_t>(target) & 15u), end = begin + d * size;
+  const int lo = min((begin + 15) & ~15, end), hi = max(end & ~15, lo);
+  char* const granule = reinterpret_cast<char*>(target) - begin;
+  for (int v = lo + static_cast<int>(threadIdx.x) * 16; v < hi; v += blockDim.x * 16) {
+    *reinterpret_cast<uint4*>(granule + v) = *reinterpret_cast<const uint4*>(staging + v);
+  }
+  const int head = (lo - begin) / size, tail = (end - hi) / size;  // below 16 bytes each
+  for (int i = threadIdx.x; i < head + tail; i += blockDim.x) {
+    const int at = i < head ? begin + i * size : hi + (i - head) * size;
+    *reinterpret_cast<T*>(granule + at) = *reinterpret_cast<const T*>(staging + at);
+  }
+}
+
+template <typename T, bool kLayer, int N>
+__global__ void __launch_bounds__(kOddThreads, 2) norm_forward_odd_kernel(const NormForwardParams p) {
+  __shared__ WideShared shared;
+  extern __shared__ __align__(128) unsigned char ring_memory[];  // [groups][places][granules]; [groups][granules]: rows to store
+  const int stride = gridDim.x * blockDim.y, row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int rows = row < p.M ? (p.M - 1 - row) / stride + 1 : 0;  // of this group
+  const uint32_t array = odd_array_bytes(blockDim.x * N, sizeof(T));
+  RowRing<1> ring(shared, ring_memory, array, p.d * static_cast<uint32_t>(sizeof(T)), p.ring);
+  fence_mbar_init();
+  __syncthreads();
+  let_next_start();
+  wait_for_previous();
+  auto source = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
+  int asked = 0;  // of the group's first thread
+  auto ask = [&](int place, int n) {
+    const T* const src[1] = {source(n)};
+    const int r = row + n * stride;
+    if (r > 0 && r < p.M - 1) asked += ring.ask_granules(place, src, 1);
+    else asked += ring.ask_edge(place, src[0], src[0], src[0], 1, p.d, r == 0, r == p.M - 1, p.ring.withhold && r == 0);
+  };
+  const int ahead = ring.places - 1;
+  if (threadIdx.x == 0) {
+    for (int n = 0; n < ahead && n < rows; ++n) ask(n, n);
+  }
+  float w[N], b[kLayer ? N : 1];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = j * blockDim.x + threadIdx.x;
+    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
+    if (kLayer) b[j] = c < p.d ? load_vector(p.bias, c, p.w_f32, 0.0f) : 0.0f;
+  }
+  const int span = round_up_pow2(blockDim.x >> 5);
+  float2* const slots = shared.slots[span > 1 ? threadIdx.y : 0][0];
+  unsigned char* const mine = ring_memory + threadIdx.y * ring.places * array;  // the group's ring
+  unsigned char* const staging = ring_memory + (blockDim.y * ring.places + threadIdx.y) * array;
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  int turn = 0;
+  for (int n = 0; n < rows; ++n) {
+    ring.wait();
+    const T* const here = reinterpret_cast<const T*>(mine + ring.at * array + behind(source(n)));
+    float x[N], s = 0.0f, ss = 0.0f, mean = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      const float v = to_float<T>(here[c]);  // behind the row's end whatever the place holds
+      x[j] = c < p.d ? v : 0.0f;
+      s += x[j];
+    }
+    if (kLayer) {
+      mean = group_sums<false>(make_float2(0.0f, s), slots + 32 * turn, span).y * inv_d;
+      turn ^= 1;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      x[j] = static_cast<int>(j * blockDim.x + threadIdx.x) < p.d ? x[j] - mean : 0.0f;
+      ss = fmaf(x[j], x[j], ss);
+    }
+    const float rstd = rsqrtf(fmaf(group_sums<false>(make_float2(0.0f, ss), slots + 32 * turn, span).y, inv_d, p.eps));
+    turn ^= 1;
+    // the group has read this row, and the one before it long ago: its place takes another
+    if (threadIdx.x == 0 && n + ahead < rows) ask(ring.before(), n + ahead);
+    T* const y = static_cast<T*>(p.y) + (row + n * stride) * p.ldy;
+    T* const stage = kStaged<T> ? reinterpret_cast<T*>(staging + behind(y)) : y;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      if (!kStaged<T> && c >= p.d) continue;
+      stage[c] = from_float<T>(kLayer ? fmaf(x[j] * rstd, w[j], b[kLayer ? j : 0]) : x[j] * rstd * w[j]);
+    }
+    if (kStaged<T>) store_staged(y, staging, p.d, span);
+    if (threadIdx.x == 0) {
+      if (kLayer) p.mean[row + n * stride] = mean;
+      p.rstd[row + n * stride] = rstd;
+    }
+    ring.advance();
+  }
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(asked);
+}
+
+template <typename T, bool kLayer, int N>
+__global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const NormBackwardParams p) {
+  __shared__ WideShared shared;
+  extern __shared__ __align__(128) unsigned char ring_memory[];  // [groups][places][x, dy, res][granules]; [groups][granules]: rows
+                                                                  // to store; at the end [groups][2][columns] fp32
+  const int stride = gridDim.x * blockDim.y, row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int rows = row < p.M ? (p.M - 1 - row) / stride + 1 : 0;  // of this group
+  const bool residual = p.residual != nullptr;
+  const uint32_t array = odd_array_bytes(blockDim.x * N, sizeof(T));
+  RowRing<3> ring(shared, ring_memory, array, p.d * static_cast<uint32_t>(sizeof(T)), p.ring);
+  fence_mbar_init();
+  __syncthreads();
+  let_next_start();
+  wait_for_previous();
+  auto x_of = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
+  auto dy_of = [&](int n) { return static_cast<const T*>(p.dout) + (row + n * stride) * p.ld_dout; };
+  auto res_of = [&](int n) { return static_cast<const T*>(p.residual) + (residual ? (row + n * stride) * p.ld_res : 0); };
+  int asked = 0;  // of the group's first thread
+  auto ask = [&](int place, int n) {
+    const T* const src[3] = {x_of(n), dy_of(n), res_of(n)};
+    const int r = row + n * stride;
+    const int arrays = residual ? 3 : 2;
+    if (r > 0 && r < p.M - 1) asked += ring.ask_granules(place, src, arrays);
+    else asked += ring.ask_edge(place, src[0], src[1], src[2], arrays, p.d, r == 0, r == p.M - 1, p.ring.withhold && r == 0);
+  };
+  const int ahead = ring.places - 1;
+  if (threadIdx.x == 0) {
+    for (int n = 0; n < ahead && n < rows; ++n) ask(n, n);
+  }
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  if (rows > 0) {
+    if (kLayer) next_mean = p.mean[row];
+    next_rstd = p.rstd[row];
+  }
+  float w[N], dw[N], db[kLayer ? N : 1];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = j * blockDim.x + threadIdx.x;
+    w[j] = c < p.d ? load_vector(p.weight, c, p.w_f32, 1.0f) : 0.0f;
+    dw[j] = 0.0f;
+    if (kLayer) db[j] = 0.0f;
+  }
+  const int span = round_up_pow2(blockDim.x >> 5);
+  float2* const slots = shared.slots[span > 1 ? threadIdx.y : 0][0];
+  unsigned char* const mine = ring_memory + threadIdx.y * ring.places * 3 * array;  // the group's ring
+  unsigned char* const staging = ring_memory + (blockDim.y * ring.places * 3 + threadIdx.y) * array;
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  for (int n = 0; n < rows; ++n) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (n + 1 < rows) {
+      if (kLayer) next_mean = p.mean[row + (n + 1) * stride];
+      next_rstd = p.rstd[row + (n + 1) * stride];
+    }
+    ring.wait();
+    const unsigned char* const here = mine + ring.at * 3 * array;
+    const T* const x = reinterpret_cast<const T*>(here + behind(x_of(n)));
+    const T* const dy = reinterpret_cast<const T*>(here + array + behind(dy_of(n)));
+    const T* const res = reinterpret_cast<const T*>(here + 2 * array + behind(res_of(n)));
+    float z[N], a[N];
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      // behind the row's end whatever the place holds: there both are zero
+      const float xv = to_float<T>(x[c]), dyv = to_float<T>(dy[c]);
+      z[j] = c < p.d ? (xv - mean) * rstd : 0.0f;
+      a[j] = c < p.d ? dyv : 0.0f;
+      dw[j] = fmaf(a[j], z[j], dw[j]);
+      if (kLayer) db[j] += a[j];
+      a[j] *= w[j];
+      s.x += a[j];
+      s.y = fmaf(a[j], z[j], s.y);
+    }
+    s = group_sums<kLayer>(s, slots + 32 * (n & 1), span);
+    // all have read the row before this one to its end: its place takes another
+    if (threadIdx.x == 0 && n + ahead < rows) ask(ring.before(), n + ahead);
+    const float c1 = kLayer ? s.x * inv_d : 0.0f, c2 = s.y * inv_d;
+    T* const dx = static_cast<T*>(p.dx) + (row + n * stride) * p.ld_dx;
+    T* const stage = kStaged<T> ? reinterpret_cast<T*>(staging + behind(dx)) : dx;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      if (!kStaged<T> && c >= p.d) continue;
+      const float add = residual ? to_float<T>(res[c]) : 0.0f;
+      stage[c] = from_float<T>(fmaf(fmaf(-z[j], c2, a[j] - c1), rstd, add));
+    }
+    if (kStaged<T>) store_staged(dx, staging, p.d, span);
+    ring.advance();
+  }
+  if (ring.wd.aborted() && threadIdx.x == 0) ring.drain(asked);
+  if (p.partial == nullptr) return;
+  const int columns = blockDim.x * N, group_floats = 2 * columns;
+  const int threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+  float* part = p.partial + 2ll * blockIdx.x * p.d;
+  if (blockDim.y == 1) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      if (c >= p.d) continue;
+      part[c] = dw[j];
+      if (kLayer) part[p.d + c] = db[kLayer ? j : 0];
+    }
+    return;
+  }
+  // [group][2][columns]: the groups' sums side by side, joined in the order of the groups
+  float* joined = reinterpret_cast<float*>(ring_memory);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = j * blockDim.x + threadIdx.x;
+    joined[threadIdx.y * group_floats + c] = dw[j];
+    if (kLayer) joined[threadIdx.y * group_floats + columns + c] = db[kLayer ? j : 0];
+  }
+  __syncthreads();
+  for (int i = thread; i < (kLayer ? 2 * columns : columns); i += threads) {
+    const int which = i >= columns, c = i - which * columns;
+    if (c >= p.d) continue;
+    float total = 0.0f;
+    for (int g = 0; g < static_cast<int>(blockDim.y); ++g) total += joined[g * group_floats + i];
+    part[which * p.d + c] = total;
   }
 }
 

@@ -64,32 +64,6 @@ int norm_splits(int64_t M) { return static_cast<int>(std::max<int64_t>(1, std::m
 
 constexpr size_t kRingBytes = 216 * 1024;  // of the 227 KB of a block
 
-// How a width is laid out over threads: groups of `group` threads hold a row, `groups` of them make a block.
-struct RowShape {
-  int vectors;  // of a thread; 0: the width is too large for registers
-  int group, groups;
-};
-
-// Shape for rows of `units` vectors, at most `most` vectors a thread (a power of two) and `threads` threads a block.
-RowShape row_shape(int64_t units, int64_t M, int most, int threads) {
-  RowShape r = {0, 0, 0};
-  int n = 1;
-  while (n < most && units > 32 * n) n *= 2;
-  const int64_t group = (units + 32 * n - 1) / (32 * n) * 32;
-  if (group > threads) return r;
-  r.vectors = n;
-  r.group = static_cast<int>(group);
-  r.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({threads / group, kNarrowGroups, M})));
-  return r;
-}
-
-template <typename T, bool kLayer, int N>
-int launch_norm_forward_narrow(const NormForwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
-  const int64_t resident = static_cast<int64_t>(sms) * std::max(1, 1536 / (r.group * r.groups));
-  return launch(norm_forward_narrow_kernel<T, kLayer, N>, std::min(blocks, resident), dim3(r.group, r.groups), 0, s, p);
-}
-
 // How the wide kernels lay a row out: each thread holds `columns` of it.
 struct WidePlan {
   int columns, group, groups, places;
@@ -112,6 +86,30 @@ WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_thre
     // two places keep one row of each group on its way: enough where that is 64 KB
     if (places < 2 || (places == 2 && most_places > 2 && groups > 1 && place < 64 * 1024)) continue;
     w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), places * place};
+    break;
+  }
+  return w;
+}
+
+// The same for rows that start anywhere: values of a thread, threads of a group, and the plan.
+int odd_values(int d) { return d <= 128 ? 4 : d <= 8 * kOddThreads ? 8 : 16; }
+int odd_group(int d) { return (d + 32 * odd_values(d) - 1) / (32 * odd_values(d)) * 32; }
+WidePlan odd_plan(int d, int64_t M, size_t size, int most_threads, int arrays, int most_places, int sms) {
+  WidePlan w = {0, 0, 0, 0, 0};
+  const int64_t group = odd_group(d);
+  if (group > kOddThreads) return w;
+  const int64_t spread = std::max<int64_t>(1, (M + sms - 1) / sms);
+  int64_t groups = std::min<int64_t>({most_threads / group, group > 32 ? kWideMultiGroups : kWideGroups, spread});
+  for (; groups >= 1; --groups) {
+    const size_t array = odd_array_bytes(static_cast<int>(group) * odd_values(d), static_cast<int>(size)), place = static_cast<size_t>(arrays * groups) * array;
+    const size_t staging = size == 2 ? static_cast<size_t>(groups) * array : 0;  // and a row of each group that is stored
+    const size_t places = std::min<size_t>(static_cast<size_t>(most_places), (kRingBytes - staging) / place);
+    if (places < 2 || (places == 2 && most_places > 2 && groups > 1 && place < 64 * 1024)) continue;
+    // the groups' sums over rows are joined in the ring's memory
+    const size_t joined = arrays == 3 && groups > 1 ? static_cast<size_t>(groups * group * odd_values(d)) * 2 * sizeof(float) : 0;
+    if (joined > kRingBytes) continue;
+    w = WidePlan{odd_values(d), static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places),
+                 std::max(places * place + staging, joined)};
     break;
   }
   return w;
@@ -170,6 +168,18 @@ int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Devi
   return launch_norm_forward_wide<T, W, kLayer, 32>(p, w, dev, s);
 }
 
+template <typename T, bool kLayer, int N>
+int launch_norm_forward_odd(NormForwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  constexpr auto kernel = norm_forward_odd_kernel<T, kLayer, N>;
+  static std::atomic<uint64_t> done{0}, known{0};
+  if (int rc = opt_in(kernel, &done, dev)) return rc;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
+  const int64_t resident = dev.sms * resident_blocks(kernel, &known, w.threads(), w.ring);
+  p.ring.places = w.places;
+  p.ring.withhold = take_withhold();
+  return launch(kernel, std::min(blocks, resident), dim3(w.group, w.groups), w.ring, s, p);
+}
+
 // Lanes that take a short row.
 int short_lanes(int d, int per_vector) { return d <= 8 * per_vector ? 8 : d <= 16 * per_vector ? 16 : 32; }
 
@@ -194,23 +204,27 @@ int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cuda
       return launch_norm_forward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
     }
   } else {
-    const RowShape r = row_shape(p.d, p.M, 16, 512);
-    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_forward_narrow<T, kLayer, 2>(p, r, dev.sms, s);
-    if (r.vectors > 2 && r.vectors <= 8) return launch_norm_forward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
-    if (r.vectors == 16) return launch_norm_forward_narrow<T, kLayer, 16>(p, r, dev.sms, s);
+    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), std::max(256, odd_group(p.d)), 1, kLayer ? 4 : 3, dev.sms);
+    if (w.columns > 0) {
+      if (w.columns == 4) return launch_norm_forward_odd<T, kLayer, 4>(p, w, dev, s);
+      if (w.columns == 8) return launch_norm_forward_odd<T, kLayer, 8>(p, w, dev, s);
+      return launch_norm_forward_odd<T, kLayer, 16>(p, w, dev, s);
+    }
   }
   return launch(norm_forward_any_kernel<T, kLayer>, std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8),
                 dim3(kNormThreads), 0, s, p);
 }
 
 template <typename T, bool kLayer, int N>
-int launch_norm_backward_narrow(NormBackwardParams& p, const RowShape& r, int sms, cudaStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(p.M) + r.groups - 1) / r.groups;
-  const int64_t resident = std::min<int64_t>(static_cast<int64_t>(sms) * std::max(1, 512 / (r.group * r.groups)), kMaxNormSplits);
-  const int grid = static_cast<int>(std::min(blocks, resident));
-  p.splits = grid;
-  const size_t shared = r.groups > 1 ? static_cast<size_t>(2) * r.group * N * sizeof(float) : 0;
-  return launch(norm_backward_narrow_kernel<T, kLayer, N>, grid, dim3(r.group, r.groups), shared, s, p);
+int launch_norm_backward_odd(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+  constexpr auto kernel = norm_backward_odd_kernel<T, kLayer, N>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = opt_in(kernel, &done, dev)) return rc;
+  const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
+  p.splits = static_cast<int>(std::min<int64_t>({blocks, dev.sms, kMaxNormSplits}));
+  p.ring.places = w.places;
+  p.ring.withhold = take_withhold();
+  return launch(kernel, p.splits, dim3(w.group, w.groups), w.ring, s, p);
 }
 
 template <typename T, typename W, bool kLayer, int kColumns>
@@ -268,9 +282,12 @@ int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cu
       return launch_norm_backward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
     }
   } else {
-    const RowShape r = row_shape(p.d, p.M, 8, 512);
-    if (r.vectors > 0 && r.vectors <= 2) return launch_norm_backward_narrow<T, kLayer, 2>(p, r, dev.sms, s);
-    if (r.vectors > 2) return launch_norm_backward_narrow<T, kLayer, 8>(p, r, dev.sms, s);
+    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), kOddThreads, 3, 4, dev.sms);
+    if (w.columns > 0) {
+      if (w.columns == 4) return launch_norm_backward_odd<T, kLayer, 4>(p, w, dev, s);
+      if (w.columns == 8) return launch_norm_backward_odd<T, kLayer, 8>(p, w, dev, s);
+      return launch_norm_backward_odd<T, kLayer, 16>(p, w, dev, s);
+    }
   }
   if (int rc = launch(norm_backward_any_kernel<T, kLayer>, std::min<int64_t>(p.M, static_cast<int64_t>(dev.sms) * 8),
                       dim3(kNormThreads), 0, s, p))
@@ -312,7 +329,7 @@ int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, con
   p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0};
   p.w_f32 = w_dtype == FSWIGLU_OUT_F32 && (weight != nullptr || bias != nullptr);
   p.eps = eps;
-  // fp32 vectors are read where they are: one without the other goes the narrow way
+  // fp32 vectors are read where they are: one without the other goes the odd way
   const bool wide = !(layer && p.w_f32 && (weight == nullptr || bias == nullptr)) &&
                     d * type_bytes(x_dtype) % 16 == 0 && wide_rows(x, ldx, M, x_dtype) && wide_rows(y, ldy, M, x_dtype) &&
                     aligned(weight, 16) && aligned(bias, 16);
@@ -609,6 +626,11 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
   if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg_sq, tensors[i].numel * static_cast<int64_t>(sb)); })))
     return rc;
   if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].master, tensors[i].numel * 4); }))) return rc;
+  if (state_bits == 8) {
+    auto scales = [&](int64_t i) { return (tensors[i].numel + kAdamBlock - 1) / kAdamBlock * 4; };
+    if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg_scale, scales(i)); }))) return rc;
+    if ((rc = disjoint(count, [&](int64_t i) { return range_of(tensors[i].exp_avg_sq_scale, scales(i)); }))) return rc;
+  }
   Device dev;
   if ((rc = current_device(&dev))) return rc;
   AdamOptions o = {};

@@ -173,6 +173,8 @@ class FusedAdamW(torch.optim.Optimizer):
     def _init_state(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if not state:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("take one step before the capture: a captured one would start from zero each time")
             state["step"] = 0
             if self.state_bits == 8:
                 scales = dict(dtype=torch.float32, device=p.device)

@@ -280,7 +280,7 @@ int fswiglu_rms_norm_backward(const void* dout, int64_t ld_dout, const void* x, 
  *       finite gets NaN for its scale.
  * The tensors are described in host memory, which the call has read when it returns (it may be freed then); the
  * launches carry the pointers, so that a captured graph needs nothing but the tensors themselves.  No two tensors
- * may share parameters, masters or moments (checked: FSWIGLU_ERR_BAD_ARG).
+ * may share parameters, masters, moments or scales (checked among each kind: FSWIGLU_ERR_BAD_ARG).
  * Options: lr_device (fp32) and step_device (int64, >= 1), where not NULL, are read on the device in the place of lr
  * and step, so that a captured graph can be replayed with other values.  grad_scale (fp32, NULL: 1) is read on the
  * device too; where it is not finite the step changes nothing.

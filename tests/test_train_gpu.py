@@ -212,6 +212,21 @@ def test_norm_outputs_stay_in_their_rows(fsw, lib, cuda_dev, M, d, pitch, offset
     assert all(bool((s[M:] == 77.0).all()) for s in stats) and all(bool((v[d:] == 77.0).all()) for v in vectors)
 
 
+def test_norm_offsets_past_32_bits(lib, cuda_dev):
+    """More than 2^31 elements: the last rows are what a call of those alone gives, and the others' zeros add nothing."""
+    M, d, n = 530_000, 4096, 40
+    x, w, b, dy, res = norm_inputs(n, d, BF, BF, cuda_dev, 8)
+    big, big_dy = (torch.zeros((M, d), dtype=BF, device=cuda_dev) for _ in range(2))
+    big[-n:], big_dy[-n:] = x, dy
+    y, mean, rstd = lib.layer_norm_forward(big, w, b, 1e-5)
+    check_forward(lib, x, w, b, 1e-5, True, out=(y[-n:], mean[-n:], rstd[-n:]))
+    assert torch.equal(y[:1000], b.expand(1000, d)) and torch.equal(y[-n - 1000:-n], b.expand(1000, d))
+    del y
+    dx, dw, db = lib.layer_norm_backward(big_dy, big, mean, rstd, w, True)
+    check_backward(lib, dy, x, mean[-n:], rstd[-n:], w, None, True, (dx[-n:], dw, db), BF)
+    assert not dx[:1000].any() and not dx[-n - 1000:-n].any()
+
+
 def test_norm_without_rows(lib, cuda_dev):
     x = torch.empty((0, 72), dtype=BF, device=cuda_dev)
     w = torch.ones(72, dtype=BF, device=cuda_dev)

@@ -113,6 +113,10 @@ def test_adamw_refuses_shared_memory_in_any_order(memory):
             assert adamw(m, tensors) == capi.ERR_BAD_ARG
     shared = [dict(t, master=m(7000)) for t in apart[:2]]
     assert adamw(m, shared) == capi.ERR_BAD_ARG
+    for key in ("exp_avg_scale", "exp_avg_sq_scale"):
+        scales = [dict(t, exp_avg_scale=m(7000 + 16 * i), exp_avg_sq_scale=m(7200 + 16 * i)) for i, t in enumerate(apart)]
+        scales[2][key] = scales[0][key]
+        assert adamw(m, scales, bits=8) == capi.ERR_BAD_ARG
 
 
 def test_grad_norm_refusals(memory):

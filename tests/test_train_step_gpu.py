@@ -224,6 +224,19 @@ def test_a_step_is_seen_by_autograd(fsw, cuda_dev):
         y.sum().backward()
 
 
+def test_a_first_step_is_not_captured(fsw, cuda_dev):
+    p = torch.nn.Parameter(torch.ones(64, device=cuda_dev))
+    p.grad = torch.ones_like(p)
+    opt = fsw.train.FusedAdamW([p], capturable=True)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="one step before"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    torch.cuda.synchronize()
+    opt.step()
+    assert bool((p < 1).all())
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_whole_training_step_from_a_captured_graph(fsw, cuda_dev, bits):
     """Two graphs of one step each, replayed in turn; both give what the eager step gives from the same state."""

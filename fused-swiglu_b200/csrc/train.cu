@@ -67,14 +67,15 @@ constexpr size_t kRingBytes = 216 * 1024;  // of the 227 KB of a block
 // How the wide kernels lay a row out: each thread holds `columns` of it.
 struct WidePlan {
   int columns, group, groups, places;
-  size_t ring;  // bytes of shared memory
+  size_t place, extra;  // bytes of shared memory: of the block's places of one row each, and beside the ring
+  size_t ring() const { return places * place + extra; }
   int threads() const { return group * groups; }
 };
 
 // The plan for rows of d values of `size` bytes, `arrays` of them on their way, in blocks of at most `most_threads`;
 // columns == 0 where a row does not fit.
 WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_threads, int arrays, int most_places, int sms) {
-  WidePlan w = {0, 0, 0, 0, 0};
+  WidePlan w = {};
   const int64_t group = (d + 32 * columns - 1) / (32 * columns) * 32;
   if (group > most_threads) return w;
   // no more groups than leave every SM a block
@@ -85,7 +86,7 @@ WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_thre
     const size_t places = std::min<size_t>(static_cast<size_t>(most_places), kRingBytes / place);
     // two places keep one row of each group on its way: enough where that is 64 KB
     if (places < 2 || (places == 2 && most_places > 2 && groups > 1 && place < 64 * 1024)) continue;
-    w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), places * place};
+    w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), place, 0};
     break;
   }
   return w;
@@ -95,7 +96,7 @@ WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_thre
 int odd_values(int d) { return d <= 128 ? 4 : d <= 8 * kOddThreads ? 8 : 16; }
 int odd_group(int d) { return (d + 32 * odd_values(d) - 1) / (32 * odd_values(d)) * 32; }
 WidePlan odd_plan(int d, int64_t M, size_t size, int most_threads, int arrays, int most_places, int sms) {
-  WidePlan w = {0, 0, 0, 0, 0};
+  WidePlan w = {};
   const int64_t group = odd_group(d);
   if (group > kOddThreads) return w;
   const int64_t spread = std::max<int64_t>(1, (M + sms - 1) / sms);
@@ -108,8 +109,8 @@ WidePlan odd_plan(int d, int64_t M, size_t size, int most_threads, int arrays, i
     // the groups' sums over rows are joined in the ring's memory
     const size_t joined = arrays == 3 && groups > 1 ? static_cast<size_t>(groups * group * odd_values(d)) * 2 * sizeof(float) : 0;
     if (joined > kRingBytes) continue;
-    w = WidePlan{odd_values(d), static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places),
-                 std::max(places * place + staging, joined)};
+    w = WidePlan{odd_values(d), static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), place,
+                 std::max(places * place + staging, joined) - places * place};
     break;
   }
   return w;
@@ -126,40 +127,52 @@ int opt_in(Kernel k, std::atomic<uint64_t>* done, const Device& dev) {
   return FSWIGLU_OK;
 }
 
-// Blocks of a kernel that an SM holds; the last answer is kept with what it was for.
+// Forward kernels have several blocks on an SM.  The places of their rings are the fewest that keep 56 KB of rows on their way
+// to it: fewer wait, and more are slower, since reads far ahead of the writes take the memory's pages from them (RMS norm of
+// 32414 x 5120 bf16: two places 138 us, three 106, four 123; of 16000 x 4096 fp32: 82, 94).  Sets the plan's places, and returns the
+// SM's blocks; the last answer is kept with what it was for.
 template <typename Kernel>
-int64_t resident_blocks(Kernel k, std::atomic<uint64_t>* known, int threads, size_t shared) {
-  const uint64_t key = static_cast<uint64_t>(threads) << 40 | static_cast<uint64_t>(shared) << 8;
+int64_t fill_sm(Kernel k, std::atomic<uint64_t>* known, WidePlan& w) {
+  constexpr size_t kOnItsWay = 56 * 1024;
+  const uint64_t key = static_cast<uint64_t>(w.threads()) << 48 | static_cast<uint64_t>(w.place + w.extra) << 16 |
+                       static_cast<uint64_t>(w.places) << 12;
   const uint64_t seen = known->load(std::memory_order_relaxed);
-  if ((seen & ~0xffull) == key && (seen & 0xffu) != 0) return static_cast<int64_t>(seen & 0xffu);
-  int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, threads, shared) != cudaSuccess || n < 1) n = 1;
-  known->store(key | static_cast<uint64_t>(n), std::memory_order_relaxed);
-  return n;
+  int blocks = 0;
+  if ((seen & ~0xfffull) == key && (seen & 0xffu) != 0) {
+    w.places = static_cast<int>(seen >> 8 & 0xfu);
+    return static_cast<int64_t>(seen & 0xffu);
+  }
+  const int most = w.places;
+  for (w.places = 2;; ++w.places) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k, w.threads(), w.ring()) != cudaSuccess || blocks < 1) blocks = 1;
+    if (w.places >= most || (w.places - 1) * w.place * blocks >= kOnItsWay) break;
+  }
+  known->store(key | static_cast<uint64_t>(w.places) << 8 | static_cast<uint64_t>(blocks), std::memory_order_relaxed);
+  return blocks;
 }
 
 // Wide kernels take weights of the rows' type or fp32 ones (bf16 rows), and stand-ins for missing ones in bf16.
 template <typename T, typename W, bool kLayer, int kColumns>
-int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+int launch_norm_forward_wide(NormForwardParams& p, WidePlan w, const Device& dev, cudaStream_t s) {
   constexpr auto kernel = norm_forward_wide_kernel<T, W, kLayer, kColumns / kPerVector<T>>;
   static std::atomic<uint64_t> done{0}, known{0};
   if (int rc = opt_in(kernel, &done, dev)) return rc;
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
-  const int64_t resident = dev.sms * resident_blocks(kernel, &known, w.threads(), w.ring);
+  const int64_t resident = dev.sms * fill_sm(kernel, &known, w);
   const int grid = static_cast<int>(std::min(blocks, resident));
   p.y_step = static_cast<long long>(grid) * w.groups * p.ldy * static_cast<long long>(sizeof(T));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, grid, dim3(w.group, w.groups), w.ring, s, p);
+  return launch(kernel, grid, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 // Forward: 32 columns a thread, since a row's reductions cost every warp the same; 16 where a warp holds a whole row with
 // them, where fp32 weights are kept in registers, and for fp32 rows, whose places would take twice the shared memory.
-WidePlan forward_plan(const NormForwardParams& p, bool layer, size_t size, int sms) {
+WidePlan forward_plan(const NormForwardParams& p, size_t size, int sms) {
   const bool few = p.d <= 512 || ((p.w_f32 || size == 4) && p.d <= 16 * wide_forward_threads(16));
   const int columns = few ? 16 : 32, group = (p.d + 32 * columns - 1) / (32 * columns) * 32;
-  if (group > wide_forward_threads(columns)) return WidePlan{0, 0, 0, 0, 0};
-  return wide_plan(p.d, p.M, size, columns, std::max(256, group), 1, layer ? 4 : 3, sms);
+  if (group > wide_forward_threads(columns)) return WidePlan{};
+  return wide_plan(p.d, p.M, size, columns, std::max(256, group), 1, kWidePlaces, sms);
 }
 
 template <typename T, typename W, bool kLayer>
@@ -169,15 +182,15 @@ int launch_norm_forward_wide(NormForwardParams& p, const WidePlan& w, const Devi
 }
 
 template <typename T, bool kLayer, int N>
-int launch_norm_forward_odd(NormForwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
+int launch_norm_forward_odd(NormForwardParams& p, WidePlan w, const Device& dev, cudaStream_t s) {
   constexpr auto kernel = norm_forward_odd_kernel<T, kLayer, N>;
   static std::atomic<uint64_t> done{0}, known{0};
   if (int rc = opt_in(kernel, &done, dev)) return rc;
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
-  const int64_t resident = dev.sms * resident_blocks(kernel, &known, w.threads(), w.ring);
+  const int64_t resident = dev.sms * fill_sm(kernel, &known, w);
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, std::min(blocks, resident), dim3(w.group, w.groups), w.ring, s, p);
+  return launch(kernel, std::min(blocks, resident), dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 // Lanes that take a short row.
@@ -198,13 +211,13 @@ int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cuda
       if (p.w_f32) return launch_norm_forward_short<T, float, kLayer>(p, dev, s);
       return launch_norm_forward_short<T, __nv_bfloat16, kLayer>(p, dev, s);
     }
-    const WidePlan w = forward_plan(p, kLayer, sizeof(T), dev.sms);
+    const WidePlan w = forward_plan(p, sizeof(T), dev.sms);
     if (w.columns > 0) {
       if (p.w_f32) return launch_norm_forward_wide<T, float, kLayer>(p, w, dev, s);
       return launch_norm_forward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
     }
   } else {
-    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), std::max(256, odd_group(p.d)), 1, kLayer ? 4 : 3, dev.sms);
+    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), std::max(256, odd_group(p.d)), 1, kWidePlaces, dev.sms);
     if (w.columns > 0) {
       if (w.columns == 4) return launch_norm_forward_odd<T, kLayer, 4>(p, w, dev, s);
       if (w.columns == 8) return launch_norm_forward_odd<T, kLayer, 8>(p, w, dev, s);
@@ -224,7 +237,7 @@ int launch_norm_backward_odd(NormBackwardParams& p, const WidePlan& w, const Dev
   p.splits = static_cast<int>(std::min<int64_t>({blocks, dev.sms, kMaxNormSplits}));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, p.splits, dim3(w.group, w.groups), w.ring, s, p);
+  return launch(kernel, p.splits, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 template <typename T, typename W, bool kLayer, int kColumns>
@@ -238,15 +251,15 @@ int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const De
   p.dx_step = static_cast<long long>(grid) * w.groups * p.ld_dx * static_cast<long long>(sizeof(T));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, grid, dim3(w.group, w.groups), w.ring, s, p);
+  return launch(kernel, grid, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 // Backward: one block an SM, its registers full of the sums over rows.  Of the columns a thread may hold, those that keep most
 // warps busy.
 WidePlan backward_plan(const NormBackwardParams& p, size_t size, int sms) {
-  WidePlan best = {0, 0, 0, 0, 0};
+  WidePlan best = {};
   for (int columns = 16; columns <= 32; columns += 8) {
-    const WidePlan w = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns), 3, 4, sms);
+    const WidePlan w = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns), 3, kWidePlaces, sms);
     if (w.threads() > best.threads()) best = w;
   }
   return best;
@@ -282,7 +295,7 @@ int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cu
       return launch_norm_backward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
     }
   } else {
-    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), kOddThreads, 3, 4, dev.sms);
+    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), kOddThreads, 3, kWidePlaces, dev.sms);
     if (w.columns > 0) {
       if (w.columns == 4) return launch_norm_backward_odd<T, kLayer, 4>(p, w, dev, s);
       if (w.columns == 8) return launch_norm_backward_odd<T, kLayer, 8>(p, w, dev, s);

@@ -298,7 +298,8 @@ __device__ __forceinline__ float adam_inverse_root(float root) {
 }
 
 // fp32 moments.  P, G: types of parameters and gradients.  A thread has eight neighbours at a time; three blocks an SM
-// keep enough on its way, and more of them are slower (3 x 45 M weights: three 595 us, four 599, five 645).
+// keep enough on its way, and more of them are slower (3 x 45 M weights: three 595 us, four 599, five 645).  Bound by memory: bf16 weights and gradients with
+// fp32 copies, 28 bytes an element, 3 x 45 M weights in 559 us, 6.8 TB/s; 224 tensors of 65 k in 64 us, 6.4 TB/s.
 template <typename P, typename G, bool kMaster, int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads, 3) adamw32_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
   using Weight = typename std::conditional<kMaster, float, P>::type;
@@ -343,6 +344,9 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw32_kernel(const __grid_c
 // There is nearly as much to compute as to move, and a warp that waits for its loads does not compute: a part's values come
 // by bulk copies into a ring of shared memory, asked for by a warp of their own while the eight others work on earlier
 // parts.  A part at a tensor's end, or of a tensor whose pointers are not aligned, is loaded by its threads.
+// 3 x 45 M bf16 weights with fp32 copies, 16 bytes an element: 351 us, 6.2 TB/s, 59 instructions an element on 68 % of the issue
+// slots; with each warp loading its own values 467 us.  Places and blocks an SM: three of two 356 us, two of three 360, four of
+// two 368, three of three 386.
 
 constexpr int kAdam8Places = 3;
 constexpr int kAdam8RingThreads = kAdamThreads + 32;
@@ -605,7 +609,8 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 }
 
 // Squares of this thread's elements of kParts parts of a chunk from part `first` on, all loaded before the first is used: in
-// fp32 over two parts, sixteen elements, in fp64 from there on.
+// fp32 over two parts, sixteen elements, in fp64 from there on.  (3 x 45 M fp32 gradients 82 us, 6.6 TB/s, bound by memory; 224 of
+// 65 k bf16, from the L2 cache, 10.6 us, most of it the two launches' and each block's search for its tensors.)
 template <int kParts, typename T>
 __device__ __forceinline__ double sum_squares(const T* p, bool vector, int size, int first) {
   RawGroup<T> raw[kParts];

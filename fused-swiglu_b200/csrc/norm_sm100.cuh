@@ -425,7 +425,7 @@ struct Columns<float, N, P, false> {
 // Most threads of a block by the columns that a thread holds: what registers allow.  A scheduler holds a quarter of the
 // warps, so that 12 of them have 168 registers each, and 16 have 128.
 constexpr int wide_forward_threads(int) { return 512; }
-constexpr int wide_backward_threads(int columns) { return columns <= 24 ? 512 : 384; }
+constexpr int wide_backward_threads(int columns, bool again) { return columns <= 16 && again ? 640 : columns <= 24 ? 512 : 384; }
 
 // T: type of the rows, W: type of weight and bias.  Places of the ring behind a row's end stay zero.
 // Bound by memory: RMS norm of 32414 x 5120 bf16 103 us, 6.4 TB/s; layer norm 114 us, 5.8 TB/s, its two reductions a row one after
@@ -527,13 +527,12 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
 // dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
 // block are joined in the ring's memory at the end, and the blocks by norm_reduce_kernel.
 // Bound by memory: RMS norm with a residual, 32414 x 5120 bf16, 200 to 217 us, 6.1 to 6.6 TB/s; layer norm, whose second sum takes as many
-// registers again, 16384 x 4096 86 us, 6.3 TB/s, and 32414 x 5120 248 us, 5.4 TB/s (a thread's 24 columns there are computed twice).
-template <typename T, typename W, bool kLayer, int N>
-__global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>)) norm_backward_wide_kernel(const NormBackwardParams p) {
+// registers again, 16384 x 4096 86 us, 6.3 TB/s, and 32414 x 5120 207 us, 6.4 TB/s.  kAgain: a row's z and a are not kept over its reduction but computed
+// again from shared memory, which frees their registers.
+template <typename T, typename W, bool kLayer, int N, bool kAgain>
+__global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgain)) norm_backward_wide_kernel(const NormBackwardParams p) {
   constexpr int P = kPerVector<T>;
   constexpr long long kSize = sizeof(T);
-  // many columns' two sums leave no room for a row's z and a: they are computed again from shared memory
-  constexpr bool kAgain = kLayer && N * P > 16;
   __shared__ WideShared shared;
   extern __shared__ __align__(128) unsigned char ring_memory[];  // [groups][places][x, dy, res][N * blockDim.x][16 bytes]
   const int stride = gridDim.x * blockDim.y, row = blockIdx.x * blockDim.y + threadIdx.y;

@@ -67,6 +67,7 @@ constexpr size_t kRingBytes = 216 * 1024;  // of the 227 KB of a block
 // How the wide kernels lay a row out: each thread holds `columns` of it.
 struct WidePlan {
   int columns, group, groups, places;
+  bool again;           // backward: a row's values are computed a second time where they are used
   size_t place, extra;  // bytes of shared memory: of the block's places of one row each, and beside the ring
   size_t ring() const { return places * place + extra; }
   int threads() const { return group * groups; }
@@ -86,7 +87,7 @@ WidePlan wide_plan(int64_t d, int64_t M, size_t size, int columns, int most_thre
     const size_t places = std::min<size_t>(static_cast<size_t>(most_places), kRingBytes / place);
     // two places keep one row of each group on its way: enough where that is 64 KB
     if (places < 2 || (places == 2 && most_places > 2 && groups > 1 && place < 64 * 1024)) continue;
-    w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), place, 0};
+    w = WidePlan{columns, static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), false, place, 0};
     break;
   }
   return w;
@@ -109,7 +110,7 @@ WidePlan odd_plan(int d, int64_t M, size_t size, int most_threads, int arrays, i
     // the groups' sums over rows are joined in the ring's memory
     const size_t joined = arrays == 3 && groups > 1 ? static_cast<size_t>(groups * group * odd_values(d)) * 2 * sizeof(float) : 0;
     if (joined > kRingBytes) continue;
-    w = WidePlan{odd_values(d), static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), place,
+    w = WidePlan{odd_values(d), static_cast<int>(group), static_cast<int>(groups), static_cast<int>(places), false, place,
                  std::max(places * place + staging, joined) - places * place};
     break;
   }
@@ -240,9 +241,9 @@ int launch_norm_backward_odd(NormBackwardParams& p, const WidePlan& w, const Dev
   return launch(kernel, p.splits, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
-template <typename T, typename W, bool kLayer, int kColumns>
+template <typename T, typename W, bool kLayer, int kColumns, bool kAgain>
 int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
-  constexpr auto kernel = norm_backward_wide_kernel<T, W, kLayer, kColumns / kPerVector<T>>;
+  constexpr auto kernel = norm_backward_wide_kernel<T, W, kLayer, kColumns / kPerVector<T>, kAgain>;
   static std::atomic<uint64_t> done{0};
   if (int rc = opt_in(kernel, &done, dev)) return rc;
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
@@ -255,11 +256,20 @@ int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const De
 }
 
 // Backward: one block an SM, its registers full of the sums over rows.  Of the columns a thread may hold, those that keep most
-// warps busy.
-WidePlan backward_plan(const NormBackwardParams& p, size_t size, int sms) {
+// warps busy.  Layer norm's threads of more than 16 columns compute a row's values twice, for want of registers; those of 16
+// do where that makes room for a second group (32414 x 5120 bf16: two groups 207 us; 24 columns a thread 237).
+WidePlan backward_plan(const NormBackwardParams& p, bool layer, size_t size, int sms) {
   WidePlan best = {};
   for (int columns = 16; columns <= 32; columns += 8) {
-    const WidePlan w = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns), 3, kWidePlaces, sms);
+    const bool again = layer && columns > 16;
+    WidePlan w = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns, again), 3, kWidePlaces, sms);
+    if (layer && columns == 16 && w.groups == 1) {
+      const WidePlan two = wide_plan(p.d, p.M, size, columns, wide_backward_threads(columns, true), 3, kWidePlaces, sms);
+      if (two.groups == 2) {
+        w = two;
+        w.again = true;
+      }
+    }
     if (w.threads() > best.threads()) best = w;
   }
   return best;
@@ -268,9 +278,13 @@ WidePlan backward_plan(const NormBackwardParams& p, size_t size, int sms) {
 template <typename T, typename W, bool kLayer>
 int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
   switch (w.columns) {
-    case 16: return launch_norm_backward_wide<T, W, kLayer, 16>(p, w, dev, s);
-    case 24: return launch_norm_backward_wide<T, W, kLayer, 24>(p, w, dev, s);
-    default: return launch_norm_backward_wide<T, W, kLayer, 32>(p, w, dev, s);
+    case 16:
+      if constexpr (kLayer) {
+        if (w.again) return launch_norm_backward_wide<T, W, kLayer, 16, true>(p, w, dev, s);
+      }
+      return launch_norm_backward_wide<T, W, kLayer, 16, false>(p, w, dev, s);
+    case 24: return launch_norm_backward_wide<T, W, kLayer, 24, kLayer>(p, w, dev, s);
+    default: return launch_norm_backward_wide<T, W, kLayer, 32, kLayer>(p, w, dev, s);
   }
 }
 
@@ -289,7 +303,7 @@ int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cu
       if (p.w_f32) return launch_norm_backward_short<T, float, kLayer>(p, dev, s);
       return launch_norm_backward_short<T, __nv_bfloat16, kLayer>(p, dev, s);
     }
-    const WidePlan w = backward_plan(p, sizeof(T), dev.sms);
+    const WidePlan w = backward_plan(p, kLayer, sizeof(T), dev.sms);
     if (w.columns > 0) {
       if (p.w_f32) return launch_norm_backward_wide<T, float, kLayer>(p, w, dev, s);
       return launch_norm_backward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);

@@ -196,11 +196,22 @@ int prepare_device(int dev, int* num_sms) {
   return e == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
 }
 
+// A thread whose first CUDA call this is (autograd's, say) has no context yet, without which tensor maps cannot be encoded:
+// launches and copies would bind one, the driver's entry points do not.
+int bind_context(int dev) {
+  thread_local int bound = -1;
+  if (bound == dev) return FSWIGLU_OK;
+  if (cudaSetDevice(dev) != cudaSuccess) return FSWIGLU_ERR_NO_DEVICE;
+  bound = dev;
+  return FSWIGLU_OK;
+}
+
 // One-time per-device set-up of the ordinary entry points: the above plus the 256-byte status block.
 int device_state(DeviceState** out) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return FSWIGLU_ERR_NO_DEVICE;
   if (dev < 0 || dev >= kMaxDevices) return FSWIGLU_ERR_NO_DEVICE;
+  if (int rc = bind_context(dev)) return rc;
   std::lock_guard<std::mutex> lock(g_mutex);
   DeviceState& st = g_dev[dev];
   if (!st.ready) {
@@ -1082,6 +1093,7 @@ int static_state(StaticState** out) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return FSWIGLU_ERR_NO_DEVICE;
   if (dev < 0 || dev >= kMaxDevices) return FSWIGLU_ERR_NO_DEVICE;
+  if (int rc = bind_context(dev)) return rc;
   std::lock_guard<std::mutex> lock(g_mutex);
   StaticState& st = g_static[dev];
   if (!st.ready) {

@@ -30,6 +30,7 @@ __device__ __forceinline__ void store_shared(uint32_t at, float v) {
 __device__ __forceinline__ void store_shared(uint32_t at, __nv_bfloat16 v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__bfloat16_as_ushort(v)) : "memory");
 }
+
 // Of the kernels that wait for rows on their way (below).
 struct RingParams {
   uint32_t* status;  // where a wait that gave up is recorded

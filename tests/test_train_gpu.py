@@ -336,6 +336,28 @@ def test_norm_refusals(lib, cuda_dev):
         lib.layer_norm_backward(dy, x, mean, rstd.to(BF), w)
 
 
+def test_dispatcher_ops_are_the_module_functions(lib, cuda_dev):
+    o = torch.ops.ASMLLM
+    x, w, b, dy, res = norm_inputs(20, 96, BF, F32, cuda_dev, 1)
+    y, mean, rstd = lib.layer_norm_forward(x, w, b)
+    for p, q in zip(o.layer_norm_forward(x, w, b), (y, mean, rstd)):
+        assert torch.equal(p, q)
+    for p, q in zip(o.layer_norm_backward(dy, x, mean, rstd, w, True, res), lib.layer_norm_backward(dy, x, mean, rstd, w, True, res)):
+        assert torch.equal(p, q)
+    only = o.layer_norm_backward(dy, x, mean, rstd, w)
+    assert only[2] is None and torch.equal(only[0], lib.layer_norm_backward(dy, x, mean, rstd, w)[0])
+    assert torch.equal(o.rms_norm_forward(x, w)[0], lib.rms_norm_forward(x, w)[0])
+    assert torch.equal(o.rms_norm_backward(dy, x, rstd, w)[1], lib.rms_norm_backward(dy, x, rstd, w)[1])
+    assert torch.equal(o.grad_norm_clip([x, w], 1.0), lib.grad_norm_clip((x, w), 1.0))
+    both = [adam_inputs([700, 9], BF, BF, 8, True, cuda_dev, 2)[0] for _ in range(2)]
+    of = lambda ts, key: [t[key] for t in ts]  # noqa: E731
+    for ts, call in zip(both, (lib.adamw_step, o.adamw_step)):
+        call(of(ts, "p"), of(ts, "g"), of(ts, "m"), of(ts, "v"), 3, 1e-2, 0.9, 0.999, 1e-8, 0.0, of(ts, "w"), of(ts, "ms"),
+             of(ts, "vs"), None, 5)
+    for p, q in zip(*both):
+        assert all(torch.equal(p[k].view(torch.uint8), q[k].view(torch.uint8)) for k in p)
+
+
 # ---------------------------------------------------------------- AdamW
 
 def random_moments(n, spread, bits, g):

@@ -396,3 +396,36 @@ def test_launches_that_overlap_wait_for_what_was_written_before(fsw, cuda_dev):
     for out, ref in zip(outs, want):
         for a, b in zip(out, ref):
             assert torch.equal(a, b)
+
+
+def test_first_calls_of_a_new_thread(fsw, cuda_dev):
+    """A backward pass runs on a thread of autograd's, whose first CUDA call may be any of the library's."""
+    import threading
+
+    import fused_mlp_module as lib
+
+    x, w, b, wg, wu, wd = block_inputs(300, 520, 1096, cuda_dev, 0, "layer")
+    calls = {
+        "mlp": lambda: fsw.ops.fused_swiglu_mlp_bf16(x, wg, wu, wd),
+        "mlp_backward": lambda: fsw.ops.swiglu_mlp_backward(x, wg, wu, wd, x)[0],
+        "norm": lambda: lib.layer_norm_forward(x, w, b)[0],
+        "norm_backward": lambda: lib.rms_norm_backward(x, x, lib.rms_norm_forward(x, w)[1], w)[1],
+        "clip": lambda: lib.grad_norm_clip([x, w], 1.0),
+    }
+    for name, call in calls.items():
+        want = [call() for _ in range(2)][0]  # and the allocator has what it takes
+        torch.cuda.synchronize()
+        got = []
+
+        def work():
+            try:
+                got.append(call())
+            except Exception as e:  # noqa: BLE001
+                got.append(e)
+
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert isinstance(got[0], torch.Tensor), (name, got[0])
+        assert torch.equal(got[0], want), name

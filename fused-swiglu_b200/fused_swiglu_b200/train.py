@@ -32,6 +32,12 @@ def _rows(x: torch.Tensor, d: int) -> torch.Tensor:
     return x2 if plain else x2.contiguous()
 
 
+def _operand(x: torch.Tensor, d: int) -> torch.Tensor:
+    """Rows as the MLP's kernels read them: contiguous, from a 16-byte boundary on."""
+    x2 = x.reshape(-1, d).contiguous()
+    return x2 if x2.data_ptr() % 16 == 0 else x2.clone()
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -86,8 +92,7 @@ class _NormSwiGLUBlock(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, norm_weight, norm_bias, W_gate, W_up, W_down, eps, layer):
-        d = x.size(-1)
-        x2 = _rows(x, d)
+        x2 = _operand(x, x.size(-1))
         mean = None
         if layer:
             n, mean, rstd = _lib().layer_norm_forward(x2, norm_weight, norm_bias, eps)
@@ -101,7 +106,7 @@ class _NormSwiGLUBlock(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         x2, n, mean, rstd, norm_weight, W_gate, W_up, W_down = ctx.saved_tensors
-        d2 = _rows(dout, x2.size(1)).contiguous()
+        d2 = _operand(dout, x2.size(1))
         dn, dwg, dwu, dwd = ops.swiglu_mlp_backward(n, W_gate, W_up, W_down, d2)
         need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         # the residual's gradient joins where dx is written

@@ -115,6 +115,36 @@ def test_block_and_its_gradients(fsw, cuda_dev, M, d, F, norm):
             assert t.grad.dtype == BF and rel(t.grad, t64.grad) <= 1e-2
 
 
+def test_block_of_views_broadcasts_and_nothing(fsw, cuda_dev):
+    """Inputs that start off a boundary or have gaps, a gradient that is one value for all, frozen weights, no rows."""
+    x, w, _, wg, wu, wd = block_inputs(40, 64, 128, cuda_dev, 2, "rms")
+    want = fsw.train.norm_swiglu_block(x, w, None, wg, wu, wd)
+    flat = torch.zeros(40 * 64 + 8, dtype=BF, device=cuda_dev)
+    off = flat[1:1 + 40 * 64].view(40, 64)
+    off.copy_(x)
+    wide = torch.zeros((40, 73), dtype=BF, device=cuda_dev)
+    wide[:, 5:69] = x
+    for view in (off, wide[:, 5:69], x.t().contiguous().t(), x.view(4, 10, 64).transpose(0, 1).transpose(0, 1)):
+        leaf = view.detach().requires_grad_()
+        out = fsw.train.norm_swiglu_block(leaf, w, None, wg, wu, wd)
+        assert torch.equal(out.reshape(40, 64), want)
+        out.sum().backward()  # an expanded gradient
+        assert leaf.grad.shape == leaf.shape and bool(torch.isfinite(leaf.grad).all()) and w.grad is None
+    empty = torch.empty((0, 3, 64), dtype=BF, device=cuda_dev, requires_grad=True)
+    weights = [t.clone().requires_grad_() for t in (w, wg, wu, wd)]
+    out = fsw.train.norm_swiglu_block(empty, weights[0], None, *weights[1:])
+    out.sum().backward()
+    assert out.shape == (0, 3, 64) and empty.grad.shape == empty.shape and not any(t.grad.any() for t in weights)
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        fsw.train.norm_swiglu_block(x.float(), w, None, wg, wu, wd)
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        fsw.train.norm_swiglu_block(x, w.float(), None, wg, wu, wd)
+    with pytest.raises(ValueError):
+        fsw.train.norm_swiglu_block(x, w, w, wg, wu, wd)
+    with pytest.raises(ValueError):
+        fsw.train.norm_swiglu_block(x, w, None, wg, wu, wd, norm="batch")
+
+
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_block_module_agrees_with_the_inference_block(fsw, cuda_dev, norm):
     from fused_swiglu_b200.module import FusedNormSwiGLUBlock, NormSwiGLUBlock

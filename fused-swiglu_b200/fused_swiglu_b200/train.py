@@ -145,6 +145,10 @@ def moments_to_float(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return codes.reshape(-1).float().mul_(scales.repeat_interleave(256)[:codes.numel()]).view(codes.shape)
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) in one launch for all tensors of a kind.
 
@@ -177,9 +181,10 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _init_state(self, p: torch.Tensor) -> dict:
         state = self.state[p]
+        master = self.master and p.dtype == torch.bfloat16
+        if not state or (master and "master" not in state):
+            self._refuse_capture(p.device)
         if not state:
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("take one step before the capture: a captured one would start from zero each time")
             state["step"] = 0
             if self.state_bits == 8:
                 scales = dict(dtype=torch.float32, device=p.device)
@@ -190,9 +195,14 @@ class FusedAdamW(torch.optim.Optimizer):
             else:
                 state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            if self.master and p.dtype == torch.bfloat16:
-                state["master"] = p.detach().float()
+        if master and "master" not in state:
+            state["master"] = p.detach().float()
         return state
+
+    @staticmethod
+    def _refuse_capture(device: torch.device) -> None:
+        if _capturing(device):
+            raise RuntimeError("take one step before the capture: a captured one would start from zero each time")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -228,10 +238,11 @@ class FusedAdamW(torch.optim.Optimizer):
             lr_tensor = step_tensor = None
             if self.capturable:
                 if "step_tensor" not in group:
+                    self._refuse_capture(device)
                     group["lr_tensor"] = torch.full((1,), float(group["lr"]), dtype=torch.float32, device=device)
                     group["step_tensor"] = torch.full((1,), taken, dtype=torch.int64, device=device)
                 lr_tensor, step_tensor = group["lr_tensor"], group["step_tensor"]
-                if not torch.cuda.is_current_stream_capturing():
+                if not _capturing(device):
                     lr_tensor.fill_(float(group["lr"]))
                 if index not in stepped:
                     step_tensor.add_(1)
@@ -251,11 +262,22 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As the base class's, which would cast every state tensor to its parameter's type: moments, scales and masters
-        keep theirs."""
+        keep theirs.  The step count goes over from and to `capturable`; a captured step has to be captured again, after
+        one eager step.  Moments of the other `state_bits` are refused; a missing master is made from its parameter by the
+        next step."""
+        moments = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
+        if any(state["exp_avg"].dtype != moments for state in state_dict["state"].values() if "exp_avg" in state):
+            raise ValueError(f"the saved moments are not those of state_bits={self.state_bits}")
         super().load_state_dict(state_dict)
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(saved, params):
-            for key, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor):
-                    self.state[p][key] = value.detach().to(device=p.device, copy=True)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            steps = group.pop("step_tensor", None)
+            group.pop("lr_tensor", None)
+            for i, p in zip(saved["params"], group["params"]):
+                for key, value in state_dict["state"].get(i, {}).items():
+                    if isinstance(value, torch.Tensor):
+                        self.state[p][key] = value.detach().to(device=p.device, copy=True)
+                if self.state.get(p):
+                    if steps is not None:
+                        self.state[p]["step"] = int(steps)
+                    if not self.master:
+                        self.state[p].pop("master", None)

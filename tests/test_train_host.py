@@ -232,6 +232,44 @@ def test_optimizer_keeps_the_types_of_its_state_over_a_checkpoint(recorder):
         assert opt.state[ps[0]]["exp_avg"].dtype == (torch.float8_e4m3fn if bits == 8 else torch.float32)
 
 
+def test_optimizer_takes_its_step_count_over_a_checkpoint_either_way(recorder):
+    ps = some_params()
+    opt = train.FusedAdamW(ps, capturable=True)
+    for _ in range(3):
+        opt.step()
+    for capturable in (False, True):
+        other = train.FusedAdamW(some_params(), capturable=capturable)
+        other.load_state_dict(opt.state_dict())
+        recorder.steps.clear()
+        other.step()
+        assert len(recorder.steps) == 2
+        assert all((s["step_t"] if capturable else s["step"]) == 4 for s in recorder.steps)
+        assert ("step_tensor" in other.param_groups[0]) == capturable == ("lr_tensor" in other.param_groups[0])
+    plain = train.FusedAdamW(some_params())
+    plain.step()
+    other = train.FusedAdamW(some_params(), capturable=True)
+    other.load_state_dict(plain.state_dict())
+    recorder.steps.clear()
+    other.step()
+    assert [s["step_t"] for s in recorder.steps] == [2, 2]
+
+
+def test_optimizer_checkpoint_of_other_kinds(recorder):
+    for saved_bits, bits in ((8, 32), (32, 8)):
+        opt = train.FusedAdamW(some_params(), state_bits=saved_bits)
+        opt.step()
+        with pytest.raises(ValueError, match="state_bits"):
+            train.FusedAdamW(some_params(), state_bits=bits).load_state_dict(opt.state_dict())
+    for saved_master, master in ((False, True), (True, False)):
+        opt = train.FusedAdamW(some_params(), master=saved_master)
+        opt.step()
+        other = train.FusedAdamW(some_params(), master=master)
+        other.load_state_dict(opt.state_dict())
+        recorder.steps.clear()
+        other.step()
+        assert [len(s["masters"]) for s in recorder.steps] == [2 if master else 0, 0]
+
+
 def test_optimizer_refusals(recorder):
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(state_bits=16),
                 dict(max_grad_norm=-1.0), dict(lr=NAN)):

@@ -121,8 +121,8 @@ __device__ __forceinline__ float2 block_sum2(float2 v, float2* shared) {
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_forward_any_kernel(const NormForwardParams p) {
   __shared__ float2 shared[kNormThreads / 32];
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   for (int row = blockIdx.x; row < p.M; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     T* y = static_cast<T*>(p.y) + row * p.ldy;
@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_any_kernel(const No
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_backward_any_kernel(const NormBackwardParams p) {
   __shared__ float2 shared[kNormThreads / 32];
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   for (int row = blockIdx.x; row < p.M; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* dy = static_cast<const T*>(p.dout) + row * p.ld_dout;
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_any_kernel(const N
 template <typename T, bool kLayer>
 __global__ void __launch_bounds__(kNormThreads) norm_backward_columns_any_kernel(const NormBackwardParams p) {
   const long long tiles = (p.d + kNormThreads - 1) / kNormThreads;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   for (long long t = blockIdx.x; t < tiles * p.splits; t += gridDim.x) {
     const int split = static_cast<int>(t / tiles);
     const int i = static_cast<int>(t % tiles) * kNormThreads + threadIdx.x;
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
   }
   fence_mbar_init();
   __syncthreads();
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const void* const src[1] = {static_cast<const T*>(p.x) + (row + n * stride) * p.ldx};
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgai
   }
   fence_mbar_init();
   __syncthreads();
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const long long r = row + n * stride;
@@ -738,8 +738,8 @@ __global__ void __launch_bounds__(kOddThreads, 2) norm_forward_odd_kernel(const 
   RowRing<1> ring(shared, ring_memory, array, p.d * static_cast<uint32_t>(sizeof(T)), p.ring);
   fence_mbar_init();
   __syncthreads();
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   auto source = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
@@ -819,8 +819,8 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
   RowRing<3> ring(shared, ring_memory, array, p.d * static_cast<uint32_t>(sizeof(T)), p.ring);
   fence_mbar_init();
   __syncthreads();
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   auto x_of = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   auto dy_of = [&](int n) { return static_cast<const T*>(p.dout) + (row + n * stride) * p.ld_dout; };
   auto res_of = [&](int n) { return static_cast<const T*>(p.residual) + (residual ? (row + n * stride) * p.ld_res : 0); };
@@ -954,8 +954,8 @@ __global__ void __launch_bounds__(kShortThreads) norm_forward_short_kernel(const
   constexpr int P = kPerVector<T>, R = 4;
   const int c = threadIdx.x * P;
   const bool valid = c < p.d;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   Columns<W, 1, P> weight, bias;
   weight.init(p.weight, 0x3f803f80u, p.d);
   if (kLayer) bias.init(p.bias, 0u, p.d);
@@ -1015,8 +1015,8 @@ __global__ void __launch_bounds__(kShortThreads) norm_backward_short_kernel(cons
   __shared__ float joined[2][kShortThreads * P];  // [parts][columns]
   const int c = threadIdx.x * P;
   const bool valid = c < p.d, residual = p.residual != nullptr;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   Columns<W, 1, P> weight;
   weight.init(p.weight, 0x3f803f80u, p.d);
   Pair dw[P / 2], db[P / 2];
@@ -1098,8 +1098,8 @@ __global__ void __launch_bounds__(32 * kNormReduceRows) norm_reduce_kernel(const
   __shared__ float shared[kBias ? 2 : 1][kNormReduceRows][33];
   const int i = blockIdx.x * 32 + threadIdx.x;
   float dw = 0.0f, db = 0.0f;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   if (i < p.d) {
     for (int s = threadIdx.y; s < p.splits; s += kNormReduceRows) {
       dw += p.partial[2ll * s * p.d + i];

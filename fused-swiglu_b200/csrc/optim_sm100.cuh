@@ -304,8 +304,8 @@ template <typename P, typename G, bool kMaster, int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads, 3) adamw32_kernel(const __grid_constant__ AdamTable<kCapacity> t) {
   using Weight = typename std::conditional<kMaster, float, P>::type;
   const AdamOptions& o = t.opt;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   const AdamRates r = adam_rates(o);
   const uint32_t chunks = t.first_chunk[t.count];
   const int chunk_size = t.parts * kAdamPart;
@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(kRing ? kAdam8RingThreads : kAdamThreads, kRin
     }
     __syncthreads();
   }
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   const AdamRates r = adam_rates(o);
   if (kRing && r.skip) return;
   if (kRing && threadIdx.x >= kAdamThreads) {
@@ -643,8 +643,8 @@ template <int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradTable<kCapacity> t) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   const uint32_t chunks = t.first_chunk[t.count];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
@@ -667,8 +667,8 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const do
                                                                        float* out) {
   __shared__ double shared[kAdamThreads / 32];
   double sum = 0.0;
-  let_next_start();
-  wait_for_previous();
+  grid_launch_dependents();
+  grid_dependency_wait();
   for (int i = threadIdx.x; i < count; i += kAdamThreads) sum += slots[i];
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) {

@@ -46,12 +46,6 @@ __device__ __forceinline__ uint32_t lane_id() {
   return l;
 }
 
-// ------------------- kernels that follow one another -----------------------
-// The stream's next kernel, where it was launched so, may start once all blocks have said this or ended ...
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-// ... and waits here until this one has ended and what it wrote can be read.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ----------------------------- mbarrier ------------------------------------
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

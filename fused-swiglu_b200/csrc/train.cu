@@ -23,7 +23,7 @@ bool known_type(int t) { return t == FSWIGLU_OUT_BF16 || t == FSWIGLU_OUT_F32; }
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 size_t type_bytes(int t) { return t == FSWIGLU_OUT_F32 ? 4u : 2u; }
 
-// A launch that may start while the stream's previous kernel ends: its blocks come up, and wait (wait_for_previous) before
+// A launch that may start while the stream's previous kernel ends: its blocks come up, and wait (grid_dependency_wait) before
 // they touch memory.
 template <typename... Params, typename... Args>
 int launch(void (*kernel)(Params...), int64_t grid, dim3 block, size_t shared, cudaStream_t s, const Args&... args) {

@@ -142,6 +142,30 @@ def test_norm_forward_and_backward(lib, cuda_dev, M, d, t, wt, layer):
     check_backward(lib, dy, x, mean, rstd, w, res, layer, grads, wt)
 
 
+@pytest.mark.parametrize("layer", [True, False], ids=["layer", "rms"])
+@pytest.mark.parametrize("M,d", [(3, 4), (5, 7), (33, 128), (300, 256), (64, 1003), (150, 1032), (16, 4096), (3, 5120), (5, 8192),
+                                 (2, 8200), (2, 20001)])
+def test_norm_of_fp32_rows_with_bf16_vectors(lib, cuda_dev, M, d, layer):
+    x, w, b, dy, res = norm_inputs(M, d, F32, BF, cuda_dev, M * 5 + d, bias=layer)
+    check_forward(lib, x, w, b, 1e-5, layer)
+    _, mean, rstd = (v.float().to(cuda_dev) for v in forward64(x, w, b, 1e-5, layer))
+    if layer:
+        grads = lib.layer_norm_backward(dy, x, mean, rstd, w, True, res)
+    else:
+        grads = lib.rms_norm_backward(dy, x, rstd, w, res)
+    check_backward(lib, dy, x, mean, rstd, w, res, layer, grads, BF)
+
+
+@pytest.mark.parametrize("M", [147, 148, 149, 295, 296, 297, 1184, 1185])
+@pytest.mark.parametrize("d", [72, 99, 640])
+def test_norm_of_as_many_rows_as_blocks(lib, cuda_dev, M, d):
+    """One row less, as many, and one more than the grids have blocks."""
+    x, w, b, dy, res = norm_inputs(M, d, BF, BF, cuda_dev, M + d)
+    check_forward(lib, x, w, b, 1e-5, True)
+    _, mean, rstd = (v.float().to(cuda_dev) for v in forward64(x, w, b, 1e-5, True))
+    check_backward(lib, dy, x, mean, rstd, w, res, True, lib.layer_norm_backward(dy, x, mean, rstd, w, True, res), BF)
+
+
 @pytest.mark.parametrize("M,d", [(6, 100), (5, 4096), (40, 1003)])
 def test_norm_options(lib, cuda_dev, M, d):
     """Without weight, bias or residual; gradients in fp32; only the gradients that are asked for."""

@@ -321,6 +321,55 @@ def test_a_whole_training_step_from_a_captured_graph(fsw, cuda_dev, bits):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("before,after", [(False, False), (True, False), (False, True), (True, True)])
+def test_training_goes_on_from_a_checkpoint_on_the_host(fsw, cuda_dev, bits, before, after):
+    """The same bits as without the break, but for where the step's factors are computed (on the host, or on the device)."""
+    g = torch.Generator().manual_seed(5)
+    start = [torch.randn(n, generator=g) for n in (700, 4096, 33)]
+    grads = [[torch.randn(t.shape, generator=g).to(BF).to(cuda_dev) for t in start] for _ in range(4)]
+
+    def optimizer(values, capturable):
+        params = [torch.nn.Parameter(t.to(BF).to(cuda_dev)) for t in values]
+        return params, fsw.train.FusedAdamW(params, lr=1e-2, state_bits=bits, max_grad_norm=1.0, seed=3, capturable=capturable)
+
+    def steps(params, opt, which):
+        for gs in which:
+            for p, gr in zip(params, gs):
+                p.grad = gr
+            opt.step()
+
+    whole, opt = optimizer(start, before)
+    steps(whole, opt, grads[:2])
+    saved = {"params": [p.detach().cpu() for p in whole], "opt": {
+        "state": {i: {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in s.items()}
+                  for i, s in opt.state_dict()["state"].items()},
+        "param_groups": [{k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in group.items()}
+                         for group in opt.state_dict()["param_groups"]]}}
+    steps(whole, opt, grads[2:])
+    again, other = optimizer(saved["params"], after)
+    other.load_state_dict(saved["opt"])
+    if after:
+        for p, gr in zip(again, grads[2]):
+            p.grad = gr
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                other.step()
+        torch.cuda.synchronize()
+    steps(again, other, grads[2:])
+    for p, q in zip(whole, again):
+        if before == after:
+            assert torch.equal(p, q)
+            for key, value in opt.state[p].items():
+                if isinstance(value, torch.Tensor):
+                    assert torch.equal(value.view(torch.uint8), other.state[q][key].view(torch.uint8))
+        else:  # two steps of about lr, their size known to a few units of fp32; one rounding of the parameter may flip
+            within_steps = 2 * 1e-2 * 32 * U
+            a, b = opt.state[p]["master"].double(), other.state[q]["master"].double()
+            assert float((a - b).abs().max()) <= within_steps + 4 * U * float(a.abs().max())
+
+
 # ---------------------------------------------------------------- waits, launches that overlap
 
 @pytest.mark.parametrize("which", ["layer_forward", "rms_forward", "layer_backward", "rms_backward", "adamw_8bit"])

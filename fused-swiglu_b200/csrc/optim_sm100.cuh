@@ -639,12 +639,10 @@ __device__ __forceinline__ double sum_squares(const T* p, bool vector, int size,
   return sum;
 }
 
+// The squares of every gridDim.x-th chunk, over the block.
 template <int kCapacity>
-__global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradTable<kCapacity> t) {
-  __shared__ double shared[kAdamThreads / 32];
+__device__ __forceinline__ double sum_chunks(const GradTable<kCapacity>& t, double* shared) {
   double sum = 0.0;
-  grid_launch_dependents();
-  grid_dependency_wait();
   const uint32_t chunks = t.first_chunk[t.count];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int k = find_tensor(t.first_chunk, t.count, chunk);
@@ -658,11 +656,26 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_co
       sum += sum_squares<4>(static_cast<const __nv_bfloat16*>(a.grad) + base, a.vector, size, 0);
     }
   }
-  sum = block_sum(sum, shared);
-  if (threadIdx.x == 0) t.slots[blockIdx.x] = t.accumulate ? t.slots[blockIdx.x] + sum : sum;
+  return block_sum(sum, shared);
 }
 
 // out[0] = the norm, out[1] = min(1, max_norm / (norm + 1e-6)); NaN where the norm is not finite.
+__device__ __forceinline__ void write_norm(double sum, float max_norm, float* out) {
+  const double norm = sqrt(sum);
+  out[0] = static_cast<float>(norm);
+  out[1] = isfinite(out[0]) ? static_cast<float>(fmin(1.0, static_cast<double>(max_norm) / (norm + 1e-6)))
+                            : __uint_as_float(0x7fc00000u);
+}
+
+template <int kCapacity>
+__global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradTable<kCapacity> t) {
+  __shared__ double shared[kAdamThreads / 32];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const double sum = sum_chunks(t, shared);
+  if (threadIdx.x == 0) t.slots[blockIdx.x] = t.accumulate ? t.slots[blockIdx.x] + sum : sum;
+}
+
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const double* slots, int count, float max_norm,
                                                                        float* out) {
   __shared__ double shared[kAdamThreads / 32];
@@ -671,12 +684,28 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const do
   grid_dependency_wait();
   for (int i = threadIdx.x; i < count; i += kAdamThreads) sum += slots[i];
   sum = block_sum(sum, shared);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(sum);
-    out[0] = static_cast<float>(norm);
-    out[1] = isfinite(out[0]) ? static_cast<float>(fmin(1.0, static_cast<double>(max_norm) / (norm + 1e-6)))
-                              : __uint_as_float(0x7fc00000u);
-  }
+  if (threadIdx.x == 0) write_norm(sum, max_norm, out);
+}
+
+// Few chunks: the blocks are one cluster, which joins their sums in the memory of its first, in place of a second launch.
+constexpr int kFewBlocks = 8;  // the largest cluster that every device has
+template <int kCapacity>
+__global__ void __launch_bounds__(kAdamThreads) grad_norm_few_kernel(const __grid_constant__ GradTable<kCapacity> t, float max_norm,
+                                                                    float* out) {
+  __shared__ double shared[kAdamThreads / 32], joined[kFewBlocks];
+  cluster_arrive();
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const double sum = sum_chunks(t, shared);
+  cluster_wait();  // all blocks have started: their memory can be written
+  if (threadIdx.x == 0) store_cluster(map_to_cta(smem_u32(&joined[blockIdx.x]), 0), sum);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (blockIdx.x > 0 || threadIdx.x > 0) return;
+  double total = 0.0;
+  for (int r = 0; r < kFewBlocks; ++r) total += joined[r];
+  write_norm(total, max_norm, out);
 }
 
 }  // namespace fsw

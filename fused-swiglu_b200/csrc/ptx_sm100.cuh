@@ -370,6 +370,10 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t cluster_addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr), "d"(v) : "memory");
+}
+
 // ------------------------------- math --------------------------------------
 // silu(g) * u in fp32 with the fast exp / fast divide the reference kernel
 // uses (csrc/SwiGLU/swiglu.cu:96 under --use_fast_math).

@@ -24,22 +24,31 @@ bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(
 size_t type_bytes(int t) { return t == FSWIGLU_OUT_F32 ? 4u : 2u; }
 
 // A launch that may start while the stream's previous kernel ends: its blocks come up, and wait (grid_dependency_wait) before
-// they touch memory.
+// they touch memory.  Clusters of `cluster` blocks, where that is not 1.
 template <typename... Params, typename... Args>
-int launch(void (*kernel)(Params...), int64_t grid, dim3 block, size_t shared, cudaStream_t s, const Args&... args) {
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
+int launch_clusters(unsigned cluster, void (*kernel)(Params...), int64_t grid, dim3 block, size_t shared, cudaStream_t s,
+                    const Args&... args) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(grid));
   config.blockDim = block;
   config.dynamicSmemBytes = shared;
   config.stream = s;
-  config.attrs = &early;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster == 1 ? 1 : 2;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, static_cast<const std::decay_t<Params>&>(args)...);
   count_launch();
   return e == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_CUDA;
+}
+
+template <typename... Params, typename... Args>
+int launch(void (*kernel)(Params...), int64_t grid, dim3 block, size_t shared, cudaStream_t s, const Args&... args) {
+  return launch_clusters(1, kernel, grid, block, shared, s, args...);
 }
 
 // ---- norms ----
@@ -557,6 +566,15 @@ int adamw_launches(const fswiglu_adamw_tensor* tensors, int64_t count, const Ada
 }
 
 template <int kCapacity>
+void add_grad(GradTable<kCapacity>& t, const fswiglu_grad_tensor& a) {
+  if (a.numel == 0) return;
+  const bool f32 = a.dtype == FSWIGLU_OUT_F32;
+  t.tensors[t.count] = GradTensor{a.grad, static_cast<long long>(a.numel), f32, aligned(a.grad, f32 ? 32 : 16)};
+  t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(a.numel, kGradChunk);
+  ++t.count;
+}
+
+template <int kCapacity>
 int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double* slots, int* used, int sms, cudaStream_t s) {
   GradTable<kCapacity> t;
   t.slots = slots;
@@ -564,13 +582,7 @@ int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double
   t.first_chunk[0] = 0;
   t.accumulate = 0;
   for (int64_t i = 0; i < count; ++i) {
-    if (tensors[i].numel > 0) {
-      const bool f32 = tensors[i].dtype == FSWIGLU_OUT_F32;
-      t.tensors[t.count] = GradTensor{tensors[i].grad, static_cast<long long>(tensors[i].numel), f32,
-                                      aligned(tensors[i].grad, f32 ? 32 : 16)};
-      t.first_chunk[t.count + 1] = t.first_chunk[t.count] + chunks_of(tensors[i].numel, kGradChunk);
-      ++t.count;
-    }
+    add_grad(t, tensors[i]);
     if (t.count == 0 || (t.count < kCapacity && i + 1 < count)) continue;
     // every launch of a call has the same thread blocks: a later one adds to the slots of the first
     const int grid = std::min(kGradNormSlots, sms * 8);
@@ -580,6 +592,22 @@ int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double
     t.count = 0;
   }
   return FSWIGLU_OK;
+}
+
+// Up to this many chunks a launch of one cluster takes the place of one over all SMs and another that joins: 16 chunks of one
+// tensor 5.0 us a call (6.6 with two launches) and 2.5 to 3.2 us in a graph (3.2 to 3.5); 24 chunks 5.0 (6.5) and 3.0 to 3.9 (3.3 to
+// 3.6); 48 chunks 6.8 (6.5) and 6.2 (3.6) in fp32.
+constexpr int64_t kFewChunks = 24;
+static_assert(kFewChunks <= kSmallTable, "a tensor has a chunk at least");
+
+int grad_norm_few(const fswiglu_grad_tensor* tensors, int64_t count, float max_norm, float* out, cudaStream_t s) {
+  GradTable<kSmallTable> t;
+  t.slots = nullptr;
+  t.count = 0;
+  t.first_chunk[0] = 0;
+  t.accumulate = 0;
+  for (int64_t i = 0; i < count; ++i) add_grad(t, tensors[i]);
+  return launch_clusters(kFewBlocks, grad_norm_few_kernel<kSmallTable>, kFewBlocks, dim3(kAdamThreads), 0, s, t, max_norm, out);
 }
 
 }  // namespace
@@ -700,6 +728,7 @@ int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, fl
   if (workspace == nullptr || workspace_bytes < fswiglu_grad_norm_workspace_bytes() || !aligned(workspace, 256))
     return FSWIGLU_ERR_WORKSPACE;
   if (!aligned(out, 4)) return FSWIGLU_ERR_ALIGNMENT;
+  int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) {
     const fswiglu_grad_tensor& a = tensors[i];
     if (a.numel < 0 || !known_type(a.dtype)) return FSWIGLU_ERR_BAD_ARG;
@@ -707,10 +736,12 @@ int fswiglu_grad_norm_clip(const fswiglu_grad_tensor* tensors, int64_t count, fl
     if (a.numel > kMaxNumel) return FSWIGLU_ERR_SHAPE;
     if (a.grad == nullptr) return FSWIGLU_ERR_BAD_ARG;
     if (!aligned(a.grad, type_bytes(a.dtype))) return FSWIGLU_ERR_ALIGNMENT;
+    chunks += chunks_of(a.numel, kGradChunk);
   }
   Device dev;
   if (int rc = current_device(&dev)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (chunks <= kFewChunks) return grad_norm_few(tensors, count, max_norm, out, s);
   double* slots = static_cast<double*>(workspace);
   int used = 0;
   const int rc = count <= kSmallTable ? grad_norm_launches<kSmallTable>(tensors, count, slots, &used, dev.sms, s)

@@ -66,6 +66,10 @@ struct NormBackwardParams {
   long long ld_dout, ldx, ld_res, ld_dx;
   int M, d, splits;
   int w_f32;
+  int cluster;    // the grid is one cluster, which joins the splits itself and writes these:
+  int grad_f32;
+  void* dweight;  // NULL: not wanted
+  void* dbias;    // NULL: not wanted
   long long dx_step;  // bytes from a group's row to its next
   RingParams ring;
 };
@@ -423,6 +427,32 @@ struct Columns<float, N, P, false> {
   }
 };
 
+__device__ __forceinline__ void store_gradient(void* out, int i, bool f32, float v) {
+  if (f32) static_cast<float*>(out)[i] = v;
+  else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+}
+
+// The end of a backward kernel whose grid is one cluster: behind the cluster's barrier every block knows what the others wrote,
+// and takes its share of the columns.  In the order of the blocks; by way of L2, where the sums are.
+template <bool kLayer>
+__device__ __forceinline__ void join_in_cluster(const NormBackwardParams& p) {
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  const int threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int i = blockIdx.x * threads + thread; i < (kLayer ? 2 * p.d : p.d); i += gridDim.x * threads) {
+    const int which = i >= p.d, c = i - which * p.d;
+    void* const out = which ? p.dbias : p.dweight;
+    if (out == nullptr) continue;
+    float part[kFewBlocks], sum = 0.0f;  // all on their way at once
+#pragma unroll
+    for (int s = 0; s < kFewBlocks; ++s) part[s] = s < p.splits ? __ldcg(p.partial + (2ll * s + which) * p.d + c) : 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewBlocks; ++s) sum += part[s];
+    store_gradient(out, c, p.grad_f32, sum);
+  }
+}
+
 // Most threads of a block by the columns that a thread holds: what registers allow.  A scheduler holds a quarter of the
 // warps, so that 12 of them have 168 registers each, and 16 have 128.
 constexpr int wide_forward_threads(int) { return 512; }
@@ -675,9 +705,10 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgai
   }
   __syncthreads();
   float* part = p.partial + 2ll * blockIdx.x * p.d;
+  const bool counted = static_cast<int>(blockIdx.x) < p.splits;  // a cluster may have blocks without rows
   for (int i = thread * 4; i < (kLayer ? 2 * columns : columns); i += threads * 4) {
     const int which = i >= columns, c = i - which * columns;
-    if (c >= p.d) continue;
+    if (c >= p.d || !counted) continue;
     float4 total = *reinterpret_cast<const float4*>(joined + i);
     for (int g = 1; g < static_cast<int>(blockDim.y); ++g) {
       const float4 q = *reinterpret_cast<const float4*>(joined + g * group_floats + i);
@@ -688,6 +719,7 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgai
     }
     *reinterpret_cast<float4*>(part + which * p.d + c) = total;
   }
+  if (p.cluster) join_in_cluster<kLayer>(p);
 }
 
 // ---- rows that start anywhere ----
@@ -901,33 +933,35 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
   const int columns = blockDim.x * N, group_floats = 2 * columns;
   const int threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
   float* part = p.partial + 2ll * blockIdx.x * p.d;
+  const bool counted = static_cast<int>(blockIdx.x) < p.splits;  // a cluster may have blocks without rows
   if (blockDim.y == 1) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = j * blockDim.x + threadIdx.x;
-      if (c >= p.d) continue;
+      if (c >= p.d || !counted) continue;
       part[c] = dw[j];
       if (kLayer) part[p.d + c] = db[kLayer ? j : 0];
     }
-    return;
-  }
-  // [group][2][columns]: the groups' sums side by side, joined in the order of the groups
-  float* joined = reinterpret_cast<float*>(ring_memory);
-  __syncthreads();
+  } else {
+    // [group][2][columns]: the groups' sums side by side, joined in the order of the groups
+    float* joined = reinterpret_cast<float*>(ring_memory);
+    __syncthreads();
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = j * blockDim.x + threadIdx.x;
-    joined[threadIdx.y * group_floats + c] = dw[j];
-    if (kLayer) joined[threadIdx.y * group_floats + columns + c] = db[kLayer ? j : 0];
+    for (int j = 0; j < N; ++j) {
+      const int c = j * blockDim.x + threadIdx.x;
+      joined[threadIdx.y * group_floats + c] = dw[j];
+      if (kLayer) joined[threadIdx.y * group_floats + columns + c] = db[kLayer ? j : 0];
+    }
+    __syncthreads();
+    for (int i = thread; i < (kLayer ? 2 * columns : columns); i += threads) {
+      const int which = i >= columns, c = i - which * columns;
+      if (c >= p.d || !counted) continue;
+      float total = 0.0f;
+      for (int g = 0; g < static_cast<int>(blockDim.y); ++g) total += joined[g * group_floats + i];
+      part[which * p.d + c] = total;
+    }
   }
-  __syncthreads();
-  for (int i = thread; i < (kLayer ? 2 * columns : columns); i += threads) {
-    const int which = i >= columns, c = i - which * columns;
-    if (c >= p.d) continue;
-    float total = 0.0f;
-    for (int g = 0; g < static_cast<int>(blockDim.y); ++g) total += joined[g * group_floats + i];
-    part[which * p.d + c] = total;
-  }
+  if (p.cluster) join_in_cluster<kLayer>(p);
 }
 
 // ---- short rows ----
@@ -1081,13 +1115,15 @@ __global__ void __launch_bounds__(kShortThreads) norm_backward_short_kernel(cons
   }
   __syncthreads();
   float* part = p.partial + 2ll * blockIdx.x * p.d;
+  const bool counted = static_cast<int>(blockIdx.x) < p.splits;  // a cluster may have blocks without rows
   for (int i = thread; i < (kLayer ? 2 * columns : columns); i += kShortThreads) {
     const int which = i >= columns, column = i - which * columns;
-    if (column >= p.d) continue;
+    if (column >= p.d || !counted) continue;
     float total = 0.0f;
     for (int g = 0; g < static_cast<int>(blockDim.y); ++g) total += joined[which][g * columns + column];
     part[which * p.d + column] = total;
   }
+  if (p.cluster) join_in_cluster<kLayer>(p);
 }
 
 // Joins the splits' sums: 32 columns a block, whose 32 rows of threads take every 32nd split.  The order is fixed.  Its blocks
@@ -1115,8 +1151,7 @@ __global__ void __launch_bounds__(32 * kNormReduceRows) norm_reduce_kernel(const
   for (int r = 0; r < kNormReduceRows; ++r) sum += shared[threadIdx.y][r][threadIdx.x];
   void* out = threadIdx.y == 0 ? p.dweight : p.dbias;
   if (out == nullptr || i >= p.d) return;
-  if (p.out_f32) static_cast<float*>(out)[i] = sum;
-  else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(sum);
+  store_gradient(out, i, p.out_f32, sum);
 }
 
 }  // namespace fsw

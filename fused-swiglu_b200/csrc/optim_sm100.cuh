@@ -688,7 +688,6 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_finish_kernel(const do
 }
 
 // Few chunks: the blocks are one cluster, which joins their sums in the memory of its first, in place of a second launch.
-constexpr int kFewBlocks = 8;  // the largest cluster that every device has
 template <int kCapacity>
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_few_kernel(const __grid_constant__ GradTable<kCapacity> t, float max_norm,
                                                                     float* out) {

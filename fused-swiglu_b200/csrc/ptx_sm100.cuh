@@ -370,6 +370,7 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+constexpr int kFewBlocks = 8;  // of a grid that is one cluster, for little work: the largest that every device has
 __device__ __forceinline__ void store_cluster(uint32_t cluster_addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr), "d"(v) : "memory");
 }

@@ -238,16 +238,31 @@ int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cuda
                 dim3(kNormThreads), 0, s, p);
 }
 
+// Little work: one cluster, whose blocks join their sums over rows themselves, takes the place of a grid over all SMs and a
+// second launch.  Layer norm, bf16, a call / in a graph, us, with two launches in brackets: 64 x 128 6.5 / 3.1 (8.3 / 3.4), 128 x 256
+// 6.4 / 3.5 (8.3 / 4.0), 32 x 1024 6.6 / 3.9 (8.6 / 4.2), 8 x 4096 6.7 / 5.3 (8.5 / 4.3); above, graphs lose more than calls gain:
+// 512 x 128 6.6 / 4.6 (8.5 / 3.8), 64 x 1003 7.0 / 6.6 (8.4 / 4.6), 8 x 8192 7.9 / 7.5 (8.5 / 6.7).
+constexpr int64_t kFewValues = 1 << 15;
+bool few_values(const NormBackwardParams& p) { return p.partial != nullptr && static_cast<int64_t>(p.M) * p.d <= kFewValues; }
+int backward_splits(const NormBackwardParams& p, int64_t blocks, int64_t most) {
+  return static_cast<int>(std::min<int64_t>({blocks, p.cluster ? kFewBlocks : most, kMaxNormSplits}));
+}
+template <typename Kernel>
+int launch_backward(Kernel kernel, dim3 block, size_t shared, cudaStream_t s, const NormBackwardParams& p) {
+  if (p.cluster) return launch_clusters(kFewBlocks, kernel, kFewBlocks, block, shared, s, p);
+  return launch(kernel, p.splits, block, shared, s, p);
+}
+
 template <typename T, bool kLayer, int N>
 int launch_norm_backward_odd(NormBackwardParams& p, const WidePlan& w, const Device& dev, cudaStream_t s) {
   constexpr auto kernel = norm_backward_odd_kernel<T, kLayer, N>;
   static std::atomic<uint64_t> done{0};
   if (int rc = opt_in(kernel, &done, dev)) return rc;
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
-  p.splits = static_cast<int>(std::min<int64_t>({blocks, dev.sms, kMaxNormSplits}));
+  p.splits = backward_splits(p, blocks, dev.sms);
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, p.splits, dim3(w.group, w.groups), w.ring(), s, p);
+  return launch_backward(kernel, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 template <typename T, typename W, bool kLayer, int kColumns, bool kAgain>
@@ -256,12 +271,12 @@ int launch_norm_backward_wide(NormBackwardParams& p, const WidePlan& w, const De
   static std::atomic<uint64_t> done{0};
   if (int rc = opt_in(kernel, &done, dev)) return rc;
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
-  const int grid = static_cast<int>(std::min<int64_t>({blocks, dev.sms, kMaxNormSplits}));
-  p.splits = grid;
+  p.splits = backward_splits(p, blocks, dev.sms);
+  const int grid = p.cluster ? kFewBlocks : p.splits;
   p.dx_step = static_cast<long long>(grid) * w.groups * p.ld_dx * static_cast<long long>(sizeof(T));
   p.ring.places = w.places;
   p.ring.withhold = take_withhold();
-  return launch(kernel, grid, dim3(w.group, w.groups), w.ring(), s, p);
+  return launch_backward(kernel, dim3(w.group, w.groups), w.ring(), s, p);
 }
 
 // Backward: one block an SM, its registers full of the sums over rows.  Of the columns a thread may hold, those that keep most
@@ -301,8 +316,9 @@ template <typename T, typename W, bool kLayer>
 int launch_norm_backward_short(NormBackwardParams& p, const Device& dev, cudaStream_t s) {
   const int lanes = short_lanes(p.d, kPerVector<T>), parts = kShortThreads / lanes;
   const int64_t blocks = (static_cast<int64_t>(p.M) + parts - 1) / parts;
-  p.splits = static_cast<int>(std::min<int64_t>({blocks, static_cast<int64_t>(dev.sms) * 2, kMaxNormSplits}));
-  return launch(norm_backward_short_kernel<T, W, kLayer>, p.splits, dim3(lanes, parts), 0, s, p);
+  p.cluster = few_values(p);
+  p.splits = backward_splits(p, blocks, static_cast<int64_t>(dev.sms) * 2);
+  return launch_backward(norm_backward_short_kernel<T, W, kLayer>, dim3(lanes, parts), 0, s, p);
 }
 
 template <typename T, bool kLayer>
@@ -312,14 +328,18 @@ int launch_norm_backward(NormBackwardParams& p, bool wide, const Device& dev, cu
       if (p.w_f32) return launch_norm_backward_short<T, float, kLayer>(p, dev, s);
       return launch_norm_backward_short<T, __nv_bfloat16, kLayer>(p, dev, s);
     }
-    const WidePlan w = backward_plan(p, kLayer, sizeof(T), dev.sms);
+    const bool few = few_values(p);
+    const WidePlan w = backward_plan(p, kLayer, sizeof(T), few ? kFewBlocks : dev.sms);
     if (w.columns > 0) {
+      p.cluster = few;
       if (p.w_f32) return launch_norm_backward_wide<T, float, kLayer>(p, w, dev, s);
       return launch_norm_backward_wide<T, __nv_bfloat16, kLayer>(p, w, dev, s);
     }
   } else {
-    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), kOddThreads, 3, kWidePlaces, dev.sms);
+    const bool few = few_values(p);
+    const WidePlan w = odd_plan(p.d, p.M, sizeof(T), kOddThreads, 3, kWidePlaces, few ? kFewBlocks : dev.sms);
     if (w.columns > 0) {
+      p.cluster = few;
       if (w.columns == 4) return launch_norm_backward_odd<T, kLayer, 4>(p, w, dev, s);
       if (w.columns == 8) return launch_norm_backward_odd<T, kLayer, 8>(p, w, dev, s);
       return launch_norm_backward_odd<T, kLayer, 16>(p, w, dev, s);
@@ -414,6 +434,9 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     p.ldx = ldx;
     p.ld_res = ld_res;
     p.ld_dx = ld_dx;
+    p.grad_f32 = grad_dtype == FSWIGLU_OUT_F32;
+    p.dweight = dweight;
+    p.dbias = dbias;
     p.M = static_cast<int>(M);
     p.d = static_cast<int>(d);
     p.splits = norm_splits(M);
@@ -430,7 +453,7 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
       rc = layer ? launch_norm_backward<BF, true>(p, wide, dev, s) : launch_norm_backward<BF, false>(p, wide, dev, s);
     if (rc) return rc;
   }
-  if (!columns) return FSWIGLU_OK;
+  if (!columns || p.cluster) return FSWIGLU_OK;
   NormReduceParams q = {};  // no rows: no splits, the gradients are zero
   q.partial = p.partial;
   q.dweight = dweight;

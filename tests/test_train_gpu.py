@@ -166,6 +166,25 @@ def test_norm_of_as_many_rows_as_blocks(lib, cuda_dev, M, d):
     check_backward(lib, dy, x, mean, rstd, w, res, True, lib.layer_norm_backward(dy, x, mean, rstd, w, True, res), BF)
 
 
+@pytest.mark.parametrize("t", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("d", [8, 56, 99, 136, 1003, 1032, 4096, 8192])
+def test_norm_gradients_of_few_rows(lib, cuda_dev, d, t):
+    """Row counts around those up to which one cluster takes all rows, blocks without rows among them."""
+    for M in (1, 2, 7, 8, 9, 31, 32, 33, 63, 65, 96, 97, 128, 129, 256, 257, 513, 769, 1025):
+        x, w, b, dy, res = norm_inputs(M, d, t, t, cuda_dev, M + d)
+        for layer in (True, False):
+            _, mean, rstd = (v.float().to(cuda_dev) for v in forward64(x, w, b if layer else None, 1e-5, layer))
+            if layer:
+                grads = lib.layer_norm_backward(dy, x, mean, rstd, w, True, res)
+                only_b = lib.layer_norm_backward(dy, x, mean, rstd, w, True, res, weight_grad=False)
+                only_w = lib.layer_norm_backward(dy, x, mean, rstd, w, False, res)
+                assert only_b[1] is None and torch.equal(only_b[2], grads[2])
+                assert only_w[2] is None and torch.equal(only_w[1], grads[1])
+            else:
+                grads = lib.rms_norm_backward(dy, x, rstd, w, res)
+            check_backward(lib, dy, x, mean, rstd, w, res, layer, grads, t)
+
+
 @pytest.mark.parametrize("M,d", [(6, 100), (5, 4096), (40, 1003)])
 def test_norm_options(lib, cuda_dev, M, d):
     """Without weight, bias or residual; gradients in fp32; only the gradients that are asked for."""
@@ -835,3 +854,16 @@ def test_grad_norm_is_deterministic_and_runs_twice_at_once(lib, cuda_dev):
             got += [lib.grad_norm_clip(g, 1.0) for _ in range(3)]
     torch.cuda.synchronize()
     assert all(torch.equal(v, want) for v in got)
+
+
+def test_grad_norm_of_few_and_many_chunks(lib, cuda_dev):
+    """Around the sizes where one cluster gives way to a grid over the device: one large tensor, many small ones."""
+    g = torch.Generator().manual_seed(8)
+    for k, n in ((1, 24 * 8192), (1, 24 * 8192 + 1), (1, 8 * 8192), (24, 3), (25, 3), (12, 8193), (13, 8193), (48, 1), (49, 1)):
+        grads = [torch.randn(n, generator=g).to(BF if i % 2 else F32).to(cuda_dev) for i in range(k)]
+        want = math.sqrt(sum(float(v.double().square().sum()) for v in grads))
+        out = lib.grad_norm_clip(grads, 0.5)
+        # 16 squares a thread of a chunk, summed in fp32, halved by the root; one rounding at the end
+        assert abs(float(out[0]) - want) <= (17 / 2 + 1) * U * want
+        factor = min(1.0, 0.5 / (want + 1e-6))
+        assert abs(float(out[1]) - factor) <= (17 / 2 + 2) * U * factor

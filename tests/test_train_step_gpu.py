@@ -477,6 +477,53 @@ def test_launches_that_overlap_wait_for_what_was_written_before(fsw, cuda_dev):
             assert torch.equal(a, b)
 
 
+def small_chain(fsw, x, w, dy, p, m, v):
+    """Norm forward and backward, the gradients' norm, a step: each reads what the one before it wrote."""
+    lib = fsw.train._lib()
+    y, mean, rstd = lib.layer_norm_forward(x, w)
+    dx, dw, db = lib.layer_norm_backward(dy, y, mean, rstd, w, True)
+    clip = lib.grad_norm_clip([dw, db, dx], 0.5)
+    lib.adamw_step([p], [dw], [m], [v], 1, 1e-2, grad_scale=clip[1:])
+    return dx, dw, db, clip, p, m, v
+
+
+@pytest.mark.parametrize("M,d", [(3, 56), (32, 1000), (9, 1003), (8, 4096)])
+def test_small_launches_in_a_row_on_two_streams_and_from_a_graph(fsw, cuda_dev, M, d):
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        draw = lambda *shape: torch.randn(shape, generator=g).to(cuda_dev)  # noqa: E731
+        return [draw(M, d).to(BF), draw(d).to(BF), draw(M, d).to(BF), draw(d), torch.zeros(d, device=cuda_dev),
+                torch.zeros(d, device=cuda_dev)]
+
+    def same(a, b):
+        return all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
+
+    want = []
+    for seed in range(8):
+        args = inputs(seed)
+        out = small_chain(fsw, *args)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in out])
+    args = [inputs(seed) for seed in range(8)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for seed in range(8):
+        with torch.cuda.stream(streams[seed % 2]):
+            got.append(small_chain(fsw, *args[seed]))
+    torch.cuda.synchronize()
+    assert all(same(a, b) for a, b in zip(got, want))
+    static = inputs(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = small_chain(fsw, *static)
+    for seed in (3, 5, 3):
+        for t, new in zip(static, inputs(seed)):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want[seed])
+
+
 def test_first_calls_of_a_new_thread(fsw, cuda_dev):
     """A backward pass runs on a thread of autograd's, whose first CUDA call may be any of the library's."""
     import threading

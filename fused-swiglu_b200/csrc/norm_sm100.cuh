@@ -370,21 +370,42 @@ struct RowRing {
   }
 };
 
+// Vectors may be what the kernel before this one is still writing while these blocks come up (an optimiser's step in front of a
+// norm): they are read by ordinary loads, behind grid_dependency_wait, not by way of the non-coherent path, which asks for
+// data that nobody writes while the kernel lives.  The pointer is made known behind the wait, so that a load of it, which the
+// compiler may otherwise move and issue early, stays there.
+__device__ __forceinline__ const void* behind_wait(const void* p) {
+  const void* q;
+  asm volatile("mov.b64 %0, %1;" : "=l"(q) : "l"(p) : "memory");
+  return q;
+}
+__device__ __forceinline__ float4 load_columns(const float4* p) {
+  float4 f;
+  asm("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint32_t load_columns(const uint32_t* p) {
+  uint32_t w;
+  asm("ld.global.b32 %0, [%1];" : "=r"(w) : "l"(p));
+  return w;
+}
+
 // What a thread keeps of a weight or bias vector: bf16 values as they are, and few fp32 ones; many fp32 ones come from the L1
-// cache row by row.  A missing vector is bf16 ones or zeros.
+// cache row by row.  A missing vector is bf16 ones or zeros.  `init` is called behind grid_dependency_wait.
 template <typename W, int N, int P, bool kKeep = true>
 struct Columns;
 template <int N, int P>
 struct Columns<float, N, P, true> {
   Pair w[N][P / 2];
-  __device__ __forceinline__ void init(const void* p, uint32_t, int d) {
+  __device__ __forceinline__ void init(const void* given, uint32_t, int d) {
+    const void* const p = behind_wait(given);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * blockDim.x + threadIdx.x) * P;
 #pragma unroll
       for (int i = 0; i < P / 4; ++i) {
         float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (c < d) f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c) + i);
+        if (c < d) f = load_columns(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c) + i);
         w[j][2 * i] = make_pair(f.x, f.y);
         w[j][2 * i + 1] = make_pair(f.z, f.w);
       }
@@ -398,13 +419,14 @@ struct Columns<float, N, P, true> {
 template <int N, int P, bool kKeep>
 struct Columns<__nv_bfloat16, N, P, kKeep> {
   uint32_t w[N][P / 2];
-  __device__ __forceinline__ void init(const void* p, uint32_t none, int d) {
+  __device__ __forceinline__ void init(const void* given, uint32_t none, int d) {
+    const void* const p = behind_wait(given);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * blockDim.x + threadIdx.x) * P;
       const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p) + c);
 #pragma unroll
-      for (int i = 0; i < P / 2; ++i) w[j][i] = p != nullptr && c < d ? __ldg(q + i) : none;
+      for (int i = 0; i < P / 2; ++i) w[j][i] = p != nullptr && c < d ? load_columns(q + i) : none;
     }
   }
   __device__ __forceinline__ void get(int j, bool, Pair (&v)[P / 2]) const {
@@ -415,12 +437,14 @@ struct Columns<__nv_bfloat16, N, P, kKeep> {
 template <int N, int P>
 struct Columns<float, N, P, false> {
   const float* q;
-  __device__ __forceinline__ void init(const void* p, uint32_t, int) { q = static_cast<const float*>(p) + threadIdx.x * P; }
+  __device__ __forceinline__ void init(const void* given, uint32_t, int) {
+    q = static_cast<const float*>(behind_wait(given)) + threadIdx.x * P;
+  }
   __device__ __forceinline__ void get(int j, bool valid, Pair (&v)[P / 2]) const {
 #pragma unroll
     for (int i = 0; i < P / 4; ++i) {
       float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (valid) f = __ldg(reinterpret_cast<const float4*>(q + j * blockDim.x * P) + i);
+      if (valid) f = load_columns(reinterpret_cast<const float4*>(q + j * blockDim.x * P) + i);
       v[2 * i] = make_pair(f.x, f.y);
       v[2 * i + 1] = make_pair(f.z, f.w);
     }

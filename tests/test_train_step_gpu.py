@@ -555,3 +555,40 @@ def test_first_calls_of_a_new_thread(fsw, cuda_dev):
         torch.cuda.synchronize()
         assert isinstance(got[0], torch.Tensor), (name, got[0])
         assert torch.equal(got[0], want), name
+
+
+@pytest.mark.parametrize("M,d", [(64, 128), (40, 1024), (300, 4096), (700, 5120), (30, 1003)])
+@pytest.mark.parametrize("wt", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_norms_read_the_vectors_that_a_step_has_just_written(fsw, cuda_dev, M, d, wt):
+    """The optimiser's step on the norm's vectors directly in front of both passes, whose blocks come up while it ends: the same
+    bits as with a pause behind each call."""
+    lib = fsw.train._lib()
+    g = torch.Generator().manual_seed(M + d)
+    x, dy = (torch.randn((M, d), generator=g).to(BF).to(cuda_dev) for _ in range(2))
+    grads = [torch.randn(d, generator=g).to(wt).to(cuda_dev) for _ in range(2)]
+    start = [torch.randn(d, generator=g).to(wt).to(cuda_dev) for _ in range(2)]
+
+    def steps(pause):
+        vectors = [t.clone() for t in start]
+        m, v = ([torch.zeros(d, device=cuda_dev) for _ in vectors] for _ in range(2))
+        out = []
+        for k in range(1, 41):
+            lib.adamw_step(vectors, grads, m, v, k, 0.05)
+            pause()
+            y, mean, rstd = lib.layer_norm_forward(x, *vectors)
+            pause()
+            lib.adamw_step(vectors, grads, m, v, k, 0.05)
+            pause()
+            dx, dw, db = lib.layer_norm_backward(dy, x, mean, rstd, vectors[0], True)
+            pause()
+            lib.adamw_step(vectors, grads, m, v, k, 0.05)
+            pause()
+            out += [y, dx, dw, db, lib.rms_norm_forward(x, vectors[0])[0]]
+            pause()
+        return out
+
+    want = steps(torch.cuda.synchronize)
+    for _ in range(3):
+        got = steps(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not torch.equal(want[0], want[5])  # the vectors do move

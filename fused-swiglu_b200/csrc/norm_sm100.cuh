@@ -352,6 +352,7 @@ struct RowRing {
         }
       }
     }
+    fence_proxy_async();  // the place's next row may come over these elements by a bulk copy, which this thread asks for
     return true;
   }
   __device__ __forceinline__ void wait() const { wd.wait(bars + 8 * at, phase, kSiteRowRing); }

@@ -255,6 +255,25 @@ def test_norm_outputs_stay_in_their_rows(fsw, lib, cuda_dev, M, d, pitch, offset
     assert all(bool((s[M:] == 77.0).all()) for s in stats) and all(bool((v[d:] == 77.0).all()) for v in vectors)
 
 
+@pytest.mark.parametrize("t", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,d", [(3000, 99), (9000, 37), (1300, 1003)])
+def test_norm_bits_do_not_depend_on_where_rows_start(lib, cuda_dev, M, d, t):
+    """The first row's first elements, copied one by one, lie where later rows of the same place come by bulk copies."""
+    x, w, b, dy, res = norm_inputs(M, d, t, t, cuda_dev, M + d)
+    want = lib.layer_norm_forward(x, w, b)
+    grads = lib.layer_norm_backward(dy, x, *want[1:], w, True, res)
+    for offset in range(1, 16 // t.itemsize):
+        def moved(v):
+            flat = torch.empty(M * d + 16, dtype=t, device=cuda_dev)
+            flat[offset:offset + M * d] = v.view(-1)
+            return flat[offset:offset + M * d].view(M, d)
+
+        got = lib.layer_norm_forward(moved(x), w, b)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        got = lib.layer_norm_backward(moved(dy), moved(x), *want[1:], w, True, moved(res))
+        assert all(torch.equal(p, q) for p, q in zip(got, grads))
+
+
 def test_norm_offsets_past_32_bits(lib, cuda_dev):
     """More than 2^31 elements: the last rows are what a call of those alone gives, and the others' zeros add nothing."""
     M, d, n = 530_000, 4096, 40

@@ -20,6 +20,7 @@
 #include <cstdint>
 
 #include "ptx_sm100.cuh"
+#include "row_granules.h"
 #include "vector_io_sm100.cuh"
 
 namespace fsw {
@@ -323,8 +324,8 @@ struct RowRing {
     }
     return true;
   }
-  // The first row of all or the last has no neighbours on one side: the elements of its granule there, fewer than 16 bytes, are
-  // copied one by one.
+  // The first rows of all and the last (edge_rows) have no neighbours on one side: the elements of their granules there, fewer
+  // than 16 bytes, are copied one by one.
   template <typename T>
   __device__ __noinline__ bool ask_edge(int place, const T* x, const T* dy, const T* res, int arrays, int d, bool first, bool last,
                                         bool withhold) const {
@@ -336,19 +337,18 @@ struct RowRing {
       if (turn == 1) mbar_arrive_expect_tx(bar, bytes);
       for (int i = 0; i < arrays; ++i) {
         const uint64_t begin = reinterpret_cast<uint64_t>(src[i]), end = begin + static_cast<uint64_t>(d) * sizeof(T);
-        const uint64_t granule = begin & ~15ull;
-        const uint64_t lo = first ? (begin + 15) & ~15ull : granule, hi = last ? end & ~15ull : (end + 15) & ~15ull;
-        const uint32_t here = data + place * place_bytes + i * array_bytes, size = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+        const RowGranules g(begin, end, first, last);
+        const uint32_t here = data + place * place_bytes + i * array_bytes, size = g.bytes();
         if (turn == 1) {
-          if (size > 0 && !withhold) bulk_row(here + static_cast<uint32_t>(lo - granule), reinterpret_cast<const void*>(lo), size, bar);
+          if (size > 0 && !withhold) bulk_row(here + static_cast<uint32_t>(g.lo - g.granule), reinterpret_cast<const void*>(g.lo), size, bar);
           continue;
         }
         if (!withhold) bytes += size;
-        for (uint64_t q = begin; first && q < lo && q < end; q += sizeof(T)) {
-          store_shared(here + static_cast<uint32_t>(q - granule), *reinterpret_cast<const T*>(q));
+        for (uint64_t q = begin; first && q < g.lo && q < end; q += sizeof(T)) {
+          store_shared(here + static_cast<uint32_t>(q - g.granule), *reinterpret_cast<const T*>(q));
         }
-        for (uint64_t q = hi < begin ? begin : hi; last && q < end; q += sizeof(T)) {
-          store_shared(here + static_cast<uint32_t>(q - granule), *reinterpret_cast<const T*>(q));
+        for (uint64_t q = g.hi < begin ? begin : g.hi; last && q < end; q += sizeof(T)) {
+          store_shared(here + static_cast<uint32_t>(q - g.granule), *reinterpret_cast<const T*>(q));
         }
       }
     }
@@ -797,13 +797,15 @@ __global__ void __launch_bounds__(kOddThreads, 2) norm_forward_odd_kernel(const 
   __syncthreads();
   grid_launch_dependents();
   grid_dependency_wait();
+  const int edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   auto source = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const T* const src[1] = {source(n)};
     const int r = row + n * stride;
-    if (r > 0 && r < p.M - 1) asked += ring.ask_granules(place, src, 1);
-    else asked += ring.ask_edge(place, src[0], src[0], src[0], 1, p.d, r == 0, r == p.M - 1, p.ring.withhold && r == 0);
+    const bool first = r < edge, last = r >= p.M - edge;
+    if (!first && !last) asked += ring.ask_granules(place, src, 1);
+    else asked += ring.ask_edge(place, src[0], src[0], src[0], 1, p.d, first, last, p.ring.withhold && r == 0);
   };
   const int ahead = ring.places - 1;
   if (threadIdx.x == 0) {
@@ -878,6 +880,7 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
   __syncthreads();
   grid_launch_dependents();
   grid_dependency_wait();
+  const int edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   auto x_of = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   auto dy_of = [&](int n) { return static_cast<const T*>(p.dout) + (row + n * stride) * p.ld_dout; };
   auto res_of = [&](int n) { return static_cast<const T*>(p.residual) + (residual ? (row + n * stride) * p.ld_res : 0); };
@@ -886,8 +889,9 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
     const T* const src[3] = {x_of(n), dy_of(n), res_of(n)};
     const int r = row + n * stride;
     const int arrays = residual ? 3 : 2;
-    if (r > 0 && r < p.M - 1) asked += ring.ask_granules(place, src, arrays);
-    else asked += ring.ask_edge(place, src[0], src[1], src[2], arrays, p.d, r == 0, r == p.M - 1, p.ring.withhold && r == 0);
+    const bool first = r < edge, last = r >= p.M - edge;
+    if (!first && !last) asked += ring.ask_granules(place, src, arrays);
+    else asked += ring.ask_edge(place, src[0], src[1], src[2], arrays, p.d, first, last, p.ring.withhold && r == 0);
   };
   const int ahead = ring.places - 1;
   if (threadIdx.x == 0) {

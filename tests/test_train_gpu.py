@@ -274,6 +274,23 @@ def test_norm_bits_do_not_depend_on_where_rows_start(lib, cuda_dev, M, d, t):
         assert all(torch.equal(p, q) for p, q in zip(got, grads))
 
 
+@pytest.mark.parametrize("t", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 6, 7])
+def test_norm_of_rows_within_a_granule(lib, cuda_dev, d, t):
+    """Rows of less than 16 bytes, several of which share the matrix's first granule and its last, from every start."""
+    for M in (1, 2, 3, 4, 9, 16, 17, 40, 5000):
+        x, w, b, dy, res = norm_inputs(M, d, t, t, cuda_dev, M + d)
+        want = lib.layer_norm_forward(x, w, b)
+        check_forward(lib, x, w, b, 1e-5, True, out=want)
+        for offset in range(0, 16 // t.itemsize):
+            flat = torch.full((M * d + 16,), float("nan"), dtype=t, device=cuda_dev)
+            flat[offset:offset + M * d] = x.view(-1)
+            moved = flat[offset:offset + M * d].view(M, d)
+            assert all(torch.equal(p, q) for p, q in zip(lib.layer_norm_forward(moved, w, b), want))
+        grads = lib.layer_norm_backward(dy, x, *want[1:], w, True, res)
+        check_backward(lib, dy, x, *want[1:], w, res, True, grads, t)
+
+
 def test_norm_offsets_past_32_bits(lib, cuda_dev):
     """More than 2^31 elements: the last rows are what a call of those alone gives, and the others' zeros add nothing."""
     M, d, n = 530_000, 4096, 40

@@ -74,6 +74,20 @@ def test_norm_workspace_is_host_arithmetic():
     assert capi.lib.fswiglu_grad_norm_workspace_bytes() >= 256
 
 
+def test_norm_rows_are_read_inside_their_matrix(tmp_path):
+    """What the norms copy of rows that start anywhere is plain integer code (csrc/row_granules.h): compile the checker with g++ and
+    run it over alignments, widths, pitches and row counts."""
+    import os
+    import subprocess
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe, src = tmp_path / "check_row_granules", os.path.join(here, "native", "check_row_granules.cpp")
+    inc = os.path.join(here, "..", "fused-swiglu_b200", "csrc")
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{inc}", src, "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.startswith("ok "), res.stdout[-400:]
+
+
 def adamw(m, tensors=None, pt=BF, gt=BF, bits=32, count=None, **options):
     plain = dict(param=m(), grad=m(1024), exp_avg=m(2048), exp_avg_sq=m(3072), numel=64)
     tensors = [plain] if tensors is None else [{**plain, **t} for t in tensors]

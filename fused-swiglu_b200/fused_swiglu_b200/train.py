@@ -221,8 +221,11 @@ class FusedAdamW(torch.optim.Optimizer):
                 g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
                 every.append(g)
                 kinds.setdefault((p.device, p.dtype, g.dtype, self.state.get(p, {}).get("step", 0)), []).append((p, g))
-            if self.capturable and len({(k[0], k[3]) for k in kinds}) > 1:
-                raise RuntimeError("with capturable=True all parameters of a group take every step together")
+            if self.capturable and kinds:
+                # one count for the group: those with gradients are those with state, but for the first step's
+                known = {p for p in group["params"] if self.state.get(p)}
+                if len({(k[0], k[3]) for k in kinds}) > 1 or (known and known != {p for of in kinds.values() for p, _ in of}):
+                    raise RuntimeError("with capturable=True all parameters of a group take every step together")
             work += [(index, group, key, tensors) for key, tensors in kinds.items()]
         if not work:
             return loss

@@ -268,6 +268,51 @@ def test_optimizer_takes_its_step_count_over_a_checkpoint_either_way(recorder):
     assert [s["step_t"] for s in recorder.steps] == [2, 2]
 
 
+def test_optimizer_with_its_step_on_the_device_refuses_who_joins_or_skips(recorder):
+    """One count serves the whole group: a parameter of fewer steps would get the bias corrections of another's."""
+    def refused(opt):
+        recorder.steps.clear()
+        with pytest.raises(RuntimeError, match="every step together"):
+            opt.step()
+        assert not recorder.steps
+
+    for late in range(3):
+        ps = some_params()
+        joins, grad = ps[late], ps[late].grad
+        joins.grad = None
+        opt = train.FusedAdamW(ps, capturable=True)
+        for _ in range(5):
+            opt.step()
+        count = int(opt.param_groups[0]["step_tensor"])
+        joins.grad = grad
+        refused(opt)
+        assert int(opt.param_groups[0]["step_tensor"]) == count == 5 and joins not in opt.state
+        joins.grad = None
+        opt.step()  # as before
+        other_params = some_params()
+        other = train.FusedAdamW(other_params, capturable=True)
+        other.load_state_dict(opt.state_dict())
+        refused(other)  # the checkpoint knows who has taken part
+        other_params[late].grad = None
+        other.step()
+        assert int(other.param_groups[0]["step_tensor"]) == 7
+    ps = some_params()
+    opt = train.FusedAdamW(ps, capturable=True)
+    opt.step()
+    ps[1].grad = None
+    refused(opt)
+    for p in ps:
+        p.grad = None
+    opt.step()  # nobody: no step
+    assert int(opt.param_groups[0]["step_tensor"]) == 1
+    frozen = [{"params": some_params()[:1]}, {"params": some_params()[2:]}]
+    opt = train.FusedAdamW(frozen, capturable=True)
+    opt.step()
+    opt.param_groups[0]["params"][0].grad = None  # groups have counts of their own
+    opt.step()
+    assert [int(g["step_tensor"]) for g in opt.param_groups] == [1, 2]
+
+
 def test_optimizer_checkpoint_of_other_kinds(recorder):
     for saved_bits, bits in ((8, 32), (32, 8)):
         opt = train.FusedAdamW(some_params(), state_bits=saved_bits)

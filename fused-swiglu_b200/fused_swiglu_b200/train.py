@@ -160,7 +160,7 @@ class FusedAdamW(torch.optim.Optimizer):
                   (the step counts go on).  `last_grad_norm` holds [norm, factor] of the last step, on the device.
     capturable    keep learning rate and step count on the device (`group["lr_tensor"]`, `group["step_tensor"]`), so that a
                   captured `step()` can be replayed; then all parameters of a group take every step together.  Take one
-                  step before the capture.
+                  step before the capture, which is refused without this.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
@@ -229,6 +229,8 @@ class FusedAdamW(torch.optim.Optimizer):
             work += [(index, group, key, tensors) for key, tensors in kinds.items()]
         if not work:
             return loss
+        if not self.capturable and _capturing(work[0][2][0]):
+            raise RuntimeError("a captured step needs capturable=True: replays would repeat this one's count and rounding")
         if len({key[0] for _, _, key, _ in work}) > 1 and self.max_grad_norm is not None:
             raise RuntimeError("max_grad_norm needs all gradients on one device")
         scale = None

@@ -313,6 +313,22 @@ def test_optimizer_with_its_step_on_the_device_refuses_who_joins_or_skips(record
     assert [int(g["step_tensor"]) for g in opt.param_groups] == [1, 2]
 
 
+def test_optimizer_with_its_step_on_the_host_is_not_captured(recorder, monkeypatch):
+    """A replay would take the captured step's number, learning rate and random bits over and over."""
+    ps = some_params()
+    opt, other = train.FusedAdamW(ps, max_grad_norm=1.0), train.FusedAdamW(some_params(), capturable=True)
+    for o in (opt, other):
+        o.step()
+    recorder.steps.clear()
+    recorder.norms = 0
+    monkeypatch.setattr(train, "_capturing", lambda device: True)
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        opt.step()
+    assert not recorder.steps and recorder.norms == 0 and opt.state[ps[0]]["step"] == 1
+    other.step()
+    assert len(recorder.steps) == 2
+
+
 def test_optimizer_checkpoint_of_other_kinds(recorder):
     for saved_bits, bits in ((8, 32), (32, 8)):
         opt = train.FusedAdamW(some_params(), state_bits=saved_bits)

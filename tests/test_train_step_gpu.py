@@ -267,6 +267,20 @@ def test_a_first_step_is_not_captured(fsw, cuda_dev):
     assert bool((p < 1).all())
 
 
+def test_a_step_with_its_count_on_the_host_is_not_captured(fsw, cuda_dev):
+    p = torch.nn.Parameter(torch.ones(64, device=cuda_dev))
+    p.grad = torch.ones_like(p)
+    opt = fsw.train.FusedAdamW([p])
+    opt.step()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    opt.step()
+    assert opt.state[p]["step"] == 2
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_whole_training_step_from_a_captured_graph(fsw, cuda_dev, bits):
     """Two graphs of one step each, replayed in turn; both give what the eager step gives from the same state."""

@@ -291,6 +291,31 @@ def test_norm_of_rows_within_a_granule(lib, cuda_dev, d, t):
         check_backward(lib, dy, x, *want[1:], w, res, True, grads, t)
 
 
+@pytest.mark.parametrize("M,d,where", [(300, 64, "short"), (40, 1024, "wide"), (300, 4096, "wide"), (700, 5120, "wide, computed again"),
+                                       (20, 6400, "wide"), (6, 9000, "wide, computed again"), (300, 1003, "odd"), (9, 33, "odd"), (5, 12800, "any")], ids=str)
+@pytest.mark.parametrize("t", [F32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("away", [0, 100, 1000])
+def test_norm_backward_of_rows_far_off_zero(lib, cuda_dev, M, d, where, t, away):
+    """Means far above the spread.  The mean is an input, and x - mean of close fp32 values is exact: z = (x - mean) rstd is off by the
+    roundings of the difference and the product alone, 2 u |z|, however large the mean.  dx = rstd (a - c1 - z c2) + res, with sums
+    c1 and c2 over the row that are off by (d / 32 + 16) u of their magnitudes and c2 also by z's error; dw by the rows' sums."""
+    x, w, b, dy, res = norm_inputs(M, d, F32, t, cuda_dev, M + d)
+    x = (x + away * (1 if t == F32 else 0.02)).to(t)  # bf16 rows so far off have eight bits for their spread
+    dy, res = dy.to(t), res.to(t)
+    _, mean, rstd = (v.float().to(cuda_dev) for v in forward64(x, w, b, 1e-5, True))
+    got = lib.layer_norm_backward(dy, x, mean, rstd, w, True, res, fp32_grads=True)
+    dx, dw, db, z, a = backward64(dy, x, mean, rstd, w, res, True)
+    k, r = d / 32 + 16, rstd.double().cpu()[:, None]
+    c2 = (a * z).abs().mean(1, keepdim=True)
+    # u of each term for: z 2, a 1, and at most 4 more products, sums and the quotient by d on its way
+    tol = U * (6 * a.abs() + (k + 6) * a.abs().mean(1, keepdim=True) + (k + 10) * z.abs() * c2)
+    tol = tol * r + 2 * U * (dx.abs() + res.double().cpu().abs())
+    within(got[0], dx, tol + HALF[t] * dx.abs())
+    size = dy.double().cpu().abs()
+    within(got[1], dw, (M + 12) * U * (size * z.abs()).sum(0))
+    within(got[2], db, (M + 8) * U * size.sum(0))
+
+
 def test_norm_offsets_past_32_bits(lib, cuda_dev):
     """More than 2^31 elements: the last rows are what a call of those alone gives, and the others' zeros add nothing."""
     M, d, n = 530_000, 4096, 40

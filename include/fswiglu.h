@@ -225,8 +225,9 @@ int fswiglu_transpose_bf16(const void* src, int64_t ld_src, void* dst, int64_t l
 /*
  * Training operators around the MLP: norms with their gradients, AdamW over many tensors, the clipped gradient
  * norm.  No counterpart in the reference, which is forward only.  Element types are FSWIGLU_OUT_BF16 and
- * FSWIGLU_OUT_F32.  All sums, statistics and moments' arithmetic are fp32 (the gradient norm's total fp64), every
- * output is rounded once, and every result is the same from call to call: no atomics.
+ * FSWIGLU_OUT_F32.  All sums, statistics and moments' arithmetic are fp32 (the gradient norm's total fp64; of dweight
+ * and dbias the joins of the blocks' sums carry what fp32 drops), every output is rounded once, and every result is the
+ * same from call to call: no atomics.
  *
  * Unlike the MLP's entry points these take any width, pitch (ld >= d) and element-aligned base; 16-byte aligned
  * bases and pitches take wider loads.  Outputs must not overlap inputs or one another, except where a call says

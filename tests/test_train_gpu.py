@@ -316,6 +316,26 @@ def test_norm_backward_of_rows_far_off_zero(lib, cuda_dev, M, d, where, t, away)
     within(got[2], db, (M + 8) * U * size.sum(0))
 
 
+@pytest.mark.parametrize("M,d", [(120, 1024), (120, 4096), (120, 1003), (120, 12800), (8, 1024), (8, 1003), (5, 4096)])
+@pytest.mark.parametrize("gt", [F32, BF], ids=["fp32", "bf16"])
+def test_norm_vector_gradients_of_blocks_are_joined_in_64_bits(lib, cuda_dev, M, d, gt):
+    """One row a block (fewer rows than SMs, or than a cluster's blocks), whose products are exact: eight bits of dy times four of
+    z.  dy spreads over 28 powers of two, so that no order of fp32 additions is exact, and sums in 64 bits are: what is asked is
+    the exact sum, rounded once."""
+    g = torch.Generator().manual_seed(M + d)
+    x = torch.randint(-15, 16, (M, d), generator=g).float().to(cuda_dev)
+    dy = torch.ldexp(torch.randint(-255, 256, (M, d), generator=g).float(), torch.randint(0, 21, (M, d), generator=g)).to(cuda_dev)
+    mean, rstd = torch.zeros(M, device=cuda_dev), torch.full((M,), 0.5, device=cuda_dev)
+    w = torch.ones(d, dtype=gt, device=cuda_dev)
+    dw, db = (dy.double() * x.double() * 0.5).sum(0), dy.double().sum(0)
+    for got, want in zip(lib.layer_norm_backward(dy, x, mean, rstd, w, True)[1:], (dw, db)):
+        once = want.to(F32) if gt == F32 else torch.frexp(want)
+        if gt == BF:  # to nearest even at eight bits, in one step: torch goes by way of fp32
+            once = torch.ldexp(torch.round(torch.ldexp(once[0], torch.tensor(8, device=cuda_dev))), once[1] - 8).to(BF)
+        assert torch.equal(got, once)
+    assert torch.equal(lib.rms_norm_backward(dy, x, rstd, w)[1], lib.layer_norm_backward(dy, x, mean, rstd, w)[1])
+
+
 def test_norm_offsets_past_32_bits(lib, cuda_dev):
     """More than 2^31 elements: the last rows are what a call of those alone gives, and the others' zeros add nothing."""
     M, d, n = 530_000, 4096, 40

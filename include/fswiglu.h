@@ -310,8 +310,9 @@ int fswiglu_adamw_step(const fswiglu_adamw_tensor* tensors, int64_t count, int p
 /*
  * out[0] = the 2-norm over all elements of `count` gradients, out[1] = min(1, max_norm / (out[0] + 1e-6)): the
  * grad_scale that clips them, without a copy to the host.  Where the norm is not finite out[1] is NaN, which makes
- * fswiglu_adamw_step skip the step.  Squares are summed in fp32 over the elements that one thread reads of a chunk,
- * in fp64 from there; an element above 1.8e19 makes the norm infinite.  Types may differ from gradient to gradient.
+ * fswiglu_adamw_step skip the step.  Squares are summed in fp32 over 16 elements that one thread reads of a chunk, in
+ * fp64 from there; an element above 1.8e19, or 16 whose squares together pass fp32's largest value, makes the norm
+ * infinite.  Down to the smallest values nothing is lost.  Types may differ from gradient to gradient.
  * The workspace is 256-byte aligned; calls that may overlap need one each.
  */
 typedef struct fswiglu_grad_tensor {

@@ -948,3 +948,24 @@ def test_grad_norm_of_few_and_many_chunks(lib, cuda_dev):
         assert abs(float(out[0]) - want) <= (17 / 2 + 1) * U * want
         factor = min(1.0, 0.5 / (want + 1e-6))
         assert abs(float(out[1]) - factor) <= (17 / 2 + 2) * U * factor
+
+
+@pytest.mark.parametrize("t", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n", [9, 5000, 400_003])
+def test_grad_norm_of_values_whose_squares_leave_fp32(lib, cuda_dev, n, t):
+    """Down to the smallest fp32 values: sixteen squares are summed in fp32, scaled by a power of two where they are below its
+    normal numbers, which adds no rounding: (17 / 2 + 1) u as elsewhere.  The norm is an fp32 value: half a unit more, in absolute
+    terms, below the smallest normal one."""
+    g = torch.Generator().manual_seed(n)
+    values = torch.randn(n, generator=g)
+    for size in (1e-18, 1e-20, 3e-23, 1e-25, 1e-32, 1e-38, 1e-41, 0.0):
+        for mixed in (False, True):
+            v = (values * size).to(t)
+            if mixed:
+                v[:: 7919 if n > 9 else 4] = 1e-14
+            want = math.sqrt(float(v.double().square().sum()))
+            for grads in ([v], [v[: n // 2].clone(), v[n // 2:].clone()]):
+                out = lib.grad_norm_clip([q.to(cuda_dev) for q in grads], 1e-30)
+                assert abs(float(out[0]) - want) <= (17 / 2 + 1) * U * want + 2.0 ** -150, (size, mixed, float(out[0]), want)
+                factor = min(1.0, 1e-30 / (want + 1e-6))
+                assert abs(float(out[1]) - factor) <= (17 / 2 + 3) * U * factor

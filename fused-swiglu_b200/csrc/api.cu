@@ -197,13 +197,19 @@ int prepare_device(int dev, int* num_sms) {
 }
 
 // A thread whose first CUDA call this is (autograd's, say) has no context yet, without which tensor maps cannot be encoded:
-// launches and copies would bind one, the driver's entry points do not.
+// launches and copies would bind one, the driver's entry points do not.  A context that the thread has, the host's own say, is
+// left in place; asked anew by every call, since a host may take it away again.
 int bind_context(int dev) {
-  thread_local int bound = -1;
-  if (bound == dev) return FSWIGLU_OK;
-  if (cudaSetDevice(dev) != cudaSuccess) return FSWIGLU_ERR_NO_DEVICE;
-  bound = dev;
-  return FSWIGLU_OK;
+  static const auto current = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &q) != cudaSuccess) fn = nullptr;
+    return reinterpret_cast<CUresult (*)(CUcontext*)>(fn);
+  }();
+  if (current == nullptr) return FSWIGLU_ERR_NO_DEVICE;
+  CUcontext context = nullptr;
+  if (current(&context) == CUDA_SUCCESS && context != nullptr) return FSWIGLU_OK;
+  return cudaSetDevice(dev) == cudaSuccess ? FSWIGLU_OK : FSWIGLU_ERR_NO_DEVICE;
 }
 
 // One-time per-device set-up of the ordinary entry points: the above plus the 256-byte status block.

@@ -606,3 +606,41 @@ def test_norms_read_the_vectors_that_a_step_has_just_written(fsw, cuda_dev, M, d
         got = steps(lambda: None)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not torch.equal(want[0], want[5])  # the vectors do move
+
+
+def test_a_thread_keeps_its_context_and_gets_one_when_it_has_none(fsw, cuda_dev):
+    """Calls that launch nothing, on a thread with a context of its own making, then without any."""
+    import ctypes
+    import threading
+
+    cu = ctypes.CDLL("libcuda.so.1")
+    zero = ctypes.c_void_p(0)
+    seen = []
+
+    def call():  # no rows and no gradients of vectors: the device is looked up, nothing is launched
+        return fsw.capi.lib.fswiglu_rms_norm_backward(zero, 8, zero, 8, zero, zero, zero, 0, zero, 8, zero, 0, 8, 1, 1, 1, zero, 0, zero)
+
+    def current():
+        c = ctypes.c_void_p()
+        assert cu.cuCtxGetCurrent(ctypes.byref(c)) == 0
+        return c.value
+
+    def work():
+        try:
+            own, primary = ctypes.c_void_p(), ctypes.c_void_p()
+            assert cu.cuCtxCreate_v2(ctypes.byref(own), 0, 0) == 0 and current() == own.value
+            seen.append(call() == 0 and call() == 0 and current() == own.value)
+            for _ in range(2):
+                assert cu.cuCtxSetCurrent(None) == 0 and current() is None
+                seen.append(call() == 0 and current() not in (None, own.value))
+            assert cu.cuDevicePrimaryCtxRetain(ctypes.byref(primary), 0) == 0
+            seen.append(current() == primary.value)
+            assert cu.cuDevicePrimaryCtxRelease_v2(0) == 0 and cu.cuCtxDestroy_v2(own) == 0
+        except BaseException as e:  # noqa: BLE001
+            seen.append(e)
+
+    assert call() == 0
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert seen == [True] * 4, seen

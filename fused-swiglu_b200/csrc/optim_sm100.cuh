@@ -134,20 +134,21 @@ __device__ __forceinline__ void decode_e5m2x8(uint2 q, Pair (&v)[4]) {
 }
 
 // How a block whose largest magnitude has the fp32 bits `peak` is encoded: its scale, the power of two that brings its values
-// to where the exponents of the 8-bit type, its subnormal ones too, are those of fp32, and whether they have to come down by
-// 2^-100 first, so that this power is a normal number.  `top`: the type's exponent that the largest value gets; `low`: the
-// difference of the types' biases.
+// to where the exponents of the 8-bit type, its subnormal ones too, are those of fp32, and what they have to come down by
+// first, so that this power is a normal number: 2^-100 where the largest is above 2^14 or so, 2^-114 from 2^114 on (m alone), which
+// the smaller values next to it have room for.  `top`: the type's exponent that the largest value gets; `low`: the difference
+// of the types' biases.
 struct BlockScale {
-  float scale, factor;
-  bool down;
+  float scale, factor, down;
 };
 __device__ __forceinline__ BlockScale block_scale(uint32_t peak, int top, int low) {
   const int field = max(static_cast<int>(peak >> 23), top + 1);  // keeps the scale normal
   BlockScale b;
   b.scale = field < 255 ? __uint_as_float(static_cast<uint32_t>(field - top) << 23) : __uint_as_float(0x7fc00000u);
   const int exponent = 254 + top - low - field;
-  b.down = exponent < 1;
-  b.factor = __uint_as_float(static_cast<uint32_t>(b.down ? exponent + 100 : exponent) << 23);
+  const int by = exponent >= 1 ? 0 : exponent >= -99 ? 100 : 114;
+  b.down = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
+  b.factor = __uint_as_float(static_cast<uint32_t>(exponent + by) << 23);
   return b;
 }
 
@@ -553,11 +554,12 @@ __global__ void __launch_bounds__(kRing ? kAdam8RingThreads : kAdamThreads, kRin
     const unsigned long long group = (t.first_block[k] + block) * (kAdamBlock / kAdamGroup) + lane;
     const uint32_t h = mix32(static_cast<uint32_t>(group) ^ (static_cast<uint32_t>(group >> 32) * odd_multiplier(0)) ^ r.key);
     const Pair fm = both(bm.factor), fv = both(bv.factor);
-    if (bm.down || bv.down) {
+    if (fminf(bm.down, bv.down) < 1.0f) {
+      const Pair down_m = both(bm.down), down_v = both(bv.down);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (bm.down) q.m[i] = q.m[i] * both(0x1p-100f);
-        if (bv.down) q.v[i] = q.v[i] * both(0x1p-100f);
+        q.m[i] = q.m[i] * down_m;
+        q.v[i] = q.v[i] * down_v;
       }
     }
     uint32_t cm[kAdamGroup], cv[kAdamGroup];

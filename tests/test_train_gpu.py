@@ -749,6 +749,36 @@ def test_adamw_8bit_extremes(lib, cuda_dev):
         assert bool((new["v"].float().cpu()[positive] > 0).all())
 
 
+@pytest.mark.parametrize("count", [1, 3000])  # one wave of blocks, and the ring
+def test_adamw_8bit_first_moments_up_to_the_largest(lib, cuda_dev, count):
+    """First moments of every size up to fp32's largest, small ones beside them: the rounding of the formula's fp32 value, exactly."""
+    powers = torch.arange(-20, 120, 4)
+    n = 256 * len(powers) * count
+    g = torch.Generator().manual_seed(count)
+    scales = torch.exp2(powers.float()).repeat(count)
+    codes = torch.randn(n, generator=g).clamp(-3.5, 3.5) * 2.0 ** torch.randint(-6, 7, (n,), generator=g)
+    codes[::256] = 255.0  # each block's largest, which a stochastic rounding takes up or down
+    t = {"p": torch.zeros(n), "g": torch.randn(n, generator=g), "m": codes.to(torch.float8_e4m3fn), "ms": scales,
+         "v": torch.full((n,), 2.0 ** 14).to(torch.float8_e5m2), "vs": torch.ones(n // 256)}
+    tensors = [{k: v.to(cuda_dev) for k, v in t.items()}]
+    before = snapshot(tensors)
+    take_step(lib, tensors, step=5)
+    new = tensors[0]
+    m32 = torch.tensor(0.9, dtype=F32) * decoded(before[0]["m"], before[0]["ms"]).float() + torch.tensor(0.1, dtype=F32) * t["g"]
+    q, s = encode(m32.abs(), random_bits(n, 0, 11, 5) & 0xFFFF, 7, 3, 7, False)
+    assert torch.equal(new["ms"].double().cpu(), s)
+    got, want = new["m"].double().cpu(), q * torch.where(torch.signbit(m32), -1.0, 1.0).double()
+    # Below the 8-bit type's normal numbers, 2^-6 of the scale, the kernel's scaled value is an fp32 subnormal: its last bit is
+    # 2^(-149 + 120) = 2^-29 of the scale, 2^-20 of the unit 2^-9 there, so that the product that scales it is off by 2^-21 of a
+    # unit at most.  Where value and random bits together come so close to a whole unit they may go either way.
+    units = m32.double().abs() / s.repeat_interleave(256) * 512
+    near = units + (random_bits(n, 0, 11, 5) & 0xFFFF).double() / 65536
+    either = (units < 8) & ((near - near.round()).abs() <= 2.0 ** -21)
+    bad = ((got != want) & ~either).nonzero().flatten()
+    assert not len(bad), (len(bad), float(m32[bad[0]]), float(got[bad[0]]), float(want[bad[0]]))
+    assert bool(((got - want).abs() <= 2.0 ** -9)[either].all()) and int(either.sum()) < n // 2 ** 16 + 2
+
+
 def test_adamw_8bit_rounding_is_right_on_average(lib, cuda_dev):
     """65536 equal values between two units: the mean is that value, to five times the standard error of a mean of
     independent roundings (at most half a unit each) and the 2^-16 that sixteen bits resolve."""

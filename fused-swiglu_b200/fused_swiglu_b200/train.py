@@ -179,6 +179,11 @@ class FusedAdamW(torch.optim.Optimizer):
         self.seed, self.capturable = seed, capturable
         self.last_grad_norm = None
 
+    def __getstate__(self) -> dict:
+        """As the base class's, which would leave a copy or a pickled optimiser without what is set above."""
+        mine = ("state_bits", "master", "max_grad_norm", "seed", "capturable", "last_grad_norm")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in mine}}
+
     def _init_state(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         master = self.master and p.dtype == torch.bfloat16

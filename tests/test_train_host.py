@@ -345,6 +345,34 @@ def test_optimizer_checkpoint_of_other_kinds(recorder):
         assert [len(s["masters"]) for s in recorder.steps] == [2 if master else 0, 0]
 
 
+@pytest.mark.parametrize("how", ["deepcopy", "save", "copy"])
+def test_optimizer_copies_are_whole(recorder, how):
+    import copy
+    import io
+
+    ps = some_params()
+    opt = train.FusedAdamW(ps, lr=0.5, state_bits=8, master=False, max_grad_norm=2.0, seed=9)
+    opt.step()
+    if how == "save":
+        file = io.BytesIO()
+        torch.save(opt, file)
+        file.seek(0)
+        other = torch.load(file, weights_only=False)
+    else:
+        other = getattr(copy, how)(opt)
+    for p in other.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    recorder.steps.clear()
+    opt.step()
+    wanted = recorder.steps[:]
+    other.step()
+    got = recorder.steps[len(wanted):]
+    late = 1 if how == "copy" else 0  # which shares the state
+    assert [(s["step"] + late, s["seed"], len(s["ms"]), len(s["masters"]), s["lr"]) for s in wanted] == \
+        [(s["step"], s["seed"], len(s["ms"]), len(s["masters"]), s["lr"]) for s in got]
+    assert recorder.norms == 3 and (other.state_bits, other.capturable) == (8, False)
+
+
 def test_optimizer_refusals(recorder):
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(state_bits=16),
                 dict(max_grad_norm=-1.0), dict(lr=NAN)):

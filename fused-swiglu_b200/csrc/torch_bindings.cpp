@@ -25,9 +25,16 @@ void check_status(int rc, const char* where) {
   TORCH_CHECK(rc == FSWIGLU_OK, where, ": ", fswiglu_status_string(rc), " (status ", rc, ")");
 }
 
+// A fake tensor says that it is a CUDA tensor, and as its address gives its offset from nothing.
+void check_data(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), name,
+              " has no data: traced tensors go through torch.ops.ASMLLM");
+}
+
 void check_bf16_cuda(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be a bfloat16 tensor");
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  check_data(t, name);
 }
 
 int64_t row_pitch(const at::Tensor& t, const char* name) {
@@ -207,6 +214,7 @@ int64_t norm_rows(const at::Tensor& t, const char* name, const at::Tensor& x) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == 2 && t.sizes() == x.sizes(), name, " must be 2-D, of the shape of x");
   TORCH_CHECK(t.scalar_type() == x.scalar_type() && t.device() == x.device(), name, " must have the type and device of x");
+  check_data(t, name);
   return row_pitch(t, name);
 }
 
@@ -214,6 +222,7 @@ const void* norm_vector(const std::optional<at::Tensor>& v, const char* name, co
   if (!v.has_value() || !v->defined()) return nullptr;
   TORCH_CHECK(v->dim() == 1 && v->size(0) == x.size(1) && v->is_contiguous() && v->device() == x.device(), name,
               " must be a contiguous vector of x's row length on the device of x");
+  check_data(*v, name);
   return v->data_ptr();
 }
 
@@ -227,6 +236,7 @@ const float* norm_statistic(const at::Tensor& t, const char* name, const at::Ten
   TORCH_CHECK(t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 1 && t.size(0) == x.size(0) &&
                   t.is_contiguous(),
               name, " must be a contiguous float32 vector with one entry per row of x, on the device of x");
+  check_data(t, name);
   return t.data_ptr<float>();
 }
 
@@ -359,6 +369,7 @@ void check_list(const Refs& list, const Refs& params, at::ScalarType type, const
     TORCH_CHECK(t->scalar_type() == type, name, " must all be ", type, " tensors");
     TORCH_CHECK(t->device() == device, name, " must all be on the device of the parameters");
     TORCH_CHECK(t->is_contiguous(), name, " must all be contiguous");
+    check_data(*t, name);
   }
 }
 
@@ -366,6 +377,7 @@ const void* scalar_on_device(const std::optional<at::Tensor>& t, at::ScalarType 
   if (!t.has_value() || !t->defined()) return nullptr;
   TORCH_CHECK(t->scalar_type() == type && t->numel() == 1 && t->device() == p.device(), name, " must be one ", type,
               " element on the device of the parameters");
+  check_data(*t, name);
   return t->data_ptr();
 }
 
@@ -443,6 +455,7 @@ at::Tensor grad_norm_clip_refs(const Refs& grads, double max_norm) {
     const at::Tensor& g = *grads[i];
     TORCH_CHECK(g.is_cuda() && g.device() == g0.device(), "grads must all be CUDA tensors of one device");
     TORCH_CHECK(g.is_contiguous(), "grads must all be contiguous");
+    check_data(g, "grads");
     table[i] = {g.data_ptr(), g.numel(), element_type(g, "grads")};
   }
   const c10::cuda::OptionalCUDAGuard guard(device_of(g0));

@@ -162,6 +162,25 @@ def test_operators_refuse_host_tensors():
             call()
 
 
+def test_operators_refuse_tensors_without_data():
+    """A fake tensor calls itself a CUDA tensor, and its address is its offset from nothing: a view's would reach the GPU."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import fused_mlp_module as lib
+
+    with FakeTensorMode():
+        bf = dict(dtype=torch.bfloat16, device="cuda")
+        x, s, w, mats = torch.empty((6, 64), **bf)[1:], torch.empty(9, device="cuda")[4:], torch.empty(72, **bf)[8:], torch.empty((65, 64), **bf)[1:]
+        f = torch.empty((6, 64), device="cuda")[1:]
+        for call in (lambda: lib.layer_norm_forward(x, w, w), lambda: lib.rms_norm_forward(x),
+                     lambda: lib.layer_norm_backward(x, x, s, s, w), lambda: lib.rms_norm_backward(x, x, s),
+                     lambda: lib.adamw_step([x], [x], [f], [f], 1, 1e-3), lambda: lib.grad_norm_clip([f, x], 1.0),
+                     lambda: lib.rms_scale(x), lambda: lib.fused_swiglu_mlp_bf16(x, mats, mats, mats),
+                     lambda: lib.swiglu_down_bf16(x, mats), lambda: lib.fused_swiglu_bf16(x, mats)):
+            with pytest.raises(RuntimeError, match="has no data"):
+                call()
+
+
 def test_shapes_without_data():
     import fused_mlp_module  # noqa: F401
 

@@ -9,6 +9,9 @@ gradients, the clipped gradient norm, AdamW over many tensors at once.
 The reference is forward only (csrc/torch_bindings.cpp:38-50).  The raw operators are functions of the torch extension
 `fused_mlp_module` (and `torch.ops.ASMLLM`); the arithmetic is in libfswiglu.so, without a CPU path.
 
+`layer_norm` and `rms_norm` can be traced (fake tensors, torch.compile); the block, the clipped norm and the optimiser run as they
+are, outside of traced graphs.  vmap, forward-mode and second derivatives are refused.
+
 Capturing a backward pass into a CUDA graph: as with every autograd function, no graph of an earlier eager pass over the
 same leaves may be alive then (drop its outputs first, and let the warm-up pass run on the capturing stream).
 """
@@ -24,6 +27,17 @@ def _lib():
     import fused_mlp_module
 
     return fused_mlp_module
+
+
+def _traced(x: torch.Tensor) -> bool:
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or type(x) not in (torch.Tensor, torch.nn.Parameter))
+
+
+def _norms(x: torch.Tensor):
+    """The module's functions; where x is traced or has shapes alone, the dispatcher's ops, which have forms for that."""
+    lib = _lib()  # registers the ops
+    return torch.ops.ASMLLM if _traced(x) or x.device.type == "meta" else lib
 
 
 def _rows(x: torch.Tensor, d: int) -> torch.Tensor:
@@ -42,7 +56,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         x2 = _rows(x, x.size(-1))
-        y, mean, rstd = _lib().layer_norm_forward(x2, weight, bias, eps)
+        y, mean, rstd = _norms(x2).layer_norm_forward(x2, weight, bias, eps)
         ctx.save_for_backward(x2, weight, mean, rstd)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y.view(x.shape)
@@ -54,8 +68,8 @@ class _LayerNorm(torch.autograd.Function):
         need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         # vectors' gradients have the weight's type; a bias alone says by itself
         fp32 = weight is None and ctx.bias_dtype == torch.float32
-        dx, dw, db = _lib().layer_norm_backward(_rows(dout, x2.size(1)), x2, mean, rstd, weight, need_b,
-                                                fp32_grads=fp32, weight_grad=need_w)
+        dx, dw, db = _norms(x2).layer_norm_backward(_rows(dout, x2.size(1)), x2, mean, rstd, weight, need_b,
+                                                    fp32_grads=fp32, weight_grad=need_w)
         return dx.view(dout.shape), dw, None if db is None else db.to(ctx.bias_dtype), None
 
 
@@ -63,7 +77,7 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
         x2 = _rows(x, x.size(-1))
-        y, rstd = _lib().rms_norm_forward(x2, weight, eps)
+        y, rstd = _norms(x2).rms_norm_forward(x2, weight, eps)
         ctx.save_for_backward(x2, weight, rstd)
         return y.view(x.shape)
 
@@ -71,8 +85,8 @@ class _RMSNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         x2, weight, rstd = ctx.saved_tensors
-        dx, dw = _lib().rms_norm_backward(_rows(dout, x2.size(1)), x2, rstd, weight,
-                                          weight_grad=ctx.needs_input_grad[1])
+        dx, dw = _norms(x2).rms_norm_backward(_rows(dout, x2.size(1)), x2, rstd, weight,
+                                              weight_grad=ctx.needs_input_grad[1])
         return dx.view(dout.shape), dw, None
 
 
@@ -131,7 +145,18 @@ def norm_swiglu_block(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: tor
     for name, t in (("norm_weight", norm_weight), ("norm_bias", norm_bias)):
         if t is not None and t.dtype != torch.bfloat16:
             raise RuntimeError(f"{name} must be a bfloat16 tensor, got {t.dtype}")
-    return _NormSwiGLUBlock.apply(x, norm_weight, norm_bias, W_gate, W_up, W_down, eps, norm == "layer")
+    args = (x, norm_weight, norm_bias, W_gate, W_up, W_down, eps, norm == "layer")
+    if torch.compiler.is_compiling():
+        return _block_as_it_is(*args)
+    if _traced(x):
+        raise RuntimeError("norm_swiglu_block cannot be traced: its backward pass has no shape-only form")
+    return _NormSwiGLUBlock.apply(*args)
+
+
+@torch.compiler.disable
+def _block_as_it_is(*args) -> torch.Tensor:
+    """Where torch.compile leaves its graph."""
+    return _NormSwiGLUBlock.apply(*args)
 
 
 def clip_grad_norm(grads, max_norm: float) -> torch.Tensor:
@@ -209,6 +234,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if _capturing(device):
             raise RuntimeError("take one step before the capture: a captured one would start from zero each time")
 
+    @torch.compiler.disable  # lists, dictionaries and kernels that write through pointers: torch.compile leaves its graph here
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -198,6 +198,31 @@ def test_shapes_without_data():
     assert o.adamw_step([w], [w], [w], [w], 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, [], [], []) is None
 
 
+def test_norms_can_be_traced():
+    """Shapes under fake tensors and on the meta device, both passes, and torch.compile without a graph break: on a CPU-only machine
+    the captured graph fails at run time, with the dispatcher's missing CPU kernel and nothing else."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty((3, 9, 64), dtype=torch.bfloat16, device="cuda")[:, 1:]
+        w = torch.empty(64, device="cuda")
+        for y in (train.rms_norm(x, w), train.layer_norm(x, w, w), train.layer_norm(x)):
+            assert y.shape == x.shape and y.dtype == x.dtype and y.device.type == "cuda"
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            train.norm_swiglu_block(x, None, None, x[0], x[0], x[0])
+    x, w = torch.empty((3, 8, 64), device="meta", requires_grad=True), torch.empty(64, device="meta", requires_grad=True)
+    train.layer_norm(train.rms_norm(x, w), w, w).sum().backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
+    if torch.cuda.is_available():
+        pytest.skip("compiled with real tensors by the GPU suite")
+    x, w = torch.zeros((2, 3, 64), requires_grad=True), torch.ones(64, requires_grad=True)
+    for call in (lambda: torch.compile(train.rms_norm, fullgraph=True, backend="aot_eager")(x, w),
+                 lambda: torch.compile(train.layer_norm, fullgraph=True, backend="aot_eager")(x, w, w)):
+        torch._dynamo.reset()
+        with pytest.raises(NotImplementedError, match="'CPU' backend"):
+            call()
+
+
 # ---------------------------------------------------------------- the optimiser, with the operators recorded
 
 class Recorder:

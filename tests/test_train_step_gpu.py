@@ -644,3 +644,59 @@ def test_a_thread_keeps_its_context_and_gets_one_when_it_has_none(fsw, cuda_dev)
     t.start()
     t.join()
     assert seen == [True] * 4, seen
+
+
+def test_compiled_norms_and_a_block_between_compiled_parts(fsw, cuda_dev):
+    """The norms inside a compiled function without a graph break, the block where torch.compile leaves its graph: the bits of the
+    eager calls, forward and backward."""
+    from fused_swiglu_b200.module import NormSwiGLUBlock
+
+    g = torch.Generator().manual_seed(0)
+    start = [torch.randn(s, generator=g).to(BF).to(cuda_dev) for s in ((5, 8, 64), (64,), (64,))]
+
+    def norms(x, w, b):
+        return fsw.train.layer_norm(fsw.train.rms_norm(x, w), w, b)
+
+    def both_passes(f):
+        leaves = [t.clone().requires_grad_() for t in start]
+        y = f(*leaves)
+        y.backward(start[0])
+        return [y.detach()] + [t.grad for t in leaves]
+
+    torch._dynamo.reset()
+    want = both_passes(norms)
+    for a, b in zip(both_passes(torch.compile(norms, fullgraph=True, backend="aot_eager")), want):
+        assert torch.equal(a, b)
+    block = NormSwiGLUBlock(64, 128, device=cuda_dev)
+    with torch.no_grad():
+        for p in block.mlp.parameters():
+            p.copy_(torch.randn(p.shape, generator=g))
+
+    def model(x):
+        return block(x * 2) + 1
+
+    def both_passes_of_block(f):
+        block.zero_grad()
+        x = start[0].clone().requires_grad_()
+        y = f(x)
+        y.backward(start[0])
+        return [y.detach(), x.grad] + [p.grad.clone() for p in block.parameters()]
+
+    want = both_passes_of_block(model)
+    for a, b in zip(both_passes_of_block(torch.compile(model, backend="aot_eager")), want):
+        assert torch.equal(a, b)
+    opt = fsw.train.FusedAdamW(block.parameters(), max_grad_norm=1.0)
+
+    @torch.compile(backend="aot_eager")
+    def whole_step(x):
+        opt.zero_grad()
+        y = model(x)
+        y.float().square().mean().backward()
+        opt.step()
+        return fsw.train.clip_grad_norm([p.grad for p in block.parameters()], 1.0)
+
+    before = [p.detach().clone() for p in block.parameters()]
+    assert float(whole_step(start[0])[0]) > 0 and float(whole_step(start[0])[0]) > 0
+    assert all(not torch.equal(p, q) for p, q in zip(block.parameters(), before))
+    assert all(s["step"] == 2 for s in opt.state.values())
+    torch._dynamo.reset()

@@ -25,8 +25,11 @@ void check_status(int rc, const char* where) {
   TORCH_CHECK(rc == FSWIGLU_OK, where, ": ", fswiglu_status_string(rc), " (status ", rc, ")");
 }
 
-// A fake tensor says that it is a CUDA tensor, and as its address gives its offset from nothing.
+// A fake tensor says that it is a CUDA tensor, and as its address gives its offset from nothing.  Plain tensors are told by their
+// keys: calls over many small ones pass here for each.
 void check_data(const at::Tensor& t, const char* name) {
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::Functionalize});
+  if (C10_LIKELY(!t.key_set().has_any(wrapped))) return;
   TORCH_CHECK(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), name,
               " has no data: traced tensors go through torch.ops.ASMLLM");
 }

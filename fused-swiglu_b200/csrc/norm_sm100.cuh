@@ -40,6 +40,7 @@ struct RingParams {
   unsigned long long wait_limit_ns;
   int places;
   int withhold;  // test aid: the first row of all is never copied
+  int edge;      // rows that start anywhere: edge_rows
 };
 
 struct NormForwardParams {
@@ -815,13 +816,12 @@ __global__ void __launch_bounds__(kOddThreads, 2) norm_forward_odd_kernel(const 
   __syncthreads();
   grid_launch_dependents();
   grid_dependency_wait();
-  const int edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   auto source = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   int asked = 0;  // of the group's first thread
   auto ask = [&](int place, int n) {
     const T* const src[1] = {source(n)};
     const int r = row + n * stride;
-    const bool first = r < edge, last = r >= p.M - edge;
+    const bool first = r < p.ring.edge, last = r >= p.M - p.ring.edge;
     if (!first && !last) asked += ring.ask_granules(place, src, 1);
     else asked += ring.ask_edge(place, src[0], src[0], src[0], 1, p.d, first, last, p.ring.withhold && r == 0);
   };
@@ -898,7 +898,6 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
   __syncthreads();
   grid_launch_dependents();
   grid_dependency_wait();
-  const int edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   auto x_of = [&](int n) { return static_cast<const T*>(p.x) + (row + n * stride) * p.ldx; };
   auto dy_of = [&](int n) { return static_cast<const T*>(p.dout) + (row + n * stride) * p.ld_dout; };
   auto res_of = [&](int n) { return static_cast<const T*>(p.residual) + (residual ? (row + n * stride) * p.ld_res : 0); };
@@ -907,7 +906,7 @@ __global__ void __launch_bounds__(kOddThreads) norm_backward_odd_kernel(const No
     const T* const src[3] = {x_of(n), dy_of(n), res_of(n)};
     const int r = row + n * stride;
     const int arrays = residual ? 3 : 2;
-    const bool first = r < edge, last = r >= p.M - edge;
+    const bool first = r < p.ring.edge, last = r >= p.M - p.ring.edge;
     if (!first && !last) asked += ring.ask_granules(place, src, arrays);
     else asked += ring.ask_edge(place, src[0], src[1], src[2], arrays, p.d, first, last, p.ring.withhold && r == 0);
   };

@@ -199,6 +199,7 @@ int launch_norm_forward_odd(NormForwardParams& p, WidePlan w, const Device& dev,
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
   const int64_t resident = dev.sms * fill_sm(kernel, &known, w);
   p.ring.places = w.places;
+  p.ring.edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   p.ring.withhold = take_withhold();
   return launch(kernel, std::min(blocks, resident), dim3(w.group, w.groups), w.ring(), s, p);
 }
@@ -261,6 +262,7 @@ int launch_norm_backward_odd(NormBackwardParams& p, const WidePlan& w, const Dev
   const int64_t blocks = (static_cast<int64_t>(p.M) + w.groups - 1) / w.groups;
   p.splits = backward_splits(p, blocks, dev.sms);
   p.ring.places = w.places;
+  p.ring.edge = edge_rows(p.d * static_cast<int>(sizeof(T)));
   p.ring.withhold = take_withhold();
   return launch_backward(kernel, dim3(w.group, w.groups), w.ring(), s, p);
 }
@@ -382,7 +384,7 @@ int norm_forward(bool layer, const void* x, int64_t ldx, const void* weight, con
   p.ldy = ldy;
   p.M = static_cast<int>(M);
   p.d = static_cast<int>(d);
-  p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0};
+  p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0, 1};
   p.w_f32 = w_dtype == FSWIGLU_OUT_F32 && (weight != nullptr || bias != nullptr);
   p.eps = eps;
   // fp32 vectors are read where they are: one without the other goes the odd way
@@ -440,7 +442,7 @@ int norm_backward(bool layer, const void* dout, int64_t ld_dout, const void* x, 
     p.M = static_cast<int>(M);
     p.d = static_cast<int>(d);
     p.splits = norm_splits(M);
-    p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0};
+    p.ring = RingParams{dev.status, dev.wait_limit_ns, 0, 0, 1};
     p.w_f32 = w_dtype == FSWIGLU_OUT_F32 && weight != nullptr;
     const bool wide = d * type_bytes(x_dtype) % 16 == 0 && wide_rows(dout, ld_dout, M, x_dtype) && wide_rows(x, ldx, M, x_dtype) &&
                       wide_rows(dx, ld_dx, M, x_dtype) && wide_rows(residual, residual == nullptr ? 0 : ld_res, M, x_dtype) &&

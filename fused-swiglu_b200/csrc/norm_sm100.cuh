@@ -10,8 +10,8 @@
 //
 // Memory bound: forward reads and writes a row once, backward reads two or three and writes one, at 8 to 15 operations an
 // element.  The variance is that of the centred values, from a second sum over the row as it lies on the SM.  Four forms:
-//   short   rows of at most 32 vectors of 16 bytes: a part of a warp a row (200000 x 128 bf16, layer norm: forward 23 us, against
-//           63 of the wide form; backward 49 against 109)
+//   short   rows of at most 32 vectors of 16 bytes: a part of a warp a row (200000 x 128 bf16, layer norm: forward 21 to 23 us,
+//           against 63 of the wide form; backward 51 against 109)
 //   wide    rows of whole 16-byte vectors up to 16384 columns (backward: 12288 bf16, 9216 fp32): rings of shared memory filled by
 //           bulk copies
 //   odd     other rows up to 8192 columns: the same rings, by the 16-byte granules that a row touches, element by element
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(wide_forward_threads(N * kPerVector<T>)) norm_
 // dx, and the block's part of the sums over rows: a thread keeps them for its columns over all its rows, the groups of a
 // block are joined in the ring's memory at the end, and the blocks by norm_reduce_kernel.
 // Bound by memory: RMS norm with a residual, 32414 x 5120 bf16, 200 to 217 us, 6.1 to 6.6 TB/s; layer norm, whose second sum takes as many
-// registers again, 16384 x 4096 86 us, 6.3 TB/s, and 32414 x 5120 207 us, 6.4 TB/s.  kAgain: a row's z and a are not kept over its reduction but computed
+// registers again, 16384 x 4096 87 us, 6.2 TB/s, and 32414 x 5120 207 to 217 us, 6.1 to 6.4 TB/s.  kAgain: a row's z and a are not kept over its reduction but computed
 // again from shared memory, which frees their registers.
 template <typename T, typename W, bool kLayer, int N, bool kAgain>
 __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgain)) norm_backward_wide_kernel(const NormBackwardParams p) {
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(wide_backward_threads(N * kPerVector<T>, kAgai
 //
 // The same rings for rows that are not whole granules of 16 bytes, or not all on granules' starts.  A thread takes every
 // blockDim.x-th column, element by element, so that neighbours still read and write next to one another.  Bound by the
-// instructions on single elements: layer norm of 16000 x 4097 bf16, forward 152 us, backward 283 us (1.7 and 1.9 TB/s; row by row from
+// instructions on single elements: layer norm of 16000 x 4097 bf16, forward 154 us, backward 273 us (1.7 and 1.9 TB/s; row by row from
 // memory, without a ring, 258 and 366); 16000 x 1003 fp32, backward 50 us, 5.2 TB/s.
 
 constexpr int kOddThreads = 512;  // most threads of a block
@@ -1174,7 +1174,7 @@ __global__ void __launch_bounds__(kShortThreads) norm_backward_short_kernel(cons
 
 // Joins the splits' sums: 32 columns a block, whose 32 rows of threads take every 32nd split, five at a time on their way, and
 // whose first rows join theirs.  The order is fixed.  Its blocks come up while the backward kernel ends (148 splits of 4096
-// columns: 2 us of the pass's 28).
+// columns: 2 us of the pass's 29).
 constexpr int kNormReduceRows = 32;
 template <bool kBias>
 __global__ void __launch_bounds__(32 * kNormReduceRows) norm_reduce_kernel(const NormReduceParams p) {

@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw32_kernel(const __grid_c
 // There is nearly as much to compute as to move, and a warp that waits for its loads does not compute: a part's values come
 // by bulk copies into a ring of shared memory, asked for by a warp of their own while the eight others work on earlier
 // parts.  A part at a tensor's end, or of a tensor whose pointers are not aligned, is loaded by its threads.
-// 3 x 45 M bf16 weights with fp32 copies, 16 bytes an element: 351 us, 6.2 TB/s, 59 instructions an element on 68 % of the issue
+// 3 x 45 M bf16 weights with fp32 copies, 16 bytes an element: 351 to 367 us, 5.9 to 6.2 TB/s, 59 instructions an element on 68 % of the issue
 // slots; with each warp loading its own values 467 us.  Places and blocks an SM: three of two 356 us, two of three 360, four of
 // two 368, three of three 386.
 
@@ -611,8 +611,8 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 }
 
 // Squares of this thread's elements of kParts parts of a chunk from part `first` on, all loaded before the first is used: in
-// fp32 over two parts, sixteen elements, in fp64 from there on.  (3 x 45 M fp32 gradients 82 us, 6.6 TB/s, bound by memory; 224 of
-// 65 k bf16, from the L2 cache, 10.6 us, most of it the two launches' and each block's search for its tensors.)
+// fp32 over two parts, sixteen elements, in fp64 from there on.  (3 x 45 M fp32 gradients 80 us, 6.8 TB/s, bound by memory; 224 of
+// 65 k bf16, from the L2 cache, 10.5 to 11.5 us, most of it the two launches' and each block's search for its tensors.)
 template <int kParts, bool kScaled, typename T>
 __device__ __forceinline__ double sum_squares(const T* p, bool vector, int size, int first, float& least) {
   RawGroup<T> raw[kParts];
@@ -646,7 +646,7 @@ __device__ __forceinline__ double sum_squares(const T* p, bool vector, int size,
 // The same for sums that may have lost squares below fp32's normal numbers: below kLeastSum all of sixteen values are below
 // 2^-45, and 2^100 times them have squares within the normal numbers, down to the smallest values that there are.  Read a
 // second time: what every gradient passes keeps its loads together (with the choice in place, 3 x 45 M fp32 gradients took
-// 84 us in the place of 80, bf16 48 for 42.5).
+// 84 us in the place of 80, bf16 48 for 42.5; gradients of nothing but zeros, which all come here, take 95).
 constexpr float kLeastSum = 0x1p-90f;
 template <typename T>
 __device__ __forceinline__ double sum_squares_again(const T* p, bool vector, int size) {

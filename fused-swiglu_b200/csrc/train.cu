@@ -240,9 +240,10 @@ int launch_norm_forward(NormForwardParams& p, bool wide, const Device& dev, cuda
 }
 
 // Little work: one cluster, whose blocks join their sums over rows themselves, takes the place of a grid over all SMs and a
-// second launch.  Layer norm, bf16, a call / in a graph, us, with two launches in brackets: 64 x 128 6.5 / 3.1 (8.3 / 3.4), 128 x 256
-// 6.4 / 3.5 (8.3 / 4.0), 32 x 1024 6.6 / 3.9 (8.6 / 4.2), 8 x 4096 6.7 / 5.3 (8.5 / 4.3); above, graphs lose more than calls gain:
-// 512 x 128 6.6 / 4.6 (8.5 / 3.8), 64 x 1003 7.0 / 6.6 (8.4 / 4.6), 8 x 8192 7.9 / 7.5 (8.5 / 6.7).
+// second launch.  Layer norm, bf16, a call / in a graph, us, with two launches in brackets: 64 x 128 6.7 / 3.3 (9.2 / 3.9), 128 x 256
+// 6.9 / 3.7 (9.5 / 4.3), 32 x 1024 7.0 / 4.1 (9.5 / 5.1), 32 x 1003 6.9 / 5.7 (9.6 / 5.7).  Of rows of 4096 columns and more a call
+// gains but a graph loses: 8 x 4096 7.0 / 5.9 (9.6 / 4.9), 4 x 8192 7.9 / 7.8 (9.3 / 7.4).  More values, and graphs lose as much as
+// calls gain: 512 x 128 6.6 / 4.6 (8.5 / 3.8), 64 x 1003 7.0 / 6.6 (8.4 / 4.6), 8 x 8192 7.9 / 7.5 (8.5 / 6.7).
 constexpr int64_t kFewValues = 1 << 15;
 bool few_values(const NormBackwardParams& p) { return p.partial != nullptr && static_cast<int64_t>(p.M) * p.d <= kFewValues; }
 int backward_splits(const NormBackwardParams& p, int64_t blocks, int64_t most) {
@@ -620,7 +621,7 @@ int grad_norm_launches(const fswiglu_grad_tensor* tensors, int64_t count, double
 }
 
 // Up to this many chunks a launch of one cluster takes the place of one over all SMs and another that joins: 16 chunks of one
-// tensor 5.0 us a call (6.6 with two launches) and 2.5 to 3.2 us in a graph (3.2 to 3.5); 24 chunks 5.0 (6.5) and 3.0 to 3.9 (3.3 to
+// tensor 5.0 us a call (6.6 with two launches) and 2.7 to 3.4 us in a graph (3.2 to 3.5); 24 chunks 5.0 (6.5) and 3.0 to 3.9 (3.3 to
 // 3.6); 48 chunks 6.8 (6.5) and 6.2 (3.6) in fp32.
 constexpr int64_t kFewChunks = 24;
 static_assert(kFewChunks <= kSmallTable, "a tensor has a chunk at least");

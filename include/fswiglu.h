@@ -236,7 +236,8 @@ int fswiglu_transpose_bf16(const void* src, int64_t ld_src, void* dst, int64_t l
  *     z = (x - mean) rstd      y = z w + b      rstd = 1 / sqrt(mean((x - mean)^2) + eps)      (RMS norm: mean = 0)
  *
  * x, y [M, d] of x_dtype, weight and bias [d] of w_dtype (NULL: ones and zeros), mean and rstd [M] fp32: what the
- * backward pass needs.  1 <= d <= 2^24; M == 0 is a no-op.  rstd of the RMS form is fswiglu_rms_scale_f32's.
+ * backward pass needs.  1 <= d <= 2^24; M == 0 is a no-op.  rstd of the RMS form is fswiglu_rms_scale_f32's.  A row
+ * whose squares' sum passes fp32's range (values from about 1e18 on) has rstd 0.
  */
 int fswiglu_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, void* y,
                                int64_t ldy, float* mean, float* rstd, int64_t M, int64_t d, int x_dtype,
@@ -280,7 +281,8 @@ int fswiglu_rms_norm_backward(const void* dout, int64_t ld_dout, const void* x, 
  *       gives the same bits.  A second moment above zero is kept above zero.  A block with a moment that is not
  *       finite gets NaN for its scale.
  * The tensors are described in host memory, which the call has read when it returns (it may be freed then); the
- * launches carry the pointers, so that a captured graph needs nothing but the tensors themselves.  No two tensors
+ * launches carry the pointers, so that a captured graph needs nothing but the tensors themselves.  Under the root a
+ * second moment below the smallest normal fp32 number counts as that.  No two tensors
  * may share parameters, masters, moments or scales (checked among each kind: FSWIGLU_ERR_BAD_ARG).
  * Options: lr_device (fp32) and step_device (int64, >= 1), where not NULL, are read on the device in the place of lr
  * and step, so that a captured graph can be replayed with other values.  grad_scale (fp32, NULL: 1) is read on the

@@ -29,15 +29,11 @@ def _lib():
     return fused_mlp_module
 
 
-def _traced(x: torch.Tensor) -> bool:
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or type(x) not in (torch.Tensor, torch.nn.Parameter))
-
-
 def _norms(x: torch.Tensor):
     """The module's functions; where x is traced or has shapes alone, the dispatcher's ops, which have forms for that."""
     lib = _lib()  # registers the ops
-    return torch.ops.ASMLLM if _traced(x) or x.device.type == "meta" else lib
+    plain = type(x) in (torch.Tensor, torch.nn.Parameter) and x.device.type != "meta"
+    return lib if plain and not torch.compiler.is_compiling() and not torch._C._len_torch_dispatch_stack() else torch.ops.ASMLLM
 
 
 def _rows(x: torch.Tensor, d: int) -> torch.Tensor:
@@ -148,8 +144,6 @@ def norm_swiglu_block(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: tor
     args = (x, norm_weight, norm_bias, W_gate, W_up, W_down, eps, norm == "layer")
     if torch.compiler.is_compiling():
         return _block_as_it_is(*args)
-    if _traced(x):
-        raise RuntimeError("norm_swiglu_block cannot be traced: its backward pass has no shape-only form")
     return _NormSwiGLUBlock.apply(*args)
 
 

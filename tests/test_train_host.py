@@ -208,7 +208,7 @@ def test_norms_can_be_traced():
         w = torch.empty(64, device="cuda")
         for y in (train.rms_norm(x, w), train.layer_norm(x, w, w), train.layer_norm(x)):
             assert y.shape == x.shape and y.dtype == x.dtype and y.device.type == "cuda"
-        with pytest.raises(RuntimeError, match="cannot be traced"):
+        with pytest.raises(RuntimeError, match="has no data"):
             train.norm_swiglu_block(x, None, None, x[0], x[0], x[0])
     x, w = torch.empty((3, 8, 64), device="meta", requires_grad=True), torch.empty(64, device="meta", requires_grad=True)
     train.layer_norm(train.rms_norm(x, w), w, w).sum().backward()
@@ -221,6 +221,19 @@ def test_norms_can_be_traced():
         torch._dynamo.reset()
         with pytest.raises(NotImplementedError, match="'CPU' backend"):
             call()
+
+
+def test_a_dispatch_mode_alone_is_no_tracing():
+    """Counters of operations and selective checkpointing watch what real tensors do: the block is called as without them."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    with Watch(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        train.norm_swiglu_block(x, None, None, x, x, x)
 
 
 # ---------------------------------------------------------------- the optimiser, with the operators recorded

@@ -646,6 +646,27 @@ def test_a_thread_keeps_its_context_and_gets_one_when_it_has_none(fsw, cuda_dev)
     assert seen == [True] * 4, seen
 
 
+def test_norms_and_block_under_a_dispatch_mode(fsw, cuda_dev):
+    """What watches operations, as counters of them do, changes no bits."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    def both_passes():
+        ts = [None if t is None else t.requires_grad_() for t in block_inputs(33, 72, 136, cuda_dev, 4, "layer")]
+        y = fsw.train.norm_swiglu_block(*ts, norm="layer")
+        z = fsw.train.rms_norm(fsw.train.layer_norm(y, ts[1], ts[2]), ts[1])
+        z.backward(torch.ones_like(z))
+        return [z.detach()] + [t.grad for t in ts]
+
+    want = both_passes()
+    with Watch():
+        got = both_passes()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_compiled_norms_and_a_block_between_compiled_parts(fsw, cuda_dev):
     """The norms inside a compiled function without a graph break, the block where torch.compile leaves its graph: the bits of the
     eager calls, forward and backward."""

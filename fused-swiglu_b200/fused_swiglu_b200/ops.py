@@ -36,6 +36,9 @@ def _require_bf16_cuda(**tensors: torch.Tensor) -> None:
             raise RuntimeError(f"{name} must be a bfloat16 tensor, got {t.dtype}")
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor (no CPU path exists)")
+        # a fake tensor calls itself a CUDA tensor, and as its address gives its offset from nothing
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) and t.numel() > 0 and t.untyped_storage().data_ptr() == 0:
+            raise RuntimeError(f"{name} has no data: traced tensors go through torch.ops.ASMLLM")
 
 
 def _row_major_ld(name: str, t: torch.Tensor) -> int:

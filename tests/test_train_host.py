@@ -181,6 +181,20 @@ def test_operators_refuse_tensors_without_data():
                 call()
 
 
+def test_host_layer_refuses_tensors_without_data():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from fused_swiglu_b200 import ops
+
+    with FakeTensorMode():
+        bf = dict(dtype=torch.bfloat16, device="cuda")
+        x, mats, wd = torch.empty((6, 64), **bf)[1:], torch.empty((65, 64), **bf)[1:], torch.empty((65, 64), **bf)[1:]
+        for call in (lambda: ops.rms_scale(x), lambda: ops.fused_swiglu_gateup_bf16(x, mats, mats), lambda: ops.swiglu_down_bf16(x, wd),
+                     lambda: ops.fused_swiglu_mlp_bf16(x, mats, mats, wd), lambda: ops.swiglu_mlp_backward(x, mats, mats, wd, x)):
+            with pytest.raises(RuntimeError, match="has no data"):
+                call()
+
+
 def test_shapes_without_data():
     import fused_mlp_module  # noqa: F401
 
